@@ -35,6 +35,10 @@ FLAG_DECODE_B_KEPT = 16384
 FLAG_QKV_WEIGHTS_BF16 = 1  # of the two QKV stage problems
 FLAG_GQ_DIRECT = 1  # mi355_w8a8_gq_problem.flags
 FLAG_GQ_BF16_SCALES = 2  # mi355_w8a8_gq_bwd_problem.flags
+FLAG_BF16_GROUPED_DW_F32 = 1  # mi355_w8a8_bf16_grouped_bwd_problem.flags
+FLAG_EMBEDDING_F32 = 1        # mi355_w8a8_embedding_problem.flags
+FLAG_EMBEDDING_IDS64 = 2
+GRAD_BF16, GRAD_F32 = 0, 1    # mi355_w8a8_grad_tensor.type
 STATIC_WORKSPACE_BYTES = 32 << 20
 PATH_NAMES = {1: "skinny", 2: "skinny-chunks", 3: "tiled-256x128", 4: "tiled-256x256", 5: "tiled-128x128",
               6: "tiled-256x128-pair"}
@@ -63,8 +67,13 @@ EXPORTS = (
     "mi355_w8a8_forward_path", "mi355_w8a8_calibrate_operand_bytes", "mi355_w8a8_calibrate_mfma_ops", "mi355_w8a8_calibrate_mfma_v1",
     "mi355_w8a8_calibrate_read_v1", "mi355_w8a8_calibrate_copy_v1",
 )
-# called by the torch mirror alone (csrc/w8a8_gq_bwd_api.h)
-PRIVATE_EXPORTS = ("mi355_w8a8_gq_bwd_workspace_bytes", "mi355_w8a8_gq_linear_bwd_v1")
+# called by the torch mirror alone (csrc/w8a8_gq_bwd_api.h, csrc/bf16_api.h)
+PRIVATE_EXPORTS = (
+    "mi355_w8a8_gq_bwd_workspace_bytes", "mi355_w8a8_gq_linear_bwd_v1",
+    "mi355_w8a8_bf16_grouped_v1", "mi355_w8a8_bf16_grouped_bwd_v1",
+    "mi355_w8a8_embedding_v1", "mi355_w8a8_embedding_bwd_workspace_bytes", "mi355_w8a8_embedding_bwd_v1",
+    "mi355_w8a8_grad_workspace_bytes", "mi355_w8a8_grad_norm_v1", "mi355_w8a8_grad_clip_v1",
+)
 
 _u32, _u64, _vp, _f32 = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p, ctypes.c_float
 
@@ -216,6 +225,41 @@ class GqBwdProblem(ctypes.Structure):
     ]
 
 
+class Bf16GroupedProblem(ctypes.Structure):
+    """struct mi355_w8a8_bf16_grouped_problem"""
+
+    _fields_ = [
+        ("struct_size", _u32), ("flags", _u32), ("m", _u32), ("k", _u32), ("n", _u32), ("n_groups", _u32),
+        ("x", _vp), ("weight", _vp), ("group_sizes", _vp), ("out", _vp),
+    ]
+
+
+class Bf16GroupedBwdProblem(ctypes.Structure):
+    """struct mi355_w8a8_bf16_grouped_bwd_problem"""
+
+    _fields_ = [
+        ("struct_size", _u32), ("flags", _u32), ("m", _u32), ("k", _u32), ("n", _u32), ("n_groups", _u32),
+        ("x", _vp), ("dy", _vp), ("weight", _vp), ("group_sizes", _vp), ("dx", _vp), ("dw", _vp),
+    ]
+
+
+class EmbeddingProblem(ctypes.Structure):
+    """struct mi355_w8a8_embedding_problem"""
+
+    _fields_ = [
+        ("struct_size", _u32), ("flags", _u32), ("n_tokens", _u32), ("vocab", _u32), ("width", _u32),
+        ("n_adapters", _u32), ("scale", _f32), ("reserved", _u32),
+        ("table", _vp), ("d_out", _vp), ("ids", _vp), ("adapter_indices", _vp), ("scales", _vp), ("out", _vp),
+        ("workspace", _vp), ("workspace_bytes", _u64),
+    ]
+
+
+class GradTensor(ctypes.Structure):
+    """struct mi355_w8a8_grad_tensor"""
+
+    _fields_ = [("grad", _vp), ("out", _vp), ("count", _u64), ("type", _u32), ("reserved", _u32)]
+
+
 class NativeError(RuntimeError):
     def __init__(self, fn: str, status: int, detail: str):
         super().__init__(f"{fn} failed: {STATUS.get(status, status)} ({detail})")
@@ -311,6 +355,19 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mi355_w8a8_swiglu_bwd_v1.argtypes = (_vp, _vp, _vp, _u32, _u32, _vp)
     lib.mi355_w8a8_rms_norm_bwd_v1.restype = ctypes.c_int
     lib.mi355_w8a8_rms_norm_bwd_v1.argtypes = (_vp, _vp, _vp, _vp, _u32, _u32, _f32, _vp)
+    for name, struct in (("bf16_grouped", Bf16GroupedProblem), ("bf16_grouped_bwd", Bf16GroupedBwdProblem),
+                         ("embedding", EmbeddingProblem), ("embedding_bwd", EmbeddingProblem)):
+        fn = getattr(lib, f"mi355_w8a8_{name}_v1")
+        fn.restype = ctypes.c_int
+        fn.argtypes = (ctypes.POINTER(struct), _vp)
+    lib.mi355_w8a8_embedding_bwd_workspace_bytes.restype = _u64
+    lib.mi355_w8a8_embedding_bwd_workspace_bytes.argtypes = (_u32,) * 5
+    lib.mi355_w8a8_grad_workspace_bytes.restype = _u64
+    lib.mi355_w8a8_grad_workspace_bytes.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32)
+    lib.mi355_w8a8_grad_norm_v1.restype = ctypes.c_int
+    lib.mi355_w8a8_grad_norm_v1.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32, _vp, _vp, _u64, _vp)
+    lib.mi355_w8a8_grad_clip_v1.restype = ctypes.c_int
+    lib.mi355_w8a8_grad_clip_v1.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32, _vp, _vp, _vp, _u64, _vp)
 
 
 def load() -> ctypes.CDLL:

@@ -1,6 +1,6 @@
 """Builds the gfx950 shared library of the W8A8 LoRA linear path with hipcc.
 
-``python build.py`` compiles ``csrc/w8a8_api.hip`` into ``lib/libmi355_w8a8.so`` and, with g++,
+``python build.py`` compiles ``csrc/w8a8_api.hip`` and ``csrc/bf16_api.hip`` into ``lib/libmi355_w8a8.so`` and, with g++,
 ``csrc/w8a8_host_call.cc`` into the Python module ``lib/mi355_w8a8_host.so``.
 hipcc cross-compiles without a GPU.  Flags: ``-ffp-contract=off -fno-fast-math`` keep
 the quantizer and the float32 epilogue bit-exact (no fused multiply-add, IEEE
@@ -9,6 +9,7 @@ division and square root); packed FP32 instructions are disabled.
 
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -20,6 +21,8 @@ CSRC = HERE / "csrc"
 LIB_DIR = HERE / "lib"
 LIB_PATH = LIB_DIR / "libmi355_w8a8.so"
 HOST_PATH = LIB_DIR / "mi355_w8a8_host.so"
+
+SOURCES = ("w8a8_api.hip", "bf16_api.hip")  # compiled side by side, then linked
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
@@ -94,17 +97,30 @@ def build_host(verbose: bool = False) -> Path:
     return HOST_PATH
 
 
-def build(verbose: bool = False) -> Path:
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB_DIR / "libmi355_w8a8.so.tmp"
-    cmd = [find_hipcc(), *HIPCC_FLAGS, str(CSRC / "w8a8_api.hip"), "-o", str(tmp)]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+def compile_source(source: Path, verbose: bool = False) -> Path:
+    obj = LIB_DIR / (source.stem + ".o")
+    run_hipcc([*(f for f in HIPCC_FLAGS if f != "-shared" and not f.startswith("-Wl,")), "-c", str(source), "-o", str(obj)], verbose)
+    return obj
+
+
+def run_hipcc(args: list[str], verbose: bool) -> None:
+    proc = subprocess.run([find_hipcc(), *args], capture_output=True, text=True)
     noise = "packed-fp32-ops"
     err = "\n".join(l for l in proc.stderr.splitlines() if noise not in l)
     if proc.returncode != 0:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{err}")
     if verbose and err.strip():
         print(err, file=sys.stderr)
+
+
+def build(verbose: bool = False) -> Path:
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = LIB_DIR / "libmi355_w8a8.so.tmp"
+    with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = list(pool.map(lambda name: compile_source(CSRC / name, verbose), SOURCES))
+    run_hipcc([*HIPCC_FLAGS, *map(str, objects), "-o", str(tmp)], verbose)
+    for obj in objects:
+        obj.unlink()
     os.replace(tmp, LIB_PATH)
     try:
         build_host(verbose)

@@ -1,0 +1,400 @@
+// C ABI of the operators beside the quantized path: products grouped by expert in bf16, embedding rows and their gradient,
+// the norm and the clipping of adapter gradients.  Argument validation, workspace carving and kernel launches; nothing
+// here synchronises, allocates or keeps state.
+#include "bf16_api.h"
+
+#include <hip/hip_runtime.h>
+
+#include "bf16_grouped.h"
+#include "embedding.h"
+#include "grad_clip.h"
+
+using namespace w8a8;
+
+namespace {
+
+constexpr uint32_t kMaxRows = 1u << 20;
+
+inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }
+inline bool overlaps(const void* a, uint64_t an, const void* b, uint64_t bn) {
+  if (!a || !b || an == 0 || bn == 0) return false;
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  return a0 < b0 + bn && b0 < a0 + an;
+}
+inline int launch_status() { return hipGetLastError() == hipSuccess ? MI355_W8A8_OK : MI355_W8A8_ERR_LAUNCH; }
+inline uint64_t align256(uint64_t v) { return (v + 255u) & ~uint64_t(255); }
+template <class K>
+inline bool allow_lds(K kernel, uint32_t bytes) {
+  return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
+}
+
+// ---- products grouped by expert --------------------------------------------------------------------------------------
+
+int check_grouped_dims(uint32_t m, uint32_t k, uint32_t n, uint32_t groups) {
+  if (m == 0 || k == 0 || n == 0 || groups == 0) return MI355_W8A8_ERR_SHAPE;
+  if ((k & 7u) || (n & 7u)) return MI355_W8A8_ERR_UNSUPPORTED;
+  // (a tile's offsets are 32 bits wide: 256 rows of either operand stay below 2^31 bytes)
+  if (m > kMaxRows || k > MI355_W8A8_BF16_GROUPED_MAX_FEATURES || n > MI355_W8A8_BF16_GROUPED_MAX_FEATURES || groups > kBgMaxGroups)
+    return MI355_W8A8_ERR_UNSUPPORTED;
+  return MI355_W8A8_OK;
+}
+
+// most row tiles that m rows in `groups` groups can make
+inline uint64_t most_row_tiles(uint32_t m, uint32_t groups, uint32_t tile) {
+  const uint32_t held = groups < m ? groups : m;
+  return (m + (uint64_t)(tile - 1u) * held) / tile;
+}
+
+template <int KIND>
+int launch_grouped(const BgArgs& g, hipStream_t s) {
+  constexpr int TM = 128, TN = 128, BK = 64, STAGES = 2;
+  auto kernel = &bf16_grouped_kernel<KIND, TM, TN, 2, 2, BK, STAGES>;
+  constexpr uint32_t kLds = (TM + TN) * BK * 2 * STAGES;
+  if (!allow_lds(kernel, kLds)) return MI355_W8A8_ERR_LAUNCH;
+  const uint64_t n_tiles = (g.cols + TN - 1u) / TN;
+  const uint64_t tiles = n_tiles * (KIND == kGroupedDw ? (uint64_t)g.groups * ((g.rows + TM - 1u) / TM) : most_row_tiles(g.m, g.groups + 1u, TM));
+  if (tiles > 0x7ffffff0u) return MI355_W8A8_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)((tiles + 7u) / 8u * 8u)), dim3(256), kLds, s, g);
+  return launch_status();
+}
+
+int run_grouped(const mi355_w8a8_bf16_grouped_problem* p, hipStream_t s) {
+  if (!p) return MI355_W8A8_ERR_NULL;
+  if (p->struct_size != sizeof(mi355_w8a8_bf16_grouped_problem)) return MI355_W8A8_ERR_STRUCT;
+  if (p->flags) return MI355_W8A8_ERR_SHAPE;
+  const int st = check_grouped_dims(p->m, p->k, p->n, p->n_groups);
+  if (st) return st;
+  if (!p->x || !p->weight || !p->group_sizes || !p->out) return MI355_W8A8_ERR_NULL;
+  if (!aligned(p->x, 16) || !aligned(p->weight, 16) || !aligned(p->out, 16) || !aligned(p->group_sizes, 4)) return MI355_W8A8_ERR_ALIGN;
+  const uint64_t out_bytes = (uint64_t)p->m * p->n * 2u;
+  if (overlaps(p->out, out_bytes, p->x, (uint64_t)p->m * p->k * 2u) ||
+      overlaps(p->out, out_bytes, p->weight, (uint64_t)p->n_groups * p->k * p->n * 2u) ||
+      overlaps(p->out, out_bytes, p->group_sizes, (uint64_t)p->n_groups * 4u))
+    return MI355_W8A8_ERR_ALIAS;
+  (void)hipGetLastError();
+  BgArgs g{};
+  g.a = static_cast<const uint16_t*>(p->x); g.b = static_cast<const uint16_t*>(p->weight);
+  g.sizes = p->group_sizes; g.out = p->out;
+  g.m = p->m; g.rows_ld = p->k; g.cols_ld = p->n; g.depth = p->k; g.cols = p->n; g.groups = p->n_groups;
+  g.b_group = (uint64_t)p->k * p->n;
+  return launch_grouped<kGroupedFwd>(g, s);
+}
+
+int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s) {
+  if (!p) return MI355_W8A8_ERR_NULL;
+  if (p->struct_size != sizeof(mi355_w8a8_bf16_grouped_bwd_problem)) return MI355_W8A8_ERR_STRUCT;
+  if (p->flags & ~MI355_W8A8_FLAG_BF16_GROUPED_DW_F32) return MI355_W8A8_ERR_SHAPE;
+  int st = check_grouped_dims(p->m, p->k, p->n, p->n_groups);
+  if (st) return st;
+  if (!p->dy || !p->group_sizes || (!p->dx && !p->dw)) return MI355_W8A8_ERR_NULL;
+  if ((p->dx && !p->weight) || (p->dw && !p->x)) return MI355_W8A8_ERR_NULL;
+  if (!aligned(p->x, 16) || !aligned(p->dy, 16) || !aligned(p->weight, 16) || !aligned(p->dx, 16) || !aligned(p->dw, 16) || !aligned(p->group_sizes, 4))
+    return MI355_W8A8_ERR_ALIGN;
+  const bool f32 = p->flags & MI355_W8A8_FLAG_BF16_GROUPED_DW_F32;
+  const uint64_t x_bytes = (uint64_t)p->m * p->k * 2u, dy_bytes = (uint64_t)p->m * p->n * 2u, sizes_bytes = (uint64_t)p->n_groups * 4u;
+  const uint64_t values = (uint64_t)p->n_groups * p->k * p->n, dw_bytes = values * (f32 ? 4u : 2u);
+  const void* outs[2] = {p->dx, p->dw};
+  const uint64_t bytes[2] = {x_bytes, dw_bytes};
+  for (int i = 0; i < 2; ++i) {
+    if (overlaps(outs[i], bytes[i], p->dy, dy_bytes) || overlaps(outs[i], bytes[i], p->x, x_bytes) ||
+        overlaps(outs[i], bytes[i], p->weight, values * 2u) || overlaps(outs[i], bytes[i], p->group_sizes, sizes_bytes))
+      return MI355_W8A8_ERR_ALIAS;
+  }
+  if (overlaps(p->dx, x_bytes, p->dw, dw_bytes)) return MI355_W8A8_ERR_ALIAS;
+  (void)hipGetLastError();
+  BgArgs g{};
+  g.sizes = p->group_sizes; g.m = p->m; g.groups = p->n_groups;
+  if (p->dx) {
+    g.a = static_cast<const uint16_t*>(p->dy); g.b = static_cast<const uint16_t*>(p->weight); g.out = p->dx;
+    g.rows_ld = p->n; g.cols_ld = p->n; g.depth = p->n; g.cols = p->k;
+    g.b_group = (uint64_t)p->k * p->n;
+    if ((st = launch_grouped<kGroupedDx>(g, s))) return st;
+  }
+  if (p->dw) {
+    g.a = static_cast<const uint16_t*>(p->x); g.b = static_cast<const uint16_t*>(p->dy); g.out = p->dw;
+    g.rows_ld = p->k; g.cols_ld = p->n; g.depth = 0; g.cols = p->n; g.rows = p->k; g.f32 = f32;
+    g.out_group = (uint64_t)p->k * p->n;
+    st = launch_grouped<kGroupedDw>(g, s);
+  }
+  return st;
+}
+
+// ---- embedding rows --------------------------------------------------------------------------------------------------
+
+int check_embedding(const mi355_w8a8_embedding_problem* p) {
+  if (!p) return MI355_W8A8_ERR_NULL;
+  if (p->struct_size != sizeof(mi355_w8a8_embedding_problem)) return MI355_W8A8_ERR_STRUCT;
+  if (p->flags & ~(MI355_W8A8_FLAG_EMBEDDING_F32 | MI355_W8A8_FLAG_EMBEDDING_IDS64)) return MI355_W8A8_ERR_SHAPE;
+  if (p->n_tokens == 0 || p->vocab == 0 || p->width == 0) return MI355_W8A8_ERR_SHAPE;
+  if (p->n_adapters == 0 && (p->adapter_indices || p->scales)) return MI355_W8A8_ERR_SHAPE;
+  if (p->n_adapters > 1 && !p->adapter_indices) return MI355_W8A8_ERR_NULL;
+  const uint64_t rows = (uint64_t)(p->n_adapters ? p->n_adapters : 1u) * p->vocab;
+  if (p->n_tokens > kMaxRows || p->width > MI355_W8A8_EMBEDDING_MAX_WIDTH || rows > MI355_W8A8_EMBEDDING_MAX_ROWS) return MI355_W8A8_ERR_UNSUPPORTED;
+  const uintptr_t id = p->flags & MI355_W8A8_FLAG_EMBEDDING_IDS64 ? 8 : 4;
+  if (!p->ids) return MI355_W8A8_ERR_NULL;
+  if (!aligned(p->ids, id) || !aligned(p->adapter_indices, 4) || !aligned(p->scales, 4)) return MI355_W8A8_ERR_ALIGN;
+  return MI355_W8A8_OK;
+}
+
+inline uint64_t embedding_rows(const mi355_w8a8_embedding_problem* p) { return (uint64_t)(p->n_adapters ? p->n_adapters : 1u) * p->vocab; }
+inline uint32_t value_bytes(const mi355_w8a8_embedding_problem* p) { return p->flags & MI355_W8A8_FLAG_EMBEDDING_F32 ? 4u : 2u; }
+inline bool overlaps_indices(const mi355_w8a8_embedding_problem* p, const void* out, uint64_t bytes) {
+  return overlaps(out, bytes, p->ids, (uint64_t)p->n_tokens * (p->flags & MI355_W8A8_FLAG_EMBEDDING_IDS64 ? 8u : 4u)) ||
+         overlaps(out, bytes, p->adapter_indices, (uint64_t)p->n_tokens * 4u) || overlaps(out, bytes, p->scales, (uint64_t)p->n_adapters * 4u);
+}
+
+EmbedArgs embed_args(const mi355_w8a8_embedding_problem* p) {
+  EmbedArgs e{};
+  e.table = p->table; e.out = p->out; e.dy = p->d_out; e.ids = p->ids; e.adapters = p->adapter_indices; e.scales = p->scales;
+  e.scale = p->scale; e.n = p->n_tokens; e.vocab = p->vocab; e.width = p->width; e.n_adapters = p->n_adapters ? p->n_adapters : 1u;
+  e.ids64 = (p->flags & MI355_W8A8_FLAG_EMBEDDING_IDS64) != 0;
+  return e;
+}
+inline uint32_t blocks_of(uint64_t threads) { return (uint32_t)((threads + 255u) / 256u); }
+
+int run_embedding(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
+  const int st = check_embedding(p);
+  if (st) return st;
+  if (!p->table || !p->out) return MI355_W8A8_ERR_NULL;
+  const uint32_t size = value_bytes(p);
+  if (!aligned(p->table, size) || !aligned(p->out, size)) return MI355_W8A8_ERR_ALIGN;
+  const uint64_t out_bytes = (uint64_t)p->n_tokens * p->width * size;
+  if (overlaps(p->out, out_bytes, p->table, embedding_rows(p) * p->width * size) || overlaps_indices(p, p->out, out_bytes)) return MI355_W8A8_ERR_ALIAS;
+  const EmbedArgs e = embed_args(p);
+  const bool wide = p->width % (16u / size) == 0 && aligned(p->table, 16) && aligned(p->out, 16);
+  const uint64_t threads = (uint64_t)p->n_tokens * (wide ? p->width / (16u / size) : p->width);
+  const dim3 grid(blocks_of(threads)), block(256);
+  (void)hipGetLastError();
+  if (size == 4u) {
+    if (wide) hipLaunchKernelGGL((embed_rows_kernel<float, 4>), grid, block, 0, s, e);
+    else hipLaunchKernelGGL((embed_rows_kernel<float, 1>), grid, block, 0, s, e);
+  } else {
+    if (wide) hipLaunchKernelGGL((embed_rows_kernel<uint16_t, 8>), grid, block, 0, s, e);
+    else hipLaunchKernelGGL((embed_rows_kernel<uint16_t, 1>), grid, block, 0, s, e);
+  }
+  return launch_status();
+}
+
+struct EmbedLayout {
+  uint32_t passes, bits, chunks, run, runs;
+  uint64_t keys[2], tokens[2], counts, parts, total;
+};
+
+// positions of a run: enough threads to fill the chip (2048 a CU) where the rows suffice, and no more parts than that
+EmbedLayout embed_layout(uint32_t n, uint64_t rows, uint32_t width, uint32_t flags) {
+  EmbedLayout L{};
+  uint32_t bits = 1;
+  while ((rows >> bits) != 0) ++bits;  // keys up to `rows` itself
+  L.passes = (bits + 10u) / 11u;
+  L.bits = (bits + L.passes - 1u) / L.passes;
+  L.chunks = (n + kEmbedChunk - 1u) / kEmbedChunk;
+  const uint32_t vec = flags & MI355_W8A8_FLAG_EMBEDDING_F32 ? 4u : 8u;
+  const uint64_t units = width % vec ? width : width / vec;
+  L.run = 8;
+  while (L.run < 256u && (uint64_t)n * units / (L.run * 2u) >= 524288u) L.run *= 2u;
+  L.runs = (n + L.run - 1u) / L.run;
+  uint64_t off = 0;
+  for (int i = 0; i < 2; ++i) {
+    L.keys[i] = off; off += align256((uint64_t)n * 4u);
+    L.tokens[i] = off; off += align256((uint64_t)n * 4u);
+  }
+  L.counts = off;
+  if (L.chunks > kEmbedSortChunks) off += align256(((uint64_t)L.chunks + 1u) * (4u << L.bits));
+  L.parts = off; off += align256((uint64_t)L.runs * 2u * width * 4u);
+  L.total = off;
+  return L;
+}
+
+template <typename T, int V>
+int launch_embed_sums(const EmbedSumArgs& a, hipStream_t s) {
+  const dim3 grid(blocks_of((uint64_t)a.runs * (a.e.width / V))), block(256);
+  hipLaunchKernelGGL((embed_sum_kernel<T, V>), grid, block, 0, s, a);
+  const int st = launch_status();
+  if (st || a.runs < 2u) return st;
+  hipLaunchKernelGGL((embed_join_kernel<T, V>), grid, block, 0, s, a);
+  return launch_status();
+}
+
+int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
+  int st = check_embedding(p);
+  if (st) return st;
+  if (!p->d_out || !p->out) return MI355_W8A8_ERR_NULL;
+  const uint32_t size = value_bytes(p);
+  if (!aligned(p->d_out, size) || !aligned(p->out, 16)) return MI355_W8A8_ERR_ALIGN;
+  const uint64_t rows = embedding_rows(p), out_bytes = rows * p->width * size, dy_bytes = (uint64_t)p->n_tokens * p->width * size;
+  const EmbedLayout L = embed_layout(p->n_tokens, rows, p->width, p->flags);
+  if (!p->workspace || p->workspace_bytes < L.total) return MI355_W8A8_ERR_WORKSPACE;
+  if (!aligned(p->workspace, 256)) return MI355_W8A8_ERR_ALIGN;
+  if (overlaps(p->out, out_bytes, p->d_out, dy_bytes) || overlaps_indices(p, p->out, out_bytes) || overlaps(p->out, out_bytes, p->workspace, L.total) ||
+      overlaps(p->workspace, L.total, p->d_out, dy_bytes) || overlaps_indices(p, p->workspace, L.total))
+    return MI355_W8A8_ERR_ALIAS;
+  unsigned char* ws = static_cast<unsigned char*>(p->workspace);
+  EmbedSortArgs a{};
+  a.e = embed_args(p);
+  a.digits = 1u << L.bits;
+  a.chunks = L.chunks;
+  a.counts = reinterpret_cast<uint32_t*>(ws + L.counts);
+  const uint32_t sort_lds = (2u * kEmbedDigits + 16u) * 4u + 16u * a.digits * 2u, place_lds = kEmbedDigits * 4u + 16u * a.digits * 2u;
+  if (!allow_lds(&embed_sort_kernel, sort_lds) || !allow_lds(&embed_place_kernel, place_lds)) return MI355_W8A8_ERR_LAUNCH;
+  // every pass clears its share of the gradient
+  const uint64_t pieces = out_bytes / 16u, share = pieces / L.passes;
+  (void)hipGetLastError();
+  for (uint32_t pass = 0; pass < L.passes; ++pass) {
+    a.keys = pass ? reinterpret_cast<uint32_t*>(ws + L.keys[(pass - 1u) & 1u]) : nullptr;
+    a.tokens = pass ? reinterpret_cast<uint32_t*>(ws + L.tokens[(pass - 1u) & 1u]) : nullptr;
+    a.keys_out = reinterpret_cast<uint32_t*>(ws + L.keys[pass & 1u]);
+    a.tokens_out = reinterpret_cast<uint32_t*>(ws + L.tokens[pass & 1u]);
+    a.shift = pass * L.bits;
+    const bool last = pass + 1u == L.passes;
+    a.clear = static_cast<uint4*>(p->out) + pass * share;
+    a.clear_pieces = last ? pieces - pass * share : share;
+    a.clear_rest = last ? (uint32_t)(out_bytes % 16u) : 0u;
+    const uint64_t wanted = (a.clear_pieces + 4095u) / 4096u + 1u;
+    const uint32_t clearing = (uint32_t)(wanted < 2048u ? wanted : 2048u);
+    if (L.chunks <= kEmbedSortChunks) {
+      hipLaunchKernelGGL(embed_sort_kernel, dim3(L.chunks + clearing), dim3(1024), sort_lds, s, a);
+      if ((st = launch_status())) return st;
+      continue;
+    }
+    hipLaunchKernelGGL(embed_count_kernel, dim3(L.chunks + clearing), dim3(1024), 0, s, a);
+    if ((st = launch_status())) return st;
+    hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, s, a);
+    if ((st = launch_status())) return st;
+    hipLaunchKernelGGL(embed_place_kernel, dim3(L.chunks), dim3(1024), place_lds, s, a);
+    if ((st = launch_status())) return st;
+  }
+  EmbedSumArgs b{};
+  b.e = a.e;
+  b.keys = a.keys_out; b.tokens = a.tokens_out;
+  b.parts = reinterpret_cast<float*>(ws + L.parts);
+  b.run = L.run; b.runs = L.runs;
+  const bool wide = p->width % (16u / size) == 0 && aligned(p->d_out, 16);
+  if (size == 4u) return wide ? launch_embed_sums<float, 4>(b, s) : launch_embed_sums<float, 1>(b, s);
+  return wide ? launch_embed_sums<uint16_t, 8>(b, s) : launch_embed_sums<uint16_t, 1>(b, s);
+}
+
+// ---- gradient norms and clipping -------------------------------------------------------------------------------------
+
+// values of a piece: 64 KiB of bf16, more where an adapter's parts would be more than 2048 (every workgroup of the scaling reads them all)
+uint32_t grad_piece_values(const mi355_w8a8_grad_tensor* t, uint32_t n) {
+  uint64_t values = 0;
+  for (uint32_t i = 0; i < n; ++i) values += t[i].count;
+  uint32_t piece = 32768u;
+  while (values / piece > 2048u && piece < (1u << 28)) piece *= 2u;
+  return piece;
+}
+inline uint64_t pieces_of(uint64_t count, uint32_t piece) { return (count + piece - 1u) / piece; }
+
+int check_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const float* norms, bool scale) {
+  if (!t || !norms) return MI355_W8A8_ERR_NULL;
+  if (n == 0 || adapters == 0) return MI355_W8A8_ERR_SHAPE;
+  if (n > MI355_W8A8_GRAD_MAX_TENSORS || adapters > 65535u) return MI355_W8A8_ERR_UNSUPPORTED;
+  if (!aligned(norms, 4)) return MI355_W8A8_ERR_ALIGN;
+  for (uint32_t i = 0; i < n; ++i) {
+    if (t[i].type > MI355_W8A8_GRAD_F32 || t[i].reserved) return MI355_W8A8_ERR_SHAPE;
+    if (t[i].count == 0) continue;
+    if (t[i].count > (1ull << 40) / adapters) return MI355_W8A8_ERR_UNSUPPORTED;
+    if (!t[i].grad || (scale && !t[i].out)) return MI355_W8A8_ERR_NULL;
+    const uint32_t size = t[i].type == MI355_W8A8_GRAD_F32 ? 4u : 2u;
+    if (!aligned(t[i].grad, size) || (scale && !aligned(t[i].out, size))) return MI355_W8A8_ERR_ALIGN;
+    const uint64_t bytes = t[i].count * adapters * size;
+    if (overlaps(norms, adapters * 4ull, t[i].grad, bytes) || (scale && overlaps(norms, adapters * 4ull, t[i].out, bytes))) return MI355_W8A8_ERR_ALIAS;
+    if (scale && t[i].out != t[i].grad && overlaps(t[i].out, bytes, t[i].grad, bytes)) return MI355_W8A8_ERR_ALIAS;
+  }
+  return MI355_W8A8_OK;
+}
+
+int run_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const float* limits, float* norms, void* workspace, uint64_t workspace_bytes,
+              hipStream_t s, bool scale) {
+  int st = check_grads(t, n, adapters, norms, scale);
+  if (st) return st;
+  if (scale && !limits) return MI355_W8A8_ERR_NULL;
+  if (!aligned(limits, 4)) return MI355_W8A8_ERR_ALIGN;
+  const uint64_t need = mi355_w8a8_grad_workspace_bytes(t, n, adapters);
+  if (need == 0) return MI355_W8A8_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < need) return MI355_W8A8_ERR_WORKSPACE;
+  if (!aligned(workspace, 256)) return MI355_W8A8_ERR_ALIGN;
+  if (overlaps(workspace, need, norms, adapters * 4ull) || overlaps(workspace, need, limits, adapters * 4ull) ||
+      overlaps(norms, adapters * 4ull, limits, limits ? adapters * 4ull : 0ull))
+    return MI355_W8A8_ERR_ALIAS;
+  for (uint32_t i = 0; i < n; ++i) {
+    const uint64_t bytes = t[i].count * adapters * (t[i].type == MI355_W8A8_GRAD_F32 ? 4u : 2u);
+    if (overlaps(workspace, need, t[i].grad, bytes) ||
+        (scale && (overlaps(workspace, need, t[i].out, bytes) || overlaps(limits, adapters * 4ull, t[i].out, bytes))))
+      return MI355_W8A8_ERR_ALIAS;
+  }
+  GradArgs a{};
+  a.parts = static_cast<double*>(workspace);
+  a.limits = scale ? limits : nullptr;
+  a.norms = norms;
+  a.piece = grad_piece_values(t, n);
+  uint64_t total = 0;
+  for (uint32_t i = 0; i < n; ++i) total += pieces_of(t[i].count, a.piece);
+  a.parts_ld = a.parts_used = (uint32_t)total;
+  (void)hipGetLastError();
+  if (total == 0) {  // no values: the norms are zero
+    a.pieces = 0;
+    hipLaunchKernelGGL(grad_zero_norms_kernel, dim3((adapters + 255u) / 256u), dim3(256), 0, s, norms, adapters);
+    return launch_status();
+  }
+  for (int phase = 0; phase < 2; ++phase) {
+    uint32_t i = 0, part = 0;
+    while (i < n) {
+      a.tensors = a.pieces = 0;
+      a.part0 = part;
+      for (; i < n && a.tensors < kGradTable; ++i) {
+        if (t[i].count == 0) continue;
+        a.tensor[a.tensors++] = GradTensor{t[i].grad, t[i].out, t[i].count, a.pieces, t[i].type == MI355_W8A8_GRAD_F32};
+        a.pieces += (uint32_t)pieces_of(t[i].count, a.piece);
+      }
+      if (a.pieces == 0) break;
+      part += a.pieces;
+      if (phase == 0) hipLaunchKernelGGL(grad_norm_kernel, dim3(a.pieces, adapters), dim3(256), 0, s, a);
+      else if (scale || a.part0 == 0) hipLaunchKernelGGL(grad_scale_kernel, dim3(scale ? a.pieces : 1u, adapters), dim3(256), 0, s, a);
+      if ((st = launch_status())) return st;
+    }
+  }
+  return MI355_W8A8_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi355_w8a8_bf16_grouped_v1(const mi355_w8a8_bf16_grouped_problem* problem, void* stream) {
+  return run_grouped(problem, static_cast<hipStream_t>(stream));
+}
+int mi355_w8a8_bf16_grouped_bwd_v1(const mi355_w8a8_bf16_grouped_bwd_problem* problem, void* stream) {
+  return run_grouped_bwd(problem, static_cast<hipStream_t>(stream));
+}
+int mi355_w8a8_embedding_v1(const mi355_w8a8_embedding_problem* problem, void* stream) {
+  return run_embedding(problem, static_cast<hipStream_t>(stream));
+}
+uint64_t mi355_w8a8_embedding_bwd_workspace_bytes(uint32_t n_tokens, uint32_t vocab, uint32_t width, uint32_t n_adapters, uint32_t flags) {
+  const uint64_t rows = (uint64_t)(n_adapters ? n_adapters : 1u) * vocab;
+  if (n_tokens == 0 || rows == 0 || width == 0 || n_tokens > kMaxRows || width > MI355_W8A8_EMBEDDING_MAX_WIDTH || rows > MI355_W8A8_EMBEDDING_MAX_ROWS)
+    return 0;
+  return embed_layout(n_tokens, rows, width, flags).total;
+}
+int mi355_w8a8_embedding_bwd_v1(const mi355_w8a8_embedding_problem* problem, void* stream) {
+  return run_embedding_bwd(problem, static_cast<hipStream_t>(stream));
+}
+uint64_t mi355_w8a8_grad_workspace_bytes(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters) {
+  if (!tensors || n_tensors == 0 || n_tensors > MI355_W8A8_GRAD_MAX_TENSORS || n_adapters == 0 || n_adapters > 65535u) return 0;
+  for (uint32_t i = 0; i < n_tensors; ++i)
+    if (tensors[i].count > (1ull << 40) / n_adapters) return 0;
+  const uint32_t piece = grad_piece_values(tensors, n_tensors);
+  uint64_t pieces = 0;
+  for (uint32_t i = 0; i < n_tensors; ++i) pieces += pieces_of(tensors[i].count, piece);
+  return pieces > 0x7fffffffu ? 0u : align256((pieces ? pieces : 1u) * n_adapters * 8u);
+}
+int mi355_w8a8_grad_norm_v1(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters, float* norms, void* workspace,
+                            uint64_t workspace_bytes, void* stream) {
+  return run_grads(tensors, n_tensors, n_adapters, nullptr, norms, workspace, workspace_bytes, static_cast<hipStream_t>(stream), false);
+}
+int mi355_w8a8_grad_clip_v1(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters, const float* limits, float* norms,
+                            void* workspace, uint64_t workspace_bytes, void* stream) {
+  return run_grads(tensors, n_tensors, n_adapters, limits, norms, workspace, workspace_bytes, static_cast<hipStream_t>(stream), true);
+}
+
+}  // extern "C"

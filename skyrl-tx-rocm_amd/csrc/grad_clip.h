@@ -1,0 +1,178 @@
+// The global norm over many gradient tensors, one for each adapter (the leading axis of every tensor), and the gradients scaled
+// down to that adapter's limit:
+//
+//   norm[a] = sqrt(sum over tensors and their elements of adapter a of g^2)
+//   out     = g * (norm[a] > limit[a] ? limit[a] / norm[a] : 1)
+//
+// Bound by memory: the gradients are read twice (the norm has to be known before the first value can be written) and written once.
+// Squares and sums are double: a square of a float32 is exact there and neither over- nor underflows, and the parts are added in
+// one order, so the same gradients give the same bits.
+//
+//   grad_norm_kernel   a workgroup per piece of one tensor's adapter: the sum of its squares
+//   grad_scale_kernel  a workgroup per piece: the parts of its adapter added up, then the piece scaled
+//
+// The tensors come in the kernels' arguments, kGradTable to a launch: no table in device memory that a captured graph could find
+// overwritten, no copy.
+#pragma once
+#include "w8a8_device.h"
+
+namespace w8a8 {
+
+constexpr uint32_t kGradTable = 120;
+
+struct GradTensor {
+  const void* grad;
+  void* out;
+  uint64_t count;         // values of one adapter
+  uint32_t first_piece;   // among the launch's pieces of one adapter
+  uint32_t f32;
+};
+struct GradArgs {
+  GradTensor tensor[kGradTable];
+  double* parts;          // [adapters][parts_ld]
+  const float* limits;    // [adapters]
+  float* norms;           // [adapters]
+  uint32_t tensors, pieces;        // of this launch, for one adapter
+  uint32_t part0, parts_ld, parts_used;  // first part of this launch; parts in all
+  uint32_t piece;         // values of a piece
+};
+
+struct GradPiece { const GradTensor* t; uint64_t at; uint32_t count; };  // at: first value, in the whole tensor
+
+__device__ inline GradPiece grad_piece(const GradArgs& a, uint32_t adapter, uint32_t piece) {
+  uint32_t lo = 0, hi = a.tensors;  // the last tensor whose first piece is not behind this one
+  while (hi - lo > 1u) {
+    const uint32_t mid = (lo + hi) / 2u;
+    if (a.tensor[mid].first_piece <= piece) lo = mid; else hi = mid;
+  }
+  GradPiece p;
+  p.t = &a.tensor[lo];
+  const uint64_t from = (uint64_t)(piece - p.t->first_piece) * a.piece, left = p.t->count - from;
+  p.at = adapter * p.t->count + from;
+  p.count = left < a.piece ? (uint32_t)left : a.piece;
+  return p;
+}
+
+// f(index, 16 bytes' values, how many): the piece in whole 16-byte units behind the values in front of the first one
+template <typename T> struct GradUnit;
+template <> struct GradUnit<uint16_t> {
+  static constexpr uint32_t kN = 8;
+  static __device__ inline float one(uint16_t v) { return bf16_bits_to_f32(v); }
+  static __device__ inline uint16_t back(float v) { return (uint16_t)f32_to_bf16_bits(v); }
+  static __device__ inline void open(const uint4& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ inline uint4 close(const float (&f)[8]) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+};
+template <> struct GradUnit<float> {
+  static constexpr uint32_t kN = 4;
+  static __device__ inline float one(float v) { return v; }
+  static __device__ inline float back(float v) { return v; }
+  static __device__ inline void open(const uint4& r, float (&f)[4]) {
+    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+  }
+  static __device__ inline uint4 close(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+
+template <typename T>
+__device__ inline double grad_squares(const GradPiece& p) {
+  constexpr uint32_t N = GradUnit<T>::kN;
+  const T* g = static_cast<const T*>(p.t->grad) + p.at;
+  const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T);
+  const uint32_t head = off ? (N - off < p.count ? N - off : p.count) : 0u, units = (p.count - head) / N;
+  double sum = 0.0;
+  auto add = [&](float v) { sum += (double)v * (double)v; };
+  if (threadIdx.x < head) add(GradUnit<T>::one(g[threadIdx.x]));
+  const uint4* u = reinterpret_cast<const uint4*>(g + head);
+  for (uint32_t i = threadIdx.x; i < units; i += 1024u) {
+    uint4 r[4];
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) r[x] = i + x * 256u < units ? u[i + x * 256u] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) {
+      float f[N];
+      GradUnit<T>::open(r[x], f);
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) add(f[j]);
+    }
+  }
+  const uint32_t done = head + units * N;
+  if (threadIdx.x < p.count - done) add(GradUnit<T>::one(g[done + threadIdx.x]));
+  return sum;
+}
+
+__device__ inline double grad_block_sum(double v) {
+  __shared__ double waves[4];
+  v = wave_sum(v);
+  if ((threadIdx.x & 63u) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  const double s = (waves[0] + waves[1]) + (waves[2] + waves[3]);
+  __syncthreads();
+  return s;
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
+  const uint32_t adapter = blockIdx.y, piece = blockIdx.x;
+  const GradPiece p = grad_piece(a, adapter, piece);
+  const double s = grad_block_sum(p.t->f32 ? grad_squares<float>(p) : grad_squares<uint16_t>(p));
+  if (threadIdx.x == 0) a.parts[(uint64_t)adapter * a.parts_ld + a.part0 + piece] = s;
+}
+
+template <typename T>
+__device__ inline void grad_scale(const GradPiece& p, float factor) {
+  constexpr uint32_t N = GradUnit<T>::kN;
+  const T* g = static_cast<const T*>(p.t->grad) + p.at;
+  T* o = static_cast<T*>(p.t->out) + p.at;
+  if (factor == 1.0f && g == o) return;
+  const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T);
+  const uint32_t head = off ? (N - off < p.count ? N - off : p.count) : 0u, units = (p.count - head) / N;
+  if (threadIdx.x < head) o[threadIdx.x] = GradUnit<T>::back(GradUnit<T>::one(g[threadIdx.x]) * factor);
+  const uint4* u = reinterpret_cast<const uint4*>(g + head);
+  unsigned char* w = reinterpret_cast<unsigned char*>(o + head);
+  for (uint32_t i = threadIdx.x; i < units; i += 1024u) {
+    uint4 r[4];
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) r[x] = i + x * 256u < units ? u[i + x * 256u] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) {
+      float f[N];
+      GradUnit<T>::open(r[x], f);
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) f[j] *= factor;
+      const uint4 v = GradUnit<T>::close(f);
+      if (i + x * 256u < units) __builtin_memcpy(w + (uint64_t)(i + x * 256u) * 16u, &v, 16);  // (out may lie at another offset from 16)
+    }
+  }
+  const uint32_t done = head + units * N;
+  if (threadIdx.x < p.count - done) o[done + threadIdx.x] = GradUnit<T>::back(GradUnit<T>::one(g[done + threadIdx.x]) * factor);
+}
+
+__global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs a) {
+  const uint32_t adapter = blockIdx.y, piece = blockIdx.x;
+  double s = 0.0;
+  for (uint32_t i = threadIdx.x; i < a.parts_used; i += 256u) s += a.parts[(uint64_t)adapter * a.parts_ld + i];
+  const double norm = sqrt(grad_block_sum(s));
+  if (piece == 0 && a.part0 == 0 && threadIdx.x == 0) a.norms[adapter] = (float)norm;
+  if (!a.limits) return;
+  const float given = a.limits[adapter];
+  const double limit = given < 0.0f ? 0.0 : (double)given;
+  const float factor = norm > limit ? (float)(limit / norm) : 1.0f;  // (where either is no number the gradients stay as they are)
+  const GradPiece p = grad_piece(a, adapter, piece);
+  if (p.t->f32) grad_scale<float>(p, factor); else grad_scale<uint16_t>(p, factor);
+}
+
+__global__ __launch_bounds__(256) void grad_zero_norms_kernel(float* norms, uint32_t n) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  if (i < n) norms[i] = 0.0f;
+}
+
+}  // namespace w8a8

@@ -1,0 +1,131 @@
+"""Ragged per-expert products on bf16 weights and their gradients, on the gfx950 HIP kernels.
+
+The ``ragged_dot`` of the reference's ``skyrl/tx/layers/util.py:8-59`` for the expert kernels that
+``LoRAExpert.__call__`` (skyrl/tx/layers/lora.py:394-444) holds unquantized: rows sorted by group,
+``group_sizes[g]`` of them for group ``g``, rows beyond ``sum(group_sizes)`` giving zeros.  The
+W8A8 form is ``w8a8_lora.grouped_lora_linear``.
+
+Tensors are torch CUDA (ROCm) tensors; kernels are enqueued on torch's current stream.  Nothing is read
+back to the host: the group sizes may come straight from ``w8a8_lora.moe_dispatch``.  There is no CPU
+or eager fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ... import _native
+from .w8a8_lora import _on, _require_cuda, _stream_ptr
+
+MAX_GROUPS = 1024
+MAX_ROWS = 1 << 20
+MAX_FEATURES = 65536
+
+
+def _bf16(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be BF16, got {t.dtype}")
+    _require_cuda(t, name)
+    t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()  # (a view into the middle of a buffer: the kernels load 16 bytes)
+
+
+def _geometry(rows: torch.Tensor, name: str, width: int, weight_shape, group_sizes: torch.Tensor):
+    """``(m, k, n, groups, sizes)`` of a call, or what is wrong with it."""
+    if len(weight_shape) != 3:
+        raise ValueError(f"weight must be [groups, K, N], got {tuple(weight_shape)}")
+    g, k, n = weight_shape
+    if rows.ndim != 2 or rows.shape[0] <= 0 or rows.shape[1] != weight_shape[width]:
+        raise ValueError(f"{name} must be [rows, {weight_shape[width]}] with at least one row, got {tuple(rows.shape)}")
+    if group_sizes.ndim != 1 or group_sizes.shape[0] != g:
+        raise ValueError(f"group_sizes must have shape ({g},), got {tuple(group_sizes.shape)}")
+    if group_sizes.dtype.is_floating_point or group_sizes.dtype == torch.bool:
+        raise TypeError(f"group_sizes must be integers, got {group_sizes.dtype}")
+    m = rows.shape[0]
+    if k % 8 or n % 8 or not 0 < k <= MAX_FEATURES or not 0 < n <= MAX_FEATURES:
+        raise ValueError(f"K and N must be positive multiples of 8 not exceeding {MAX_FEATURES}, got {k} and {n}")
+    if not 0 < g <= MAX_GROUPS or m > MAX_ROWS:
+        raise ValueError(f"at most {MAX_GROUPS} groups and {MAX_ROWS} rows are supported, got {g} and {m}")
+    dev = rows.device
+    sizes = group_sizes.detach()
+    if sizes.dtype != torch.int32:
+        sizes = sizes.clamp(0, m)  # (what an int32 could not hold is more than there are rows)
+    return m, k, n, g, sizes.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def _same_device(first: torch.Tensor, *others) -> None:
+    for t in others:
+        if t.device != first.device:
+            raise ValueError(f"all operands must be on {first.device}, got {t.device}")
+
+
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Tensor) -> torch.Tensor:
+    """``out[rows of g] = bf16(x[rows of g] @ weight[g])`` with float32 sums: x bf16 [rows, K], weight bf16
+    [groups, K, N], group_sizes integers [groups].  Rows behind the last group are zero."""
+    xc, w = _bf16(x, "x"), _bf16(weight, "weight")
+    _same_device(x, weight)
+    m, k, n, g, sizes = _geometry(x, "x", 1, weight.shape, group_sizes)
+    out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    p = _native.Bf16GroupedProblem(ctypes.sizeof(_native.Bf16GroupedProblem), 0, m, k, n, g, xc.data_ptr(), w.data_ptr(),
+                                   sizes.data_ptr(), out.data_ptr())
+    with _on(x.device):
+        status = _native.load().mi355_w8a8_bf16_grouped_v1(ctypes.byref(p), _stream_ptr(x.device))
+    _native.check("mi355_w8a8_bf16_grouped_v1", status)
+    return out
+
+
+def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: torch.Tensor | None, group_sizes: torch.Tensor, *,
+                            need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.bfloat16):
+    """Cotangents ``(dx, dw)`` of ``grouped_matmul``: ``dx[rows of g] = bf16(dy[rows of g] @ weight[g].T)`` and
+    ``dw[g] = x[rows of g].T @ dy[rows of g]`` in ``dw_dtype`` (bf16 or float32), both from float32 sums; None for the one
+    that is not wanted.  ``x`` may be None without ``need_dw``, ``weight`` without ``need_dx``."""
+    if not need_dx and not need_dw:
+        return None, None
+    if (need_dw and x is None) or (need_dx and weight is None):
+        raise ValueError("dw needs x and dx needs weight")
+    if dw_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"dw_dtype must be BF16 or FP32, got {dw_dtype}")
+    d = _bf16(dy, "dy")
+    xc = _bf16(x, "x") if need_dw else None
+    w = _bf16(weight, "weight") if need_dx else None
+    _same_device(dy, *(t for t in (xc, w) if t is not None))
+    shape = weight.shape if weight is not None else (group_sizes.shape[0] if group_sizes.ndim else 0, x.shape[-1], dy.shape[-1])
+    m, k, n, g, sizes = _geometry(dy, "dy", 2, shape, group_sizes)
+    if need_dw and tuple(x.shape) != (m, k):
+        raise ValueError(f"x must be [{m}, {k}], got {tuple(x.shape)}")
+    dx = torch.empty((m, k), dtype=torch.bfloat16, device=dy.device) if need_dx else None
+    dw = torch.empty((g, k, n), dtype=dw_dtype, device=dy.device) if need_dw else None
+    p = _native.Bf16GroupedBwdProblem(ctypes.sizeof(_native.Bf16GroupedBwdProblem),
+                                      _native.FLAG_BF16_GROUPED_DW_F32 if dw_dtype == torch.float32 else 0, m, k, n, g,
+                                      xc.data_ptr() if need_dw else None, d.data_ptr(), w.data_ptr() if need_dx else None,
+                                      sizes.data_ptr(), dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None)
+    with _on(dy.device):
+        status = _native.load().mi355_w8a8_bf16_grouped_bwd_v1(ctypes.byref(p), _stream_ptr(dy.device))
+    _native.check("mi355_w8a8_bf16_grouped_bwd_v1", status)
+    return dx, dw
+
+
+class _GroupedMatmulFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, group_sizes):
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None, group_sizes)
+        ctx.shape = tuple(weight.shape)
+        return grouped_matmul(x, weight, group_sizes)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, group_sizes = ctx.saved_tensors
+        dx, dw = grouped_matmul_backward(x, dy, weight, group_sizes, need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
+        return dx, dw, None
+
+
+def bf16_grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Tensor) -> torch.Tensor:
+    """``grouped_matmul`` that autograd can differentiate in ``x`` and ``weight``."""
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+        return grouped_matmul(x, weight, group_sizes)
+    return _GroupedMatmulFunction.apply(x, weight, group_sizes)
+
+
+__all__ = ("MAX_FEATURES", "MAX_GROUPS", "MAX_ROWS", "bf16_grouped_linear", "grouped_matmul", "grouped_matmul_backward")

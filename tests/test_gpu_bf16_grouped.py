@@ -1,0 +1,187 @@
+"""Products grouped by expert on bf16 weights and their gradients against float64.
+
+Tolerance: products of bf16 values are exact in float32, so a sum of d of them is off by at most d * 2^-23 * S (S the sum of the
+products' magnitudes; one unit of the last place an addition, whichever way the matrix instruction rounds), and the one
+rounding to bf16 by half a step, 2^-8 of the value."""
+
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def gl():
+    return load_package().bf16_grouped_linear
+
+
+def make(rows, k, n, sizes, seed=0):
+    print(f"[case] {rows} rows, {k} -> {n}, sizes {sizes if len(sizes) < 20 else len(sizes)}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    t = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)
+    return t(rows, k), t(len(sizes), k, n), t(rows, n), torch.tensor(sizes, dtype=torch.int32, device=DEV)
+
+
+def spans(rows, sizes):
+    at = 0
+    for g, s in enumerate(sizes):
+        s = min(max(0, s), rows)
+        yield g, slice(min(at, rows), min(at + s, rows))
+        at += s
+
+
+def exact_forward(x, w, sizes):
+    out = torch.zeros(x.shape[0], w.shape[2], dtype=torch.float64, device=x.device)
+    for g, r in spans(x.shape[0], sizes):
+        out[r] = x[r].double() @ w[g].double()
+    return out
+
+
+def exact_dw(x, dy, sizes):
+    out = torch.zeros(len(sizes), x.shape[1], dy.shape[1], dtype=torch.float64, device=x.device)
+    for g, r in spans(x.shape[0], sizes):
+        out[g] = x[r].double().T @ dy[r].double()
+    return out
+
+
+def close(got, want, magnitudes, depth):
+    tol = depth * 2.0 ** -23 * magnitudes + (2.0 ** -8 * want.abs() if got.dtype == torch.bfloat16 else 0.0)
+    off = (got.double() - want).abs() - tol
+    assert not torch.isnan(got).any() and float(off.max()) <= 0.0, f"{float(off.max())} beyond at {int(off.argmax())}"
+
+
+def check(gl, x, w, dy, sizes_t, sizes, dw_dtype=torch.bfloat16):
+    k, n = w.shape[1:]
+    close(gl.grouped_matmul(x, w, sizes_t), exact_forward(x, w, sizes), exact_forward(x.abs(), w.abs(), sizes), k)
+    dx, dw = gl.grouped_matmul_backward(x, dy, w, sizes_t, dw_dtype=dw_dtype)
+    wt = w.transpose(1, 2)
+    close(dx, exact_forward(dy, wt, sizes), exact_forward(dy.abs(), wt.abs(), sizes), n)
+    assert dw.dtype == dw_dtype
+    close(dw, exact_dw(x, dy, sizes), exact_dw(x.abs(), dy.abs(), sizes), max(1, max(min(max(0, s), x.shape[0]) for s in sizes)))
+
+
+@pytest.mark.parametrize("rows,k,n,sizes", [
+    (1, 8, 8, [1]),                                   # the least
+    (1, 64, 128, [0, 0, 1, 0]),
+    (5, 72, 40, [0, 2, 0, 3, 0]),                     # nothing is a multiple of a tile
+    (64, 512, 768, [1] * 64),                         # decode: a row a group
+    (127, 136, 264, [127]),
+    (129, 128, 128, [0, 129]),
+    (300, 200, 328, [3, 128, 0, 129, 40]),
+    (1003, 712, 1096, [100, 0, 250, 1, 7, 0, 0, 333, 64, 65, 63, 20, 81]),  # rows behind the last group
+    (1537, 264, 520, [17] * 60 + [500]),
+    (2048, 1024, 512, [2048]),
+    (2000, 512, 1024, [900, 700, 400]),
+    (700, 64, 64, [1] * 500 + [0] * 523 + [200]),     # as many groups as there may be
+])
+def test_against_float64(gl, rows, k, n, sizes):
+    x, w, dy, st = make(rows, k, n, sizes)
+    check(gl, x, w, dy, st, sizes)
+    check(gl, x, w, dy, st, sizes, torch.float32)
+
+
+@pytest.mark.parametrize("sizes", [[0, 0, 0], [40, 200, 7], [-5, 40, -1], [1 << 30, 5, 1 << 30], [100, 0, 0]])
+def test_sizes_that_do_not_fit_the_rows(gl, sizes):
+    x, w, dy, st = make(100, 96, 72, sizes)
+    check(gl, x, w, dy, st, sizes)
+
+
+def test_longest_depths(gl):
+    for rows, k, n in ((70, 16384, 64), (40, 64, 24576), (9000, 64, 96)):
+        sizes = [rows // 2, rows - rows // 2]
+        x, w, dy, st = make(rows, k, n, sizes)
+        check(gl, x, w, dy, st, sizes, torch.float32)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_values_of_other_rows_stay_there(gl, bad):
+    """A NaN or infinity in one group's rows or weight, or in rows of no group, reaches that group's results alone, also where K and
+    the rows end inside a tile."""
+    sizes = [30, 50, 0, 20]
+    x, w, dy, st = make(120, 40, 72, sizes)
+    want, (wdx, wdw) = gl.grouped_matmul(x, w, st), gl.grouped_matmul_backward(x, dy, w, st)
+    x[30:80], dy[30:80], w[1], w[2] = bad, bad, bad, bad
+    x[100:], dy[100:] = bad, bad
+    out, (dx, dw) = gl.grouped_matmul(x, w, st), gl.grouped_matmul_backward(x, dy, w, st)
+    for got, ref in ((out, want), (dx, wdx)):
+        assert torch.equal(got[:30], ref[:30]) and torch.equal(got[80:], ref[80:]) and not torch.isfinite(got[30:80]).any()
+        assert not got[100:].any()
+    assert torch.equal(dw[0], wdw[0]) and torch.equal(dw[2:], wdw[2:]) and not torch.isfinite(dw[1]).any() and not dw[2].any()
+
+
+def test_differences(gl):
+    """Small whole numbers: every sum is exact in bf16, so a change of one value changes the output by the gradient times the change."""
+    sizes = [3, 0, 6, 2]
+    g = torch.Generator(device=DEV).manual_seed(5)
+    ints = lambda *s: torch.randint(-1, 2, s, generator=g, device=DEV).to(torch.bfloat16)
+    x, w, dy = ints(13, 16), ints(4, 16, 24), ints(13, 24)
+    st = torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    dx, dw = gl.grouped_matmul_backward(x, dy, w, st)
+    base = gl.grouped_matmul(x, w, st).double()
+    for i, c in ((0, 0), (2, 15), (3, 7), (10, 3), (12, 2)):
+        moved = x.clone()
+        moved[i, c] += 1
+        assert float(((gl.grouped_matmul(moved, w, st).double() - base) * dy.double()).sum()) == float(dx[i, c])
+    for e, r, c in ((0, 0, 0), (1, 5, 5), (2, 15, 23), (3, 8, 1)):
+        moved = w.clone()
+        moved[e, r, c] += 1
+        assert float(((gl.grouped_matmul(x, moved, st).double() - base) * dy.double()).sum()) == float(dw[e, r, c])
+
+
+def test_autograd_strides_and_offsets(gl):
+    sizes = [20, 0, 45]
+    x, w, dy, st = make(70, 48, 56, sizes)
+    want = gl.grouped_matmul(x, w, st), *gl.grouped_matmul_backward(x, dy, w, st)
+    wide = torch.zeros(70, 96, dtype=torch.bfloat16, device=DEV)
+    wide[:, ::2] = x
+    xs = wide[:, ::2].requires_grad_()
+    buffer = torch.empty(w.numel() + 3, dtype=torch.bfloat16, device=DEV)
+    ws = buffer[3:].view_as(w).copy_(w).detach().requires_grad_()
+    out = gl.bf16_grouped_linear(xs, ws, st.long())
+    out.backward(dy.t().contiguous().t())
+    assert torch.equal(out, want[0]) and torch.equal(xs.grad, want[1]) and torch.equal(ws.grad, want[2])
+    only_w = w.clone().requires_grad_()
+    gl.bf16_grouped_linear(x, only_w, st).backward(dy)
+    assert torch.equal(only_w.grad, want[2])
+    only_x = x.clone().requires_grad_()
+    gl.bf16_grouped_linear(only_x, w, st).backward(dy)
+    assert torch.equal(only_x.grad, want[1])
+
+
+def test_graph_replays_with_other_sizes_and_streams(gl):
+    sizes = [33, 60, 7]
+    x, w, dy, st = make(100, 64, 96, sizes)
+    other = torch.tensor([0, 90, 5], dtype=torch.int32, device=DEV)
+    want = {}
+    for key, s in (("a", st.clone()), ("b", other)):
+        want[key] = gl.grouped_matmul(x, w, s), *gl.grouped_matmul_backward(x, dy, w, s)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        side = gl.grouped_matmul(x, w, other)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(side, want["b"][0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gl.grouped_matmul(x, w, st)
+        dx, dw = gl.grouped_matmul_backward(x, dy, w, st)
+    for key, s in (("b", other), ("a", torch.tensor(sizes, dtype=torch.int32, device=DEV)), ("b", other)):
+        st.copy_(s)
+        graph.replay()
+        eager = gl.grouped_matmul(x, w, st)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[key][0])
+        for got, ref in zip((out, dx, dw), want[key]):
+            assert torch.equal(got, ref)
+
+
+def test_same_bits_at_every_call(gl):
+    sizes = [700, 0, 1200, 100]
+    x, w, dy, st = make(2048, 256, 384, sizes)
+    first = gl.grouped_matmul(x, w, st), *gl.grouped_matmul_backward(x, dy, w, st, dw_dtype=torch.float32)
+    for _ in range(3):
+        again = gl.grouped_matmul(x, w, st), *gl.grouped_matmul_backward(x, dy, w, st, dw_dtype=torch.float32)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))

@@ -1,0 +1,149 @@
+"""What the bf16 grouped products, the embedding rows and the gradient clipping refuse, on the CPU: the C calls with addresses that are
+never read, the Python entry points with CPU tensors."""
+
+import ctypes
+
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+
+A = 0x100000  # never dereferenced: validation fails first
+STEP = 0x10000000
+
+
+@pytest.fixture(scope="module")
+def native():
+    native = load_package()._native
+    if not native.LIB_PATH.exists():
+        pytest.skip("libmi355_w8a8.so not built (run __graft_entry__.build())")
+    return native
+
+
+def fill(struct, **kw):
+    p = struct()
+    p.struct_size = ctypes.sizeof(struct)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(struct_size=8), -8), (dict(flags=1), -2), (dict(m=0), -2), (dict(n_groups=0), -2), (dict(k=12), -7), (dict(n=4), -7),
+    (dict(k=65544), -7), (dict(n_groups=1025), -7), (dict(m=(1 << 20) + 1), -7), (dict(x=None), -1), (dict(weight=None), -1),
+    (dict(group_sizes=None), -1), (dict(out=None), -1), (dict(x=A + 8), -3), (dict(weight=A + STEP + 2), -3),
+    (dict(group_sizes=A + 2), -3), (dict(out=A + 16), -4), (dict(out=A + STEP + 1024), -4)])
+def test_grouped_call(native, change, status):
+    p = fill(native.Bf16GroupedProblem, **{**dict(m=16, k=64, n=32, n_groups=4, x=A, weight=A + STEP, group_sizes=A + 2 * STEP,
+                                                  out=A + 3 * STEP), **change})
+    assert native.load().mi355_w8a8_bf16_grouped_v1(ctypes.byref(p), None) == status
+    assert native.load().mi355_w8a8_bf16_grouped_v1(None, None) == -1
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(struct_size=8), -8), (dict(flags=2), -2), (dict(n=0), -2), (dict(k=4), -7), (dict(dy=None), -1), (dict(dx=None, dw=None), -1),
+    (dict(weight=None), -1), (dict(x=None), -1), (dict(dx=A + 3 * STEP + 4), -3), (dict(dw=A + STEP), -4), (dict(dx=A), -4),
+    (dict(dx=A + 3 * STEP, dw=A + 3 * STEP + 512), -4), (dict(dw=A + 2 * STEP), -4)])
+def test_grouped_backward_call(native, change, status):
+    p = fill(native.Bf16GroupedBwdProblem, **{**dict(m=16, k=64, n=32, n_groups=4, x=A, dy=A + STEP, weight=A + 2 * STEP,
+                                                     dx=A + 3 * STEP, dw=A + 4 * STEP, group_sizes=A + 5 * STEP), **change})
+    assert native.load().mi355_w8a8_bf16_grouped_bwd_v1(ctypes.byref(p), None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(struct_size=8), -8), (dict(flags=4), -2), (dict(n_tokens=0), -2), (dict(vocab=0), -2), (dict(width=0), -2),
+    (dict(n_tokens=(1 << 20) + 1), -7), (dict(width=65537), -7), (dict(vocab=(1 << 30) + 1), -7), (dict(n_adapters=2), -1),
+    (dict(n_adapters=1 << 22, vocab=1 << 22, adapter_indices=A + 2 * STEP), -7), (dict(adapter_indices=A), -2), (dict(scales=A), -2),
+    (dict(ids=None), -1), (dict(ids=A + 2), -3), (dict(flags=2, ids=A + 4), -3), (dict(out=None), -1)])
+def test_embedding_calls(native, change, status):
+    base = dict(n_tokens=8, vocab=100, width=24, ids=A, table=A + STEP, d_out=A + STEP, out=A + 3 * STEP, workspace=A + 4 * STEP,
+                workspace_bytes=1 << 20)
+    lib = native.load()
+    for fn in (lib.mi355_w8a8_embedding_v1, lib.mi355_w8a8_embedding_bwd_v1):
+        assert fn(ctypes.byref(fill(native.EmbeddingProblem, **{**base, **change})), None) == status
+    fwd = lambda **kw: lib.mi355_w8a8_embedding_v1(ctypes.byref(fill(native.EmbeddingProblem, **{**base, **kw})), None)
+    bwd = lambda **kw: lib.mi355_w8a8_embedding_bwd_v1(ctypes.byref(fill(native.EmbeddingProblem, **{**base, **kw})), None)
+    assert fwd(table=None) == -1 and bwd(d_out=None) == -1
+    assert fwd(out=A + STEP + 64) == -4 and bwd(out=A + STEP) == -4 and fwd(out=A) == -4
+    assert fwd(table=A + STEP + 1) == -3 and bwd(out=A + 3 * STEP + 8) == -3
+    assert bwd(workspace=None) == -5 and bwd(workspace_bytes=64) == -5 and bwd(workspace=A + 4 * STEP + 16) == -3
+    assert bwd(workspace=A + 3 * STEP) == -4
+    assert lib.mi355_w8a8_embedding_bwd_workspace_bytes(0, 100, 8, 0, 0) == 0
+    assert lib.mi355_w8a8_embedding_bwd_workspace_bytes(8, 100, 8, 0, 0) % 256 == 0
+
+
+def test_gradient_calls(native):
+    lib = native.load()
+
+    def clip(tensors, adapters=2, limits=A, norms=A + 64, ws=A + 5 * STEP, ws_bytes=1 << 20, n=None):
+        table = (native.GradTensor * max(1, len(tensors)))(*[native.GradTensor(*t) for t in tensors])
+        return lib.mi355_w8a8_grad_clip_v1(table, len(tensors) if n is None else n, adapters, limits, norms, ws, ws_bytes, None)
+
+    good = (A + STEP, A + 2 * STEP, 100, 0, 0)
+    assert lib.mi355_w8a8_grad_clip_v1(None, 1, 1, A, A, A, 1, None) == -1
+    assert clip([]) == -2 and clip([good], adapters=0) == -2 and clip([good], adapters=65536) == -7
+    assert clip([good], limits=None) == -1 and clip([good], norms=None) == -1
+    assert clip([(None, A, 100, 0, 0)]) == -1 and clip([(A + STEP, None, 100, 0, 0)]) == -1
+    assert clip([(A + STEP, A + 2 * STEP, 100, 2, 0)]) == -2 and clip([(A + STEP, A + 2 * STEP, 100, 0, 1)]) == -2
+    assert clip([(A + STEP + 1, A + 2 * STEP, 100, 0, 0)]) == -3 and clip([(A + STEP + 2, A + 2 * STEP, 100, 1, 0)]) == -3
+    assert clip([(A + STEP, A + STEP + 16, 100, 0, 0)]) == -4 and clip([good], norms=A + STEP) == -4 and clip([good], limits=A + 2 * STEP) == -4
+    assert clip([good], ws=None) == -5 and clip([good], ws_bytes=4) == -5 and clip([good], ws=A + 5 * STEP + 8) == -3
+    assert clip([good], ws=A + STEP) == -4 and clip([(A + STEP, A + 2 * STEP, 1 << 40, 0, 0)]) == -7
+    assert lib.mi355_w8a8_grad_norm_v1((native.GradTensor * 1)(native.GradTensor(*good)), 1, 1, None, A, 1 << 20, None) == -1
+
+
+def test_python_grouped(native):
+    gl = load_package().bf16_grouped_linear
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    sizes = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(TypeError, match="BF16"):
+        gl.grouped_matmul(torch.zeros(4, 8), bf(2, 8, 8), sizes)
+    with pytest.raises(RuntimeError, match="GPU"):
+        gl.grouped_matmul(bf(4, 8), bf(2, 8, 8), sizes)
+    with pytest.raises(TypeError, match="dw_dtype"):
+        gl.grouped_matmul_backward(bf(4, 8), bf(4, 8), bf(2, 8, 8), sizes, dw_dtype=torch.float16)
+    with pytest.raises(ValueError, match="needs"):
+        gl.grouped_matmul_backward(None, bf(4, 8), bf(2, 8, 8), sizes)
+    geometry = lambda x, w, s: gl._geometry(x, "x", 1, w.shape, s)
+    for x, w, s in ((bf(4, 8), bf(8, 8), sizes), (bf(4, 16), bf(2, 8, 8), sizes), (bf(0, 8), bf(2, 8, 8), sizes), (bf(4, 2, 8), bf(2, 8, 8), sizes),
+                    (bf(4, 8), bf(2, 8, 8), torch.zeros(3, dtype=torch.int32)), (bf(4, 12), bf(2, 12, 8), sizes), (bf(4, 8), bf(2, 8, 20), sizes),
+                    (bf(4, 8), bf(1025, 8, 8), torch.zeros(1025, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            geometry(x, w, s)
+    with pytest.raises(TypeError, match="integers"):
+        geometry(bf(4, 8), bf(2, 8, 8), torch.zeros(2))
+
+
+def test_python_embedding(native):
+    em = load_package().embedding
+    ids = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="GPU"):
+        em.lookup(torch.zeros(4, 8), ids)
+    with pytest.raises(RuntimeError, match="GPU"):
+        em.lookup_backward(torch.zeros(3, 8), ids, (4, 8))
+    dev = torch.device("cpu")
+
+    def problem(ids=ids, shape=(4, 8), scale=None, index=None, dtype=torch.bfloat16):
+        return em._problem(ids, shape, scale, index, dtype, dev)
+
+    with pytest.raises(TypeError, match="FP32"):
+        problem(dtype=torch.float16)
+    with pytest.raises(TypeError, match="INT"):
+        problem(ids=torch.zeros(3))
+    with pytest.raises(RuntimeError, match="GPU"):
+        problem()
+    leaf = torch.ones(2, requires_grad=True)
+    with pytest.raises(ValueError, match="constant"):
+        em.embed(torch.zeros(2, 4, 8), ids, leaf, adapter_indices=ids)
+
+
+def test_python_clipping(native):
+    gc = load_package().grad_clip
+    with pytest.raises(ValueError, match="at least one"):
+        gc.grad_norm([])
+    with pytest.raises(TypeError, match="BF16"):
+        gc.grad_norm([torch.zeros(3, dtype=torch.float16)])
+    with pytest.raises(RuntimeError, match="GPU"):
+        gc.grad_norm([torch.zeros(3)])
+    with pytest.raises(TypeError, match="bool"):
+        gc.clip_grad_norm([torch.zeros(3)], 1.0, per_adapter=1)
