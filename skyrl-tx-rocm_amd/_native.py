@@ -36,6 +36,7 @@ FLAG_QKV_WEIGHTS_BF16 = 1  # of the two QKV stage problems
 FLAG_GQ_DIRECT = 1  # mi355_w8a8_gq_problem.flags
 FLAG_GQ_BF16_SCALES = 2  # mi355_w8a8_gq_bwd_problem.flags
 FLAG_BF16_GROUPED_DW_F32 = 1  # mi355_w8a8_bf16_grouped_bwd_problem.flags
+FLAG_BF16_GROUPED_TILE_256X256, FLAG_BF16_GROUPED_TILE_128X256, FLAG_BF16_GROUPED_TILE_64X128 = 4, 8, 16
 FLAG_EMBEDDING_F32 = 1        # mi355_w8a8_embedding_problem.flags
 FLAG_EMBEDDING_IDS64 = 2
 GRAD_BF16, GRAD_F32 = 0, 1    # mi355_w8a8_grad_tensor.type

@@ -17,9 +17,13 @@ extern "C" {
  * MI355_W8A8_BF16_GROUPED_MAX_FEATURES; m at most 2^20, n_groups at most 1024.
  */
 #define MI355_W8A8_BF16_GROUPED_MAX_FEATURES 65536u
+/* tiles of the products (at most one of the three; default: by the rows, the groups and how many tiles result) */
+#define MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256 4u
+#define MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256 8u
+#define MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128 16u
 typedef struct mi355_w8a8_bf16_grouped_problem {
   uint32_t struct_size;     /* sizeof(mi355_w8a8_bf16_grouped_problem) */
-  uint32_t flags;           /* 0 */
+  uint32_t flags;
   uint32_t m;               /* rows of x */
   uint32_t k;               /* in features */
   uint32_t n;               /* out features */

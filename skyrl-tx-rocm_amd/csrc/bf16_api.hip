@@ -5,6 +5,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "bf16_grouped.h"
 #include "embedding.h"
 #include "grad_clip.h"
@@ -30,6 +32,9 @@ inline bool allow_lds(K kernel, uint32_t bytes) {
 
 // ---- products grouped by expert --------------------------------------------------------------------------------------
 
+constexpr uint32_t kGroupedTiles = MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256 | MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256 | MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128;
+inline bool one_bit_at_most(uint32_t v) { return (v & (v - 1u)) == 0; }
+
 int check_grouped_dims(uint32_t m, uint32_t k, uint32_t n, uint32_t groups) {
   if (m == 0 || k == 0 || n == 0 || groups == 0) return MI355_W8A8_ERR_SHAPE;
   if ((k & 7u) || (n & 7u)) return MI355_W8A8_ERR_UNSUPPORTED;
@@ -45,23 +50,44 @@ inline uint64_t most_row_tiles(uint32_t m, uint32_t groups, uint32_t tile) {
   return (m + (uint64_t)(tile - 1u) * held) / tile;
 }
 
-template <int KIND>
-int launch_grouped(const BgArgs& g, hipStream_t s) {
-  constexpr int TM = 128, TN = 128, BK = 64, STAGES = 2;
-  auto kernel = &bf16_grouped_kernel<KIND, TM, TN, 2, 2, BK, STAGES>;
-  constexpr uint32_t kLds = (TM + TN) * BK * 2 * STAGES;
-  if (!allow_lds(kernel, kLds)) return MI355_W8A8_ERR_LAUNCH;
+template <int KIND, int TM, int TN, int WM, int WN, int STAGES, int LOADERS, bool F32>
+int launch_grouped_tiles(const BgArgs& g, hipStream_t s) {
+  auto kernel = &bf16_grouped_kernel<KIND, TM, TN, WM, WN, STAGES, LOADERS, F32>;
+  const uint32_t lds = (TM + TN) * kBgDepth * 2u * STAGES + (kBgScratch + 2u * (g.groups + 2u)) * 4u;
+  if (!allow_lds(kernel, lds)) return MI355_W8A8_ERR_LAUNCH;
   const uint64_t n_tiles = (g.cols + TN - 1u) / TN;
   const uint64_t tiles = n_tiles * (KIND == kGroupedDw ? (uint64_t)g.groups * ((g.rows + TM - 1u) / TM) : most_row_tiles(g.m, g.groups + 1u, TM));
-  if (tiles > 0x7ffffff0u) return MI355_W8A8_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)((tiles + 7u) / 8u * 8u)), dim3(256), kLds, s, g);
+  const uint32_t grid = (uint32_t)(tiles < 256u ? (tiles + 7u) / 8u * 8u : 256u);  // (one workgroup a CU: its stages fill the LDS)
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * (WM * WN + LOADERS)), lds, s, g);
   return launch_status();
+}
+
+// Which tiles.  A call costs the rounds of its tiles on the 256 CUs times what a round takes: 4 units for 256 x 256, 2.2 for 128 x 256 and
+// 1.15 for 64 x 128 (half and an eighth of the products; 32768 rows of 4096 -> 12288 in 8 groups 2740, 3060 and 6100 us).  Groups end
+// in the middle of a tile, half a tile on average.  The smaller tiles have room for more stages, which is what counts where the
+// weights come from memory for few rows.  us, 256 x 256 / 128 x 256 / 64 x 128, 2048 -> 1536, 128 groups of uneven sizes: forward 16384 rows 235 / 197 /
+// 250, 8192 224 / 176 / 194, 512 172 / 142 / 146, 64 100 / 70 / 60, dW 16384 rows 259 / 245 / 373, 8192 180 / 194 / 286; 4096 -> 4096, 4 groups,
+// 2048 rows 91 / 109 / 133; 1024 -> 1024, 8 groups, 4096 rows 31 / 23 / 29.
+template <int KIND, bool F32 = false>
+int launch_grouped(const BgArgs& g, uint32_t forced, hipStream_t s) {
+  auto cost = [&](uint32_t tm, uint32_t tn, float round) {
+    const float held = (float)(g.groups < g.m ? g.groups : g.m);
+    const float row_tiles = KIND == kGroupedDw ? (float)((uint64_t)g.groups * ((g.rows + tm - 1u) / tm)) : fmaxf((float)g.m / tm + 0.5f * held, held);
+    return ceilf(row_tiles * ((g.cols + tn - 1u) / tn) / 256.0f) * round;
+  };
+  if (forced == MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
+  if (forced == MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
+  if (forced) return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
+  const float large = cost(256u, 256u, 4.0f), middle = cost(128u, 256u, 2.2f), small = cost(64u, 128u, 1.15f);
+  if (large <= middle && large <= small) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
+  if (middle <= small) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
+  return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
 }
 
 int run_grouped(const mi355_w8a8_bf16_grouped_problem* p, hipStream_t s) {
   if (!p) return MI355_W8A8_ERR_NULL;
   if (p->struct_size != sizeof(mi355_w8a8_bf16_grouped_problem)) return MI355_W8A8_ERR_STRUCT;
-  if (p->flags) return MI355_W8A8_ERR_SHAPE;
+  if ((p->flags & ~kGroupedTiles) || !one_bit_at_most(p->flags)) return MI355_W8A8_ERR_SHAPE;
   const int st = check_grouped_dims(p->m, p->k, p->n, p->n_groups);
   if (st) return st;
   if (!p->x || !p->weight || !p->group_sizes || !p->out) return MI355_W8A8_ERR_NULL;
@@ -77,13 +103,14 @@ int run_grouped(const mi355_w8a8_bf16_grouped_problem* p, hipStream_t s) {
   g.sizes = p->group_sizes; g.out = p->out;
   g.m = p->m; g.rows_ld = p->k; g.cols_ld = p->n; g.depth = p->k; g.cols = p->n; g.groups = p->n_groups;
   g.b_group = (uint64_t)p->k * p->n;
-  return launch_grouped<kGroupedFwd>(g, s);
+  return launch_grouped<kGroupedFwd>(g, p->flags, s);
 }
 
 int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s) {
   if (!p) return MI355_W8A8_ERR_NULL;
   if (p->struct_size != sizeof(mi355_w8a8_bf16_grouped_bwd_problem)) return MI355_W8A8_ERR_STRUCT;
-  if (p->flags & ~MI355_W8A8_FLAG_BF16_GROUPED_DW_F32) return MI355_W8A8_ERR_SHAPE;
+  const uint32_t forced = p->flags & kGroupedTiles;
+  if ((p->flags & ~(kGroupedTiles | MI355_W8A8_FLAG_BF16_GROUPED_DW_F32)) || !one_bit_at_most(forced)) return MI355_W8A8_ERR_SHAPE;
   int st = check_grouped_dims(p->m, p->k, p->n, p->n_groups);
   if (st) return st;
   if (!p->dy || !p->group_sizes || (!p->dx && !p->dw)) return MI355_W8A8_ERR_NULL;
@@ -108,13 +135,13 @@ int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s)
     g.a = static_cast<const uint16_t*>(p->dy); g.b = static_cast<const uint16_t*>(p->weight); g.out = p->dx;
     g.rows_ld = p->n; g.cols_ld = p->n; g.depth = p->n; g.cols = p->k;
     g.b_group = (uint64_t)p->k * p->n;
-    if ((st = launch_grouped<kGroupedDx>(g, s))) return st;
+    if ((st = launch_grouped<kGroupedDx>(g, forced, s))) return st;
   }
   if (p->dw) {
     g.a = static_cast<const uint16_t*>(p->x); g.b = static_cast<const uint16_t*>(p->dy); g.out = p->dw;
-    g.rows_ld = p->k; g.cols_ld = p->n; g.depth = 0; g.cols = p->n; g.rows = p->k; g.f32 = f32;
+    g.rows_ld = p->k; g.cols_ld = p->n; g.depth = 0; g.cols = p->n; g.rows = p->k;
     g.out_group = (uint64_t)p->k * p->n;
-    st = launch_grouped<kGroupedDw>(g, s);
+    st = f32 ? launch_grouped<kGroupedDw, true>(g, forced, s) : launch_grouped<kGroupedDw>(g, forced, s);
   }
   return st;
 }

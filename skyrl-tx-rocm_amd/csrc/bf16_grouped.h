@@ -15,13 +15,17 @@
 //
 // Fragments are those of v_mfma_f32_16x16x32_bf16: lane l holds the eight t = 8 (l / 16) .. + 7 of row l % 16.  The columns of C
 // are the instruction's rows, so that a lane ends up with values of neighbouring columns: fragment j, row 4 q + v of 64 columns is
-// column 32 (j / 2) + 8 q + 4 (j % 2) + v, and two fragments give the lane 16 bytes to store.
+// column 32 (j / 2) + 8 q + 4 (j % 2 ^ q % 2) + v, and two fragments give the lane 16 bytes to store.  (The exclusive or puts the 8-byte
+// pieces that a transposing read takes from neighbouring units into different halves of them: without it two of its rows meet on the
+// same banks, a third more clocks in the LDS.)
 //
 // Stages come by buffer_load_dwordx4 .. lds, whose range check puts zeros in the place of what lies beyond K, N or a group's rows: an
 // invalid lane's offset is kOutside, past every record count.  A row of the LDS has its 16-byte units permuted by an exclusive or
 // with bits of the row number (the load's lane picks the unit of memory that belongs at its place), so that a wave's read
 // touches every bank equally.
 #pragma once
+#include <type_traits>
+
 #include "w8a8_device.h"
 
 namespace w8a8 {
@@ -31,6 +35,7 @@ enum GroupedKind { kGroupedFwd = 0, kGroupedDx = 1, kGroupedDw = 2 };
 constexpr uint32_t kBgMaxGroups = 1024;
 constexpr uint32_t kOutside = 0x80000000u;     // beyond every buffer's records (at most 2^31 - 1 bytes)
 constexpr uint32_t kRecords = 0x7ffffff0u;
+constexpr int kBgDepth = 64;    // contraction indices of a stage
 
 struct BgArgs {
   const uint16_t* a;   // rows' operand: x (forward, dW) or dy (dx)
@@ -40,17 +45,18 @@ struct BgArgs {
   uint32_t m, rows_ld, cols_ld;  // rows in all; elements between rows of a and of b
   uint32_t depth;                // contraction length of forward and dx
   uint32_t cols, rows;           // columns of C; rows of C a group (dW)
-  uint32_t groups, f32;          // f32: C is float32
+  uint32_t groups;
   uint64_t b_group, out_group;   // elements between groups of b and of C (forward, dx: of b alone)
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-// 1 KiB to the LDS, lane l 16 bytes from base + voff to lds_addr + 16 l; lanes at kOutside give zeros.  (A statement of its own: the
-// compiler drains every counter behind the builtin.)
-__device__ inline void lds_buffer_load_1k(v4i rsrc, uint32_t voff, uint32_t lds_addr_uniform) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :: "v"(voff), "s"(rsrc), "s"(lds_addr_uniform) : "memory", "m0");
+// 1 KiB to the LDS, lane l 16 bytes from base + soff + voff to lds_addr + 16 l; lanes at kOutside give zeros.  (A statement of its own:
+// the compiler drains every counter behind the builtin.)
+__device__ inline void lds_buffer_load_1k(v4i rsrc, uint32_t voff, uint32_t soff_uniform, uint32_t lds_addr_uniform) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               :: "v"(voff), "s"(rsrc), "s"(soff_uniform), "s"(lds_addr_uniform) : "memory", "m0");
 }
 __device__ inline v4i buffer_of(const void* base_uniform) {
   const uint64_t a = reinterpret_cast<uint64_t>(base_uniform);
@@ -62,19 +68,33 @@ __device__ inline v4i buffer_of(const void* base_uniform) {
   return r;
 }
 
-// Where a group's rows start, and the tile a workgroup has.
-struct BgPlace {
-  uint32_t group, start, size;  // rows of the group; group == groups: the rows behind the last one
-  uint32_t tile, tiles;         // this workgroup's place among the tiles of its group
+// (The offset comes in the lanes' registers alone: behind a 16-byte store with a scalar offset the compiler lets the next instruction
+// write the data's registers, and the memory then got what that instruction wrote.  Without one it keeps the wait states.)
+__device__ inline void buffer_store_16(v4i v, v4i rsrc, uint32_t voff) {
+  void* base = reinterpret_cast<void*>((uint64_t)(uint32_t)rsrc[0] | (uint64_t)(uint32_t)rsrc[1] << 32);
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), __builtin_amdgcn_make_buffer_rsrc(base, 0, rsrc[2], rsrc[3]), (int)voff, 0, 2);
+}
+
+// (a tile without products has one stage, of zeros)
+__device__ inline uint32_t bg_stages(uint32_t depth) { return depth ? (depth + kBgDepth - 1u) / kBgDepth : 1u; }
+
+// Tables of a call in the LDS, made by every workgroup from the sizes: the first row and the first tile of every group (and of the rows
+// behind the last one, which are a group of their own for the forward and dx).
+struct BgTables {
+  uint32_t* start;   // [groups + 2]
+  uint32_t* tile;    // [groups + 2]; behind the last group: the tiles in all
 };
 
+// The die of this workgroup and the share of the tiles that it takes: the workgroups are dealt out to the eight dies in turn, a die has
+// tiles that follow each other (its workgroups then share operands in its L2), and the shares cost the same.
+struct BgShare { uint32_t first, end; };
+constexpr uint32_t kBgScratch = 64;
+
 // Sizes are clamped to [0, m] one by one, starts to [0, m]: whatever the array holds, no row beyond m is touched.
-// per_group: tiles of a group of `size` rows.  Workgroup b of the grid takes tile (b % 8) * ceil(total / 8) + b / 8, so that the
-// workgroups of one of the eight dies (which are dealt out in turn) hold tiles that follow each other and share operands
-// in that die's L2.  False: no tile is left.
-template <int THREADS, class PerGroup>
-__device__ inline bool bg_place(const BgArgs& g, uint32_t groups_with_tail, uint32_t* lds, PerGroup per_group, BgPlace& place) {
-  constexpr uint32_t kPer = (kBgMaxGroups + THREADS) / THREADS;  // groups a thread looks at, one more for the tail
+// tiles_of, cost_of: tiles of a group with `rows` rows (nothing behind the last of `held` groups), what each costs.  scratch: kBgScratch words.
+template <int THREADS, class TilesOf, class CostOf>
+__device__ inline BgShare bg_tables(const BgArgs& g, uint32_t held, const BgTables& tab, uint32_t* scratch, TilesOf tiles_of, CostOf cost_of) {
+  constexpr uint32_t kPer = (kBgMaxGroups + THREADS) / THREADS, kWaves = THREADS / 64;  // groups a thread looks at, one more for the rows behind them
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   uint32_t size[kPer], rows = 0, first = tid * kPer;
 #pragma unroll
@@ -85,110 +105,135 @@ __device__ inline bool bg_place(const BgArgs& g, uint32_t groups_with_tail, uint
   }
   // rows in front of this thread's groups
   const uint32_t incl = wave_scan(rows);
-  if (lane == 63u) lds[wave] = incl;
+  if (lane == 63u) scratch[wave] = incl;
   __syncthreads();
-  uint32_t before = incl - rows;
-  for (uint32_t w = 0; w < wave; ++w) before += lds[w];
-  // the groups' tiles
-  uint32_t start[kPer], tiles[kPer], mine = 0, at = before;
+  uint32_t at = incl - rows;
+  for (uint32_t w = 0; w < wave; ++w) at += scratch[w];
+  // the groups' tiles and what they cost (64 bits: thousands of stages times millions of tiles)
+  uint32_t tiles[kPer], mine = 0;
+  uint64_t cost = 0;
 #pragma unroll
   for (uint32_t i = 0; i < kPer; ++i) {
-    const uint32_t gi = first + i;
-    start[i] = at < g.m ? at : g.m;
+    const uint32_t gi = first + i, start = at < g.m ? at : g.m;
     at += size[i];
-    const uint32_t end = at < g.m ? at : g.m;
-    size[i] = gi < g.groups ? end - start[i] : g.m - start[i];
-    tiles[i] = gi < groups_with_tail ? per_group(gi, size[i]) : 0u;
+    const uint32_t end = gi < g.groups && at < g.m ? at : g.m;
+    size[i] = end - start;
+    tiles[i] = gi < held ? tiles_of(size[i]) : 0u;
     mine += tiles[i];
+    cost += (uint64_t)tiles[i] * cost_of(gi, size[i]);
+    if (gi <= g.groups) tab.start[gi] = start;
   }
+  uint64_t* costs = reinterpret_cast<uint64_t*>(scratch + 32);
   const uint32_t incl_t = wave_scan(mine);
-  if (lane == 63u) lds[16 + wave] = incl_t;
+  uint64_t incl_c = cost;
+#pragma unroll
+  for (uint32_t o = 1; o < 64u; o <<= 1) {
+    const uint64_t before = __shfl_up(incl_c, o);
+    if (lane >= o) incl_c += before;
+  }
+  if (lane == 63u) {
+    scratch[16 + wave] = incl_t;
+    costs[wave] = incl_c;
+  }
   __syncthreads();
   uint32_t total = 0, first_tile = incl_t - mine;
+  uint64_t all = 0, at_cost = incl_c - cost;
 #pragma unroll
-  for (uint32_t w = 0; w < THREADS / 64; ++w) {
-    const uint32_t n = lds[16 + w];
-    first_tile += w < wave ? n : 0u;
-    total += n;
+  for (uint32_t w = 0; w < kWaves; ++w) {
+    first_tile += w < wave ? scratch[16 + w] : 0u;
+    total += scratch[16 + w];
+    at_cost += w < wave ? costs[w] : 0u;
+    all += costs[w];
   }
-  const uint32_t each = (total + 7u) / 8u, in_die = blockIdx.x >> 3, wanted = (blockIdx.x & 7u) * each + in_die;
-  const bool any = in_die < each && wanted < total;
-  if (any) {
-#pragma unroll
-    for (uint32_t i = 0; i < kPer; ++i) {
-      if (wanted >= first_tile && wanted < first_tile + tiles[i]) {
-        lds[32] = first + i; lds[33] = start[i]; lds[34] = size[i]; lds[35] = wanted - first_tile; lds[36] = tiles[i];
-      }
-      first_tile += tiles[i];
-    }
+  // tiles in front of the share that starts at x eighths of the cost: found by the thread whose groups hold that place
+  const uint32_t die = blockIdx.x & 7u;
+  const uint64_t from = all * die / 8u, to = all * (die + 1u) / 8u;
+  if (tid == 0) {
+    tab.start[g.groups + 1u] = g.m;
+    tab.tile[g.groups + 1u] = total;
+    scratch[12] = 0;  // (behind the rows of the at most twelve waves)
+    scratch[13] = total;
   }
   __syncthreads();
-  if (!any) return false;
-  place.group = __builtin_amdgcn_readfirstlane(lds[32]);
-  place.start = __builtin_amdgcn_readfirstlane(lds[33]);
-  place.size = __builtin_amdgcn_readfirstlane(lds[34]);
-  place.tile = __builtin_amdgcn_readfirstlane(lds[35]);
-  place.tiles = __builtin_amdgcn_readfirstlane(lds[36]);
+#pragma unroll
+  for (uint32_t i = 0; i < kPer; ++i) {
+    const uint64_t each = cost_of(first + i, size[i]), own = tiles[i] * each;
+    if (first + i <= g.groups) tab.tile[first + i] = first_tile;
+    if (die > 0u && from >= at_cost && from < at_cost + own) scratch[12] = first_tile + (uint32_t)((from - at_cost) / each);
+    if (die < 7u && to >= at_cost && to < at_cost + own) scratch[13] = first_tile + (uint32_t)((to - at_cost) / each);
+    first_tile += tiles[i];
+    at_cost += own;
+  }
   __syncthreads();
-  return true;
+  return {(uint32_t)__builtin_amdgcn_readfirstlane(scratch[12]), (uint32_t)__builtin_amdgcn_readfirstlane(scratch[13])};
+}
+
+// The last group whose first tile is not behind `tile`: 64 places at a time, at most 17 between two of them.
+__device__ inline uint32_t bg_group_of(const uint32_t* first, uint32_t groups, uint32_t tile, uint32_t lane) {
+  const uint32_t step = (groups + 64u) / 64u, at = lane * step;
+  const uint32_t coarse = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(at <= groups && first[at <= groups ? at : 0u] <= tile)) - 1u;
+  const uint32_t fine = coarse * step + lane;
+  const bool below = lane < step && fine <= groups;
+  return coarse * step + (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(below && first[below ? fine : 0u] <= tile)) - 1u;
 }
 
 // The unit permutations.  ALONG: the operand is staged as [T][BK] (its rows run along the contraction), else as [BK][T].
 // PAIRED: the fragment's rows are those of the columns' operand (see the head).
-template <bool PAIRED>
-__device__ inline uint32_t bg_unit_along(uint32_t row) {  // 128-byte rows: the 16 rows of a fragment on all banks
+template <int BK, bool PAIRED>
+__device__ inline uint32_t bg_unit_along(uint32_t row) {  // rows of 64 or 128 bytes: the 16 rows of a fragment on all banks
+  if (BK == 32) return PAIRED ? (row >> 3) & 3u : (row >> 2) & 3u;
   return PAIRED ? ((row >> 1) & 1u) | ((row >> 3) & 3u) << 1 : (row >> 1) & 7u;
 }
 template <bool PAIRED>
 __device__ inline uint32_t bg_unit_across(uint32_t t) {  // rows of 256 bytes: four rows t of 128 bytes on all banks
-  return PAIRED ? (t & 3u) << 2 : ((t & 3u) << 1) | ((t >> 3) & 1u) << 3;
+  return PAIRED ? (t & 3u) << 2 | ((t >> 3) & 1u) : ((t & 3u) << 1) | ((t >> 3) & 1u) << 3;
 }
 
-// One operand's share of a stage: LOADS loads of 1 KiB a wave.
+// One operand's share of a stage: kLoads loads of 1 KiB a wave, of kPlaces rows (ALONG) or contraction indices each.  Load number
+// `index` of the workgroup holds the places index * kPlaces + lane / kUnits; the permutation of a place is the exclusive or of that of its lane
+// part and that of its load's, which share no bits.
 template <int T, int BK, bool ALONG, bool PAIRED, int WAVES>
 struct BgOperand {
   static constexpr int kBytes = T * BK * 2, kLoads = kBytes / 1024 / WAVES;
-  static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
-  uint32_t voff[kLoads], need[kLoads];  // offset from the stage's base; the contraction index a lane needs
-  uint32_t step_lo;                     // bytes between stages
-  const unsigned char* base;
+  static constexpr uint32_t kUnits = (ALONG ? BK : T) / 8u, kPlaces = 64u / kUnits;
+  static_assert(kBytes % (1024 * WAVES) == 0 && BK == 64, "whole loads");
+  const unsigned char* base;  // of the stage that is loaded next
+  uint32_t ld_bytes, valid;   // bytes between rows in memory; rows (ALONG) or columns of the tile that exist
+  uint32_t place, unit, voff; // of the lane: its place in a load, the 16-byte unit of a place of even permutation, the offset of its place
 
-  // valid: rows (ALONG) or columns of the tile that exist
-  __device__ inline void init(const uint16_t* first, uint32_t ld, uint32_t valid, uint32_t wave, uint32_t lane) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t off = (wave * kLoads + i) * 1024u + lane * 16u;
-      if constexpr (ALONG) {
-        const uint32_t row = off / (BK * 2u), unit = ((off >> 4) % (BK / 8u)) ^ (bg_unit_along<PAIRED>(row) % (BK / 8u));
-        need[i] = unit * 8u;
-        voff[i] = row < valid ? row * ld * 2u + unit * 16u : kOutside;
-      } else {
-        const uint32_t t = off / (T * 2u), unit = ((off >> 4) % (T / 8u)) ^ (bg_unit_across<PAIRED>(t) % (T / 8u));
-        need[i] = t;
-        voff[i] = unit * 8u < valid ? t * ld * 2u + unit * 16u : kOutside;
-      }
-    }
-    step_lo = ALONG ? BK * 2u : BK * ld * 2u;
+  static __device__ inline uint32_t permutation(uint32_t p) {
+    if constexpr (ALONG) return bg_unit_along<BK, PAIRED>(p) % kUnits;
+    else return bg_unit_across<PAIRED>(p) % kUnits;
+  }
+  __device__ inline void init(uint32_t ld, uint32_t lane) {
+    ld_bytes = ld * 2u;
+    place = lane / kUnits;
+    unit = (lane % kUnits) ^ permutation(place);
+    voff = place * ld_bytes;
+  }
+  __device__ inline void open(const uint16_t* first, uint32_t existing) {
     base = reinterpret_cast<const unsigned char*>(first);
+    valid = existing;
   }
-  // left: contraction indices from the stage's start on
-  __device__ inline void load(uint32_t left, uint32_t lds, uint32_t wave) {
-    const v4i r = buffer_of(base);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      lds_buffer_load_1k(r, need[i] < left ? voff[i] : kOutside, __builtin_amdgcn_readfirstlane(lds + (wave * kLoads + i) * 1024u));
-    base += step_lo;
+  // load i of the stage at base; left: contraction indices from there on
+  __device__ inline void load(int i, uint32_t left, uint32_t lds, uint32_t wave) const {
+    const uint32_t index = wave * kLoads + i, at = index * kPlaces;
+    const uint32_t u = unit ^ permutation(at);
+    const bool in_row = u * 8u < (ALONG ? left : valid), in_places = (int)place < (int)((ALONG ? valid : left) - at);
+    lds_buffer_load_1k(buffer_of(base), in_row && in_places ? voff + u * 16u : kOutside, __builtin_amdgcn_readfirstlane(at * ld_bytes),
+                       __builtin_amdgcn_readfirstlane(lds + index * 1024u));
   }
+  __device__ inline void next() { base += ALONG ? BK * 2u : BK * ld_bytes; }
   // the lane's eight contraction values 32 step + 8 (lane / 16) .. of fragment f
   __device__ static inline v8bf fragment(const unsigned char* tile, uint32_t first, int f, int step, uint32_t lane) {
     const uint32_t i = lane & 15u, q = lane >> 4;
     if constexpr (ALONG) {
-      const uint32_t row = first + (PAIRED ? 32u * (f >> 1) + 8u * (i >> 2) + 4u * (f & 1) + (i & 3u) : 16u * f + i);
-      const uint32_t unit = (4u * step + q) ^ (bg_unit_along<PAIRED>(row) % (BK / 8u));
+      const uint32_t row = first + (PAIRED ? 32u * (f >> 1) + 8u * (i >> 2) + 4u * ((f ^ (i >> 2)) & 1u) + (i & 3u) : 16u * f + i);
+      const uint32_t unit = (4u * step + q) ^ bg_unit_along<BK, PAIRED>(row);
       return *reinterpret_cast<const v8bf*>(tile + row * (BK * 2u) + unit * 16u);
     } else {
       typedef __attribute__((address_space(3))) v4s* lds_v4s;
-      const uint32_t c = i & 3u, col = first + (PAIRED ? 32u * (f >> 1) + 8u * c + 4u * (f & 1) : 16u * f + 4u * c);
+      const uint32_t c = i & 3u, col = first + (PAIRED ? 32u * (f >> 1) + 8u * c + 4u * ((f ^ c) & 1u) : 16u * f + 4u * c);
       v4s h[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -203,104 +248,230 @@ struct BgOperand {
   }
 };
 
-// TM x TN tiles, WM x WN waves, stages of BK.
-template <int KIND, int TM, int TN, int WM, int WN, int BK, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void bf16_grouped_kernel(BgArgs g) {
-  constexpr int kWaves = WM * WN, FM = TM / WM / 16, FN = TN / WN / 16;
-  static_assert(FN % 2 == 0, "a lane stores two fragments together");
-  using OpA = BgOperand<TM, BK, KIND != kGroupedDw, false, kWaves>;
-  using OpB = BgOperand<TN, BK, KIND == kGroupedDx, true, kWaves>;
+// One tile of a call.
+struct BgTile {
+  uint32_t group, start, row0, col0, rows, depth;  // rows: of the tile's group from row0 on (at least one); start: the group's first row
+};
+
+// TM x TN tiles, WM x WN waves, STAGES stages of 64 in the LDS.  LOADERS: waves that do nothing but request the stages (0: every wave its
+// share).  A wave's loads and stores return in one order, so one that waits for a stage waits for the results it stored before: with
+// loaders nobody does, which is what a dW of few stages a tile is made of.  A workgroup takes tile after tile, and the stages of one follow those of
+// the tile before in one stream: while a tile's results are stored the first stages of the next are on their way.
+// A die's workgroups take the tiles of its share in turn.
+template <int KIND, int TM, int TN, int WM, int WN, int STAGES, int LOADERS = 0, bool F32 = false>
+__global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(BgArgs g) {
+  constexpr int BK = kBgDepth;
+  constexpr int kWaves = WM * WN, kLoading = LOADERS ? LOADERS : kWaves, FM = TM / WM / 16, FN = TN / WN / 16;
+  static_assert(FN % (F32 ? 2 : 4) == 0, "a wave stores whole lines");
+  using OpA = BgOperand<TM, BK, KIND != kGroupedDw, false, kLoading>;
+  using OpB = BgOperand<TN, BK, KIND == kGroupedDx, !F32, kLoading>;
+  constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes;
+  constexpr int kLoads = OpA::kLoads + OpB::kLoads, kLoadsA = OpA::kLoads, kStores = FM * FN / (F32 ? 1 : 2);
   extern __shared__ __align__(1024) unsigned char lds[];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t n_tiles = (g.cols + TN - 1u) / TN;
-  BgPlace place;
-  const uint32_t with_tail = KIND == kGroupedDw ? g.groups : g.groups + 1u;
-  auto per_group = [&](uint32_t, uint32_t size) {
-    return (KIND == kGroupedDw ? (g.rows + TM - 1u) / TM : (size + TM - 1u) / TM) * n_tiles;
-  };
-  if (!bg_place<64 * kWaves>(g, with_tail, reinterpret_cast<uint32_t*>(lds), per_group, place)) return;
-  // the row tiles of a group in bands of eight, in a band column by column: workgroups that run side by side share both operands
-  const uint32_t m_tiles = place.tiles / n_tiles, band = place.tile / (8u * n_tiles), in_band = place.tile - band * 8u * n_tiles;
-  const uint32_t band_tiles = m_tiles - band * 8u < 8u ? m_tiles - band * 8u : 8u;
-  const uint32_t tn = in_band / band_tiles, tm = band * 8u + in_band - tn * band_tiles;
-  const uint32_t row0 = tm * TM, col0 = tn * TN;
-  const uint32_t rows = (KIND == kGroupedDw ? g.rows : place.size) - row0;  // (at least one)
-  const bool tail = KIND != kGroupedDw && place.group == g.groups;
-  const uint32_t depth = KIND == kGroupedDw ? place.size : (tail ? 0u : g.depth);
+  BgTables tab;
+  uint32_t* scratch = reinterpret_cast<uint32_t*>(lds + STAGES * kStage);  // (not in the stages: some waves load while others still read it)
+  tab.start = scratch + kBgScratch;
+  tab.tile = tab.start + g.groups + 2u;
+  const uint32_t held = KIND == kGroupedDw ? g.groups : g.groups + 1u;
+  const BgShare share = bg_tables<64 * (kWaves + LOADERS)>(
+      g, held, tab, scratch,
+      [&](uint32_t rows) { return ((KIND == kGroupedDw ? g.rows : rows) + TM - 1u) / TM * n_tiles; },
+      // (a tile's results take about as long to store as three of its stages to compute)
+      [&](uint32_t group, uint32_t rows) { return 3u + bg_stages(KIND == kGroupedDw ? rows : (group < g.groups ? g.depth : 0u)); });
+  const uint32_t stride = gridDim.x >> 3, end = share.end;
+  uint32_t tile = share.first + (blockIdx.x >> 3);
+  if (tile >= end) return;
 
+  auto describe = [&](uint32_t t) {
+    BgTile d;
+    d.group = __builtin_amdgcn_readfirstlane(bg_group_of(tab.tile, held, t, lane));
+    d.start = __builtin_amdgcn_readfirstlane(tab.start[d.group]);
+    const uint32_t size = __builtin_amdgcn_readfirstlane(tab.start[d.group + 1u]) - d.start;
+    const uint32_t in_group = t - __builtin_amdgcn_readfirstlane(tab.tile[d.group]);
+    // the row tiles of a group in bands of eight, in a band column by column: workgroups that run side by side share both operands
+    const uint32_t m_tiles = ((KIND == kGroupedDw ? g.rows : size) + TM - 1u) / TM;
+    const uint32_t band = in_group / (8u * n_tiles), in_band = in_group - band * 8u * n_tiles;
+    const uint32_t band_tiles = m_tiles - band * 8u < 8u ? m_tiles - band * 8u : 8u;
+    const uint32_t tn = in_band / band_tiles;
+    d.row0 = (band * 8u + in_band - tn * band_tiles) * TM;
+    d.col0 = tn * TN;
+    d.rows = (KIND == kGroupedDw ? g.rows : size) - d.row0;
+    d.depth = KIND == kGroupedDw ? size : (d.group == g.groups ? 0u : g.depth);
+    return d;
+  };
   OpA a;
   OpB b;
-  if constexpr (KIND == kGroupedDw) {
-    a.init(g.a + (uint64_t)place.start * g.rows_ld + row0, g.rows_ld, rows, wave, lane);
-    b.init(g.b + (uint64_t)place.start * g.cols_ld + col0, g.cols_ld, g.cols - col0, wave, lane);
-  } else {
-    const uint16_t* w = g.b + (uint64_t)(tail ? 0u : place.group) * g.b_group;
-    a.init(g.a + (uint64_t)(place.start + row0) * g.rows_ld, g.rows_ld, rows, wave, lane);
-    b.init(w + (KIND == kGroupedFwd ? (uint64_t)col0 : (uint64_t)col0 * g.cols_ld), g.cols_ld, g.cols - col0, wave, lane);
-  }
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds;
-  constexpr uint32_t kStage = OpA::kBytes + OpB::kBytes, kStageLoads = OpA::kLoads + OpB::kLoads;
-  const uint32_t wm = wave / WN, wn = wave % WN;
-
-  v4f acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-
-  const uint32_t stages = (depth + BK - 1u) / BK;
-  auto request = [&](uint32_t s) {
-    const uint32_t at = lds0 + (s % STAGES) * kStage, left = depth - s * BK;  // (beyond the last stage: nothing is left)
-    const uint32_t l = s < stages ? left : 0u;
-    a.load(l, at, wave);
-    b.load(l, at + OpA::kBytes, wave);
-  };
-  // (a request beyond the last stage reads nothing and leaves zeros: every wave counts the same loads)
-  for (uint32_t s = 0; s + 1 < STAGES; ++s) request(s);
-  for (uint32_t s = 0; s < stages; ++s) {
-    wait_vmcnt<(STAGES - 2) * (int)kStageLoads>();
-    lds_barrier();
-    request(s + STAGES - 1);
-    const unsigned char* at = lds + (s % STAGES) * kStage;
-#pragma unroll
-    for (int step = 0; step < BK / 32; ++step) {
-      v8bf fa[FM], fb[FN];
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = OpB::fragment(at + OpA::kBytes, wn * (TN / WN), j, step, lane);
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = OpA::fragment(at, wm * (TM / WM), i, step, lane);
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+  a.init(g.rows_ld, lane);
+  b.init(g.cols_ld, lane);
+  uint32_t next_tile = tile, left = 0;  // of the stage that is requested next; left: contraction indices of its tile from there on
+  auto open = [&](uint32_t t) {
+    const BgTile d = describe(t);
+    left = d.depth;
+    if constexpr (KIND == kGroupedDw) {
+      a.open(g.a + (uint64_t)d.start * g.rows_ld + d.row0, d.rows);
+      b.open(g.b + (uint64_t)d.start * g.cols_ld + d.col0, g.cols - d.col0);
+    } else {
+      const uint16_t* w = g.b + (uint64_t)(d.group == g.groups ? 0u : d.group) * g.b_group;
+      a.open(g.a + (uint64_t)(d.start + d.row0) * g.rows_ld, d.rows);
+      b.open(w + (KIND == kGroupedFwd ? (uint64_t)d.col0 : (uint64_t)d.col0 * g.cols_ld), g.cols - d.col0);
     }
-  }
-  wait_vmcnt0();  // (no load into the LDS outlives the workgroup)
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds, loader = LOADERS ? wave - kWaves : wave;
+  auto request = [&](uint32_t s, int i) {
+    const uint32_t at = lds0 + (s % STAGES) * kStage;
+    if (i < kLoadsA) a.load(i, left, at, loader);
+    else b.load(i - kLoadsA, left, at + OpA::kBytes, loader);
+  };
+  auto request_all = [&](uint32_t s) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) request(s, i);
+  };
+  auto requested = [&] {  // on to the next stage; behind the last tile nothing is left: zeros, that every wave may count the same loads
+    if (left > (uint32_t)BK) {
+      left -= BK;
+      a.next();
+      b.next();
+      return;
+    }
+    next_tile += stride;
+    left = 0;
+    if (next_tile < end) open(next_tile);
+  };
 
-  const uint64_t out0 = KIND == kGroupedDw ? place.group * g.out_group : (uint64_t)place.start * g.cols;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const uint32_t r = wm * (TM / WM) + 16u * i + (lane & 15u);
-    if (r >= rows) continue;
-    const uint64_t at = out0 + (uint64_t)(row0 + r) * g.cols;
-#pragma unroll
-    for (int j = 0; j < FN; j += 2) {
-      const uint32_t c = col0 + wn * (TN / WN) + 32u * (j >> 1) + 8u * (lane >> 4);
-      if (c >= g.cols) continue;
-      if (KIND == kGroupedDw && g.f32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(g.out) + at + c);
-        p[0] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
-        p[1] = make_float4(acc[i][j + 1][0], acc[i][j + 1][1], acc[i][j + 1][2], acc[i][j + 1][3]);
-      } else {
-        uint4 v;  // the one rounding to bf16
-        v.x = pack_bf16x2(acc[i][j][0], acc[i][j][1]);
-        v.y = pack_bf16x2(acc[i][j][2], acc[i][j][3]);
-        v.z = pack_bf16x2(acc[i][j + 1][0], acc[i][j + 1][1]);
-        v.w = pack_bf16x2(acc[i][j + 1][2], acc[i][j + 1][3]);
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + at + c) = v;
+  if (LOADERS && wave >= kWaves) {
+    open(tile);
+    for (uint32_t s = 0; s < STAGES; ++s) {
+      request_all(s);
+      requested();
+    }
+    wait_vmcnt<(STAGES - 1) * kLoads>();
+    lds_barrier();
+    for (uint32_t s = 0; tile < end; tile += stride) {
+      for (const uint32_t last = s + bg_stages(describe(tile).depth); s < last; ++s) {
+        wait_vmcnt<(STAGES - 2) * kLoads>();
+        lds_barrier();
+        request_all(s + STAGES);
+        requested();
       }
     }
+    wait_vmcnt0();  // (no load into the LDS outlives the workgroup)
+    return;
   }
+
+  const uint32_t wm = wave / WN, wn = wave % WN;
+  v4f acc[FM][FN];
+  v8bf fa[2][FM], fb[2][FN];
+  auto fetch = [&](uint32_t s, int step, int f) {  // columns' fragments first
+    const unsigned char* at = lds + (s % STAGES) * kStage;
+    if (f < FN) fb[step][f] = OpB::fragment(at + OpA::kBytes, wn * (TN / WN), f, step, lane);
+    else fa[step][f - FN] = OpA::fragment(at, wm * (TM / WM), f - FN, step, lane);
+  };
+  // Half of a stage's products, and between them, so that neither waits for the other, the fragments of the next half out of the LDS
+  // and (LOAD) the requests of the stage after next.  A wave issues in order: with the reads and requests in front of
+  // the products both waves of a SIMD, which the barrier holds together, left the matrix unit idle meanwhile (32768 rows of 4096 ->
+  // 12288 in 8 groups 2840 us, 2660 this way).
+  auto half = [&](auto step_c, uint32_t s_fetch, auto load_c, uint32_t s_load, auto fresh_c) {  // FRESH: a tile's first sums
+    constexpr int step = step_c.value, next = 1 - step;
+    constexpr bool load = load_c.value, fresh = fresh_c.value;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l)
+        if (!LOADERS && load && l * FM / kLoads == i) request(s_load, l);
+#pragma unroll
+      for (int f = 0; f < FM + FN; ++f)
+        if (f * FM / (FM + FN) == i) fetch(s_fetch, next, f);
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[step][j], fa[step][i], fresh ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Eight neighbouring columns from two fragments, with the one rounding to bf16.  Lanes of odd lane / 16 hold the second four in the first.
+  auto rounded = [&](int i, int j) {
+    const bool odd = (lane >> 4) & 1u;
+    const int h0 = (int)pack_bf16x2(acc[i][j][0], acc[i][j][1]), h1 = (int)pack_bf16x2(acc[i][j][2], acc[i][j][3]);
+    const int k0 = (int)pack_bf16x2(acc[i][j + 1][0], acc[i][j + 1][1]), k1 = (int)pack_bf16x2(acc[i][j + 1][2], acc[i][j + 1][3]);
+    return v4i{odd ? k0 : h0, odd ? k1 : h1, odd ? h0 : k0, odd ? h1 : k1};
+  };
+  // Every wave stores the same number of times, lanes outside the tile's rows or columns beyond the buffer's end.  A lane holds 16
+  // bytes of either half of a row's 128-byte line; lanes eight rows apart exchange one, and an instruction stores eight whole lines.
+  auto store = [&](const BgTile& d) {
+    constexpr uint32_t size = F32 ? 4u : 2u, kLine = 128u / size;
+    const uint64_t at = (KIND == kGroupedDw ? d.group * g.out_group : (uint64_t)d.start * g.cols) + (uint64_t)d.row0 * g.cols + d.col0;
+    const v4i out = buffer_of(static_cast<unsigned char*>(g.out) + at * size);
+    const bool high = lane & 8u;
+    const uint32_t row = lane & 7u, col = (lane >> 4) * (16u / size) + (high ? kLine / 2u : 0u), voff = (row * g.cols + col) * size;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const uint32_t r0 = wm * (TM / WM) + 16u * i;
+#pragma unroll
+      for (uint32_t c0 = 0; c0 < TN / WN; c0 += kLine) {
+        v4i x, y;  // the halves of the line
+        if constexpr (F32) {
+          x = __builtin_bit_cast(v4i, acc[i][c0 / 16u]);
+          y = __builtin_bit_cast(v4i, acc[i][c0 / 16u + 1u]);
+        } else {
+          x = rounded(i, c0 / 16u);
+          y = rounded(i, c0 / 16u + 2u);
+        }
+        v4i mine, theirs;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          mine[v] = high ? y[v] : x[v];
+          theirs[v] = __builtin_amdgcn_update_dpp(0, high ? x[v] : y[v], 0x128, 0xf, 0xf, false);  // row_ror:8
+        }
+        v4i upper, lower;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          upper[v] = high ? theirs[v] : mine[v];
+          lower[v] = high ? mine[v] : theirs[v];
+        }
+        const uint32_t c = wn * (TN / WN) + c0, to = voff + (r0 * g.cols + c) * size;
+        const bool in_cols = (int)col < (int)(g.cols - d.col0 - c);
+        buffer_store_16(upper, out, in_cols && (int)row < (int)(d.rows - r0) ? to : kOutside);
+        buffer_store_16(lower, out, in_cols && (int)row < (int)(d.rows - r0 - 8u) ? to + 8u * g.cols * size : kOutside);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  constexpr std::integral_constant<int, 0> first{};
+  constexpr std::integral_constant<int, 1> second{};
+  if constexpr (!LOADERS) {
+    open(tile);
+    for (uint32_t s = 0; s < STAGES; ++s) {
+      request_all(s);
+      requested();
+    }
+    wait_vmcnt<(STAGES - 1) * kLoads>();
+  }
+  lds_barrier();
+#pragma unroll
+  for (int f = 0; f < FM + FN; ++f) fetch(0, 0, f);
+  bool stored = false;   // the stores of the tile before are the newest of what is on its way
+  for (uint32_t s = 0; tile < end; tile += stride) {
+    const BgTile d = describe(tile);
+    const uint32_t last = s + bg_stages(d.depth);
+    for (bool fresh = true; s < last; ++s, fresh = false) {
+      if (fresh) half(first, s, std::false_type{}, 0u, std::true_type{});
+      else half(first, s, std::false_type{}, 0u, std::false_type{});
+      // the one barrier of a stage: behind it the next stage has arrived for every wave, and nobody reads this one any more
+      if constexpr (!LOADERS) {
+        if (stored) wait_vmcnt<(STAGES - 2) * kLoads + kStores>();
+        else wait_vmcnt<(STAGES - 2) * kLoads>();
+        stored = false;
+      }
+      lds_barrier();
+      half(second, s + 1u, std::true_type{}, s + STAGES, std::false_type{});
+      if constexpr (!LOADERS) requested();
+    }
+    store(d);
+    stored = true;
+  }
+  if constexpr (!LOADERS) wait_vmcnt0();
 }
 
 }  // namespace w8a8

@@ -61,14 +61,15 @@ def _same_device(first: torch.Tensor, *others) -> None:
             raise ValueError(f"all operands must be on {first.device}, got {t.device}")
 
 
-def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Tensor) -> torch.Tensor:
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Tensor, *, flags: int = 0) -> torch.Tensor:
     """``out[rows of g] = bf16(x[rows of g] @ weight[g])`` with float32 sums: x bf16 [rows, K], weight bf16
-    [groups, K, N], group_sizes integers [groups].  Rows behind the last group are zero."""
+    [groups, K, N], group_sizes integers [groups].  Rows behind the last group are zero.  ``flags`` may force the tiles
+    (``_native.FLAG_BF16_GROUPED_TILE_*``); by default they follow the sizes."""
     xc, w = _bf16(x, "x"), _bf16(weight, "weight")
     _same_device(x, weight)
     m, k, n, g, sizes = _geometry(x, "x", 1, weight.shape, group_sizes)
     out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
-    p = _native.Bf16GroupedProblem(ctypes.sizeof(_native.Bf16GroupedProblem), 0, m, k, n, g, xc.data_ptr(), w.data_ptr(),
+    p = _native.Bf16GroupedProblem(ctypes.sizeof(_native.Bf16GroupedProblem), flags, m, k, n, g, xc.data_ptr(), w.data_ptr(),
                                    sizes.data_ptr(), out.data_ptr())
     with _on(x.device):
         status = _native.load().mi355_w8a8_bf16_grouped_v1(ctypes.byref(p), _stream_ptr(x.device))
@@ -77,7 +78,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Ten
 
 
 def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: torch.Tensor | None, group_sizes: torch.Tensor, *,
-                            need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.bfloat16):
+                            need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.bfloat16, flags: int = 0):
     """Cotangents ``(dx, dw)`` of ``grouped_matmul``: ``dx[rows of g] = bf16(dy[rows of g] @ weight[g].T)`` and
     ``dw[g] = x[rows of g].T @ dy[rows of g]`` in ``dw_dtype`` (bf16 or float32), both from float32 sums; None for the one
     that is not wanted.  ``x`` may be None without ``need_dw``, ``weight`` without ``need_dx``."""
@@ -98,7 +99,7 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=dy.device) if need_dx else None
     dw = torch.empty((g, k, n), dtype=dw_dtype, device=dy.device) if need_dw else None
     p = _native.Bf16GroupedBwdProblem(ctypes.sizeof(_native.Bf16GroupedBwdProblem),
-                                      _native.FLAG_BF16_GROUPED_DW_F32 if dw_dtype == torch.float32 else 0, m, k, n, g,
+                                      flags | (_native.FLAG_BF16_GROUPED_DW_F32 if dw_dtype == torch.float32 else 0), m, k, n, g,
                                       xc.data_ptr() if need_dw else None, d.data_ptr(), w.data_ptr() if need_dx else None,
                                       sizes.data_ptr(), dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None)
     with _on(dy.device):

@@ -53,10 +53,10 @@ def close(got, want, magnitudes, depth):
     assert not torch.isnan(got).any() and float(off.max()) <= 0.0, f"{float(off.max())} beyond at {int(off.argmax())}"
 
 
-def check(gl, x, w, dy, sizes_t, sizes, dw_dtype=torch.bfloat16):
+def check(gl, x, w, dy, sizes_t, sizes, dw_dtype=torch.bfloat16, flags=0):
     k, n = w.shape[1:]
-    close(gl.grouped_matmul(x, w, sizes_t), exact_forward(x, w, sizes), exact_forward(x.abs(), w.abs(), sizes), k)
-    dx, dw = gl.grouped_matmul_backward(x, dy, w, sizes_t, dw_dtype=dw_dtype)
+    close(gl.grouped_matmul(x, w, sizes_t, flags=flags), exact_forward(x, w, sizes), exact_forward(x.abs(), w.abs(), sizes), k)
+    dx, dw = gl.grouped_matmul_backward(x, dy, w, sizes_t, dw_dtype=dw_dtype, flags=flags)
     wt = w.transpose(1, 2)
     close(dx, exact_forward(dy, wt, sizes), exact_forward(dy.abs(), wt.abs(), sizes), n)
     assert dw.dtype == dw_dtype
@@ -83,6 +83,18 @@ def test_against_float64(gl, rows, k, n, sizes):
     check(gl, x, w, dy, st, sizes, torch.float32)
 
 
+@pytest.mark.parametrize("tile", ["256X256", "128X256", "64X128"])
+@pytest.mark.parametrize("rows,k,n,sizes", [
+    (1, 8, 8, [1]), (70, 200, 72, [0, 30, 5, 0, 35]), (257, 64, 264, [257]), (900, 328, 520, [3, 300, 0, 129, 40, 64, 65, 200]),
+    (3000, 136, 1000, [100, 900, 0, 1, 255, 256, 257, 700, 17, 300, 40, 60]),  # several tiles a workgroup
+    (2500, 1032, 2056, [7, 0, 1500, 600, 64, 128, 100]), (1100, 2056, 1544, [1] * 100 + [0] * 20 + [500, 400])])
+def test_each_tile(gl, rows, k, n, sizes, tile):
+    flags = getattr(load_package()._native, f"FLAG_BF16_GROUPED_TILE_{tile}")
+    x, w, dy, st = make(rows, k, n, sizes, seed=1)
+    check(gl, x, w, dy, st, sizes, flags=flags)
+    check(gl, x, w, dy, st, sizes, torch.float32, flags=flags)
+
+
 @pytest.mark.parametrize("sizes", [[0, 0, 0], [40, 200, 7], [-5, 40, -1], [1 << 30, 5, 1 << 30], [100, 0, 0]])
 def test_sizes_that_do_not_fit_the_rows(gl, sizes):
     x, w, dy, st = make(100, 96, 72, sizes)
@@ -96,16 +108,17 @@ def test_longest_depths(gl):
         check(gl, x, w, dy, st, sizes, torch.float32)
 
 
+@pytest.mark.parametrize("flags", [0, 4, 8, 16])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-def test_values_of_other_rows_stay_there(gl, bad):
+def test_values_of_other_rows_stay_there(gl, bad, flags):
     """A NaN or infinity in one group's rows or weight, or in rows of no group, reaches that group's results alone, also where K and
     the rows end inside a tile."""
     sizes = [30, 50, 0, 20]
     x, w, dy, st = make(120, 40, 72, sizes)
-    want, (wdx, wdw) = gl.grouped_matmul(x, w, st), gl.grouped_matmul_backward(x, dy, w, st)
+    want, (wdx, wdw) = gl.grouped_matmul(x, w, st, flags=flags), gl.grouped_matmul_backward(x, dy, w, st, flags=flags)
     x[30:80], dy[30:80], w[1], w[2] = bad, bad, bad, bad
     x[100:], dy[100:] = bad, bad
-    out, (dx, dw) = gl.grouped_matmul(x, w, st), gl.grouped_matmul_backward(x, dy, w, st)
+    out, (dx, dw) = gl.grouped_matmul(x, w, st, flags=flags), gl.grouped_matmul_backward(x, dy, w, st, flags=flags)
     for got, ref in ((out, want), (dx, wdx)):
         assert torch.equal(got[:30], ref[:30]) and torch.equal(got[80:], ref[80:]) and not torch.isfinite(got[30:80]).any()
         assert not got[100:].any()

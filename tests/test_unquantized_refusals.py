@@ -29,7 +29,7 @@ def fill(struct, **kw):
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(struct_size=8), -8), (dict(flags=1), -2), (dict(m=0), -2), (dict(n_groups=0), -2), (dict(k=12), -7), (dict(n=4), -7),
+    (dict(struct_size=8), -8), (dict(flags=1), -2), (dict(flags=12), -2), (dict(m=0), -2), (dict(n_groups=0), -2), (dict(k=12), -7), (dict(n=4), -7),
     (dict(k=65544), -7), (dict(n_groups=1025), -7), (dict(m=(1 << 20) + 1), -7), (dict(x=None), -1), (dict(weight=None), -1),
     (dict(group_sizes=None), -1), (dict(out=None), -1), (dict(x=A + 8), -3), (dict(weight=A + STEP + 2), -3),
     (dict(group_sizes=A + 2), -3), (dict(out=A + 16), -4), (dict(out=A + STEP + 1024), -4)])
