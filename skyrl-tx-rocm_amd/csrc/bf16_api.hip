@@ -79,6 +79,8 @@ int launch_grouped(const BgArgs& g, uint32_t forced, hipStream_t s) {
   if (forced == MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
   if (forced) return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
   const float large = cost(256u, 256u, 4.0f), middle = cost(128u, 256u, 2.2f), small = cost(64u, 128u, 1.15f);
+  // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 23 / 20.5)
+  if (KIND == kGroupedDw && large == 4.0f && g.m / g.groups < 8u * kBgDepth) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
   if (large <= middle && large <= small) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
   if (middle <= small) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
   return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
@@ -204,7 +206,7 @@ int run_embedding(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
 
 struct EmbedLayout {
   uint32_t passes, bits, chunks, run, runs;
-  uint64_t keys[2], tokens[2], counts, parts, total;
+  uint64_t keys[2], tokens[2], notes, counts, joins, parts, total;
 };
 
 // positions of a run: enough threads to fill the chip (2048 a CU) where the rows suffice, and no more parts than that
@@ -225,8 +227,10 @@ EmbedLayout embed_layout(uint32_t n, uint64_t rows, uint32_t width, uint32_t fla
     L.keys[i] = off; off += align256((uint64_t)n * 4u);
     L.tokens[i] = off; off += align256((uint64_t)n * 4u);
   }
+  L.notes = off; off += kEmbedNotes * 4u;
   L.counts = off;
-  if (L.chunks > kEmbedSortChunks) off += align256(((uint64_t)L.chunks + 1u) * (4u << L.bits));
+  if (L.chunks > 1u) off += align256(((uint64_t)L.chunks + 1u) * (4u << L.bits));
+  L.joins = off; off += align256((uint64_t)L.runs * 4u);
   L.parts = off; off += align256((uint64_t)L.runs * 2u * width * 4u);
   L.total = off;
   return L;
@@ -234,11 +238,15 @@ EmbedLayout embed_layout(uint32_t n, uint64_t rows, uint32_t width, uint32_t fla
 
 template <typename T, int V>
 int launch_embed_sums(const EmbedSumArgs& a, hipStream_t s) {
-  const dim3 grid(blocks_of((uint64_t)a.runs * (a.e.width / V))), block(256);
-  hipLaunchKernelGGL((embed_sum_kernel<T, V>), grid, block, 0, s, a);
+  const uint32_t units = a.e.width / V;
+  const dim3 block(256);
+  const dim3 grid(blocks_of((uint64_t)a.runs * (units >= 64u ? (units + 63u) / 64u * 64u : units)));
+  if (units >= 64u) hipLaunchKernelGGL((embed_sum_kernel<T, V, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((embed_sum_kernel<T, V, false>), grid, block, 0, s, a);
   const int st = launch_status();
   if (st || a.runs < 2u) return st;
-  hipLaunchKernelGGL((embed_join_kernel<T, V>), grid, block, 0, s, a);
+  const uint64_t most = ((uint64_t)a.runs * units + 255u) / 256u;
+  hipLaunchKernelGGL((embed_join_kernel<T, V>), dim3((uint32_t)(most < 2048u ? most : 2048u)), block, 0, s, a);
   return launch_status();
 }
 
@@ -256,44 +264,61 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
       overlaps(p->workspace, L.total, p->d_out, dy_bytes) || overlaps_indices(p, p->workspace, L.total))
     return MI355_W8A8_ERR_ALIAS;
   unsigned char* ws = static_cast<unsigned char*>(p->workspace);
+  auto words = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
   EmbedSortArgs a{};
   a.e = embed_args(p);
-  a.digits = 1u << L.bits;
-  a.chunks = L.chunks;
-  a.counts = reinterpret_cast<uint32_t*>(ws + L.counts);
-  const uint32_t sort_lds = (2u * kEmbedDigits + 16u) * 4u + 16u * a.digits * 2u, place_lds = kEmbedDigits * 4u + 16u * a.digits * 2u;
-  if (!allow_lds(&embed_sort_kernel, sort_lds) || !allow_lds(&embed_place_kernel, place_lds)) return MI355_W8A8_ERR_LAUNCH;
-  // every pass clears its share of the gradient
-  const uint64_t pieces = out_bytes / 16u, share = pieces / L.passes;
-  (void)hipGetLastError();
-  for (uint32_t pass = 0; pass < L.passes; ++pass) {
-    a.keys = pass ? reinterpret_cast<uint32_t*>(ws + L.keys[(pass - 1u) & 1u]) : nullptr;
-    a.tokens = pass ? reinterpret_cast<uint32_t*>(ws + L.tokens[(pass - 1u) & 1u]) : nullptr;
-    a.keys_out = reinterpret_cast<uint32_t*>(ws + L.keys[pass & 1u]);
-    a.tokens_out = reinterpret_cast<uint32_t*>(ws + L.tokens[pass & 1u]);
-    a.shift = pass * L.bits;
-    const bool last = pass + 1u == L.passes;
-    a.clear = static_cast<uint4*>(p->out) + pass * share;
-    a.clear_pieces = last ? pieces - pass * share : share;
+  a.bits = L.bits; a.passes = L.passes; a.chunks = L.chunks;
+  a.notes = words(L.notes);
+  // the launches that place the keys clear a share of the gradient each
+  const uint64_t pieces = out_bytes / 16u;
+  const bool small = L.chunks == 1u;
+  const uint32_t launches = small ? 1u : L.passes;
+  uint32_t launched = 0, clearing = 0;
+  auto share = [&] {
+    const uint64_t each = pieces / launches;
+    const bool last = launched + 1u == launches;
+    a.clear = static_cast<uint4*>(p->out) + launched * each;
+    a.clear_pieces = last ? pieces - launched * each : each;
     a.clear_rest = last ? (uint32_t)(out_bytes % 16u) : 0u;
-    const uint64_t wanted = (a.clear_pieces + 4095u) / 4096u + 1u;
-    const uint32_t clearing = (uint32_t)(wanted < 2048u ? wanted : 2048u);
-    if (L.chunks <= kEmbedSortChunks) {
-      hipLaunchKernelGGL(embed_sort_kernel, dim3(L.chunks + clearing), dim3(1024), sort_lds, s, a);
+    const uint64_t wanted = (a.clear_pieces + 4095u) / 4096u + (a.clear_rest ? 1u : 0u);
+    clearing = (uint32_t)(wanted < 2048u ? wanted : 2048u);
+    ++launched;
+  };
+  const uint32_t place_lds = (kEmbedDigits + 16u) * 4u + (32u << L.bits), small_lds = place_lds + 8192u;
+  (void)hipGetLastError();
+  if (small) {
+    if (!allow_lds(&embed_sort_small_kernel, small_lds)) return MI355_W8A8_ERR_LAUNCH;
+    a.keys_out = words(L.keys[0]); a.tokens_out = words(L.tokens[0]);
+    share();
+    hipLaunchKernelGGL(embed_sort_small_kernel, dim3(1u + clearing), dim3(1024), small_lds, s, a);
+    if ((st = launch_status())) return st;
+  } else {
+    const bool scan = L.chunks > kEmbedSumChunks;
+    if (!allow_lds(&embed_place_kernel<true>, place_lds) || !allow_lds(&embed_place_kernel<false>, place_lds)) return MI355_W8A8_ERR_LAUNCH;
+    a.counts = words(L.counts);
+    for (uint32_t pass = 0; pass < L.passes; ++pass) {
+      a.keys = pass ? words(L.keys[(pass - 1u) & 1u]) : nullptr;
+      a.tokens = pass ? words(L.tokens[(pass - 1u) & 1u]) : nullptr;
+      a.keys_out = words(L.keys[pass & 1u]);
+      a.tokens_out = words(L.tokens[pass & 1u]);
+      a.shift = pass * L.bits;
+      hipLaunchKernelGGL(embed_count_kernel, dim3(L.chunks), dim3(1024), 0, s, a);
       if ((st = launch_status())) return st;
-      continue;
+      if (scan) {
+        hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, s, a);
+        if ((st = launch_status())) return st;
+      }
+      share();
+      if (scan) hipLaunchKernelGGL(embed_place_kernel<true>, dim3(L.chunks + clearing), dim3(1024), place_lds, s, a);
+      else hipLaunchKernelGGL(embed_place_kernel<false>, dim3(L.chunks + clearing), dim3(1024), place_lds, s, a);
+      if ((st = launch_status())) return st;
     }
-    hipLaunchKernelGGL(embed_count_kernel, dim3(L.chunks + clearing), dim3(1024), 0, s, a);
-    if ((st = launch_status())) return st;
-    hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, s, a);
-    if ((st = launch_status())) return st;
-    hipLaunchKernelGGL(embed_place_kernel, dim3(L.chunks), dim3(1024), place_lds, s, a);
-    if ((st = launch_status())) return st;
   }
   EmbedSumArgs b{};
   b.e = a.e;
   b.keys = a.keys_out; b.tokens = a.tokens_out;
   b.parts = reinterpret_cast<float*>(ws + L.parts);
+  b.joins = words(L.joins); b.notes = a.notes;
   b.run = L.run; b.runs = L.runs;
   const bool wide = p->width % (16u / size) == 0 && aligned(p->d_out, 16);
   if (size == 4u) return wide ? launch_embed_sums<float, 4>(b, s) : launch_embed_sums<float, 1>(b, s);

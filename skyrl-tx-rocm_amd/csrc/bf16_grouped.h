@@ -70,9 +70,11 @@ __device__ inline v4i buffer_of(const void* base_uniform) {
 
 // (The offset comes in the lanes' registers alone: behind a 16-byte store with a scalar offset the compiler lets the next instruction
 // write the data's registers, and the memory then got what that instruction wrote.  Without one it keeps the wait states.)
+// STREAM: past the caches (non-temporal).
+template <bool STREAM>
 __device__ inline void buffer_store_16(v4i v, v4i rsrc, uint32_t voff) {
   void* base = reinterpret_cast<void*>((uint64_t)(uint32_t)rsrc[0] | (uint64_t)(uint32_t)rsrc[1] << 32);
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), __builtin_amdgcn_make_buffer_rsrc(base, 0, rsrc[2], rsrc[3]), (int)voff, 0, 2);
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), __builtin_amdgcn_make_buffer_rsrc(base, 0, rsrc[2], rsrc[3]), (int)voff, 0, STREAM ? 2 : 0);
 }
 
 // (a tile without products has one stage, of zeros)
@@ -402,6 +404,10 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
     constexpr uint32_t size = F32 ? 4u : 2u, kLine = 128u / size;
     const uint64_t at = (KIND == kGroupedDw ? d.group * g.out_group : (uint64_t)d.start * g.cols) + (uint64_t)d.row0 * g.cols + d.col0;
     const v4i out = buffer_of(static_cast<unsigned char*>(g.out) + at * size);
+    // A dW is larger than the caches and leaves x and dy there no room: it is streamed where its rows are whole lines (us, streamed /
+    // not, 768 -> 2048, 128 groups, 32768 rows: bf16 162 / 184, float32 205 / 269; parts of lines are not joined on that way: 712 ->
+    // 1096, 13 groups, 1003 rows, float32 28 / 23).
+    const bool stream = KIND == kGroupedDw && g.cols * size % 128u == 0u;
     const bool high = lane & 8u;
     const uint32_t row = lane & 7u, col = (lane >> 4) * (16u / size) + (high ? kLine / 2u : 0u), voff = (row * g.cols + col) * size;
 #pragma unroll
@@ -431,8 +437,15 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
         }
         const uint32_t c = wn * (TN / WN) + c0, to = voff + (r0 * g.cols + c) * size;
         const bool in_cols = (int)col < (int)(g.cols - d.col0 - c);
-        buffer_store_16(upper, out, in_cols && (int)row < (int)(d.rows - r0) ? to : kOutside);
-        buffer_store_16(lower, out, in_cols && (int)row < (int)(d.rows - r0 - 8u) ? to + 8u * g.cols * size : kOutside);
+        const uint32_t to_upper = in_cols && (int)row < (int)(d.rows - r0) ? to : kOutside;
+        const uint32_t to_lower = in_cols && (int)row < (int)(d.rows - r0 - 8u) ? to + 8u * g.cols * size : kOutside;
+        if (stream) {
+          buffer_store_16<true>(upper, out, to_upper);
+          buffer_store_16<true>(lower, out, to_lower);
+        } else {
+          buffer_store_16<false>(upper, out, to_upper);
+          buffer_store_16<false>(lower, out, to_lower);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }

@@ -7,12 +7,14 @@
 // forward gives zeros, the backward leaves the token out.
 //
 //   embed_rows_kernel          a thread per 16 bytes of the output
-//   embed_sort_kernel          one stable pass of a radix sort of the rows' numbers; its other workgroups clear the gradient
+//   embed_sort_small_kernel    up to 1024 tokens: a stable radix sort of the rows' numbers in one launch
+//   embed_count_kernel, embed_scan_kernel, embed_place_kernel   more of them: the digits counted, and a launch a digit (the scan
+//                              where there are many chunks); workgroups beside those of the sort clear the gradient meanwhile
 //   embed_sum_kernel           a thread per (run of positions of the sorted order, 16 bytes of a row): the sums of the rows that begin
 //                              and end inside a run are written, the others' parts are left in the workspace
-//   embed_join_kernel          rows that reach over several runs: their parts in order
+//   embed_join_kernel          rows that reach over several runs: their parts
 //
-// Sums are float32 in the order of the tokens: the same bits at every call.
+// Sums are float32 in a fixed order of the tokens: the same bits at every call.
 #pragma once
 #include "w8a8_device.h"
 
@@ -95,7 +97,9 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs e) {
 // ---------------------------------------------------------------------------------------
 constexpr uint32_t kEmbedChunk = 1024;      // keys a workgroup places
 constexpr uint32_t kEmbedDigits = 2048;     // most values of one digit
-constexpr uint32_t kEmbedSortChunks = 64;   // up to here a workgroup counts all keys for itself
+constexpr uint32_t kEmbedSumChunks = 64;    // up to here a workgroup adds up the chunks' counts for itself
+constexpr uint32_t kEmbedNotes = 64;        // words in front of the counts; the first: rows of many parts
+constexpr uint32_t kEmbedShort = 8;         // parts that a thread of the join adds up by itself
 
 struct EmbedSortArgs {
   EmbedArgs e;
@@ -103,8 +107,9 @@ struct EmbedSortArgs {
   const uint32_t* tokens;
   uint32_t* keys_out;
   uint32_t* tokens_out;
-  uint32_t* counts;         // [chunks][digits], where the counting has launches of its own
-  uint32_t shift, digits, chunks;
+  uint32_t* counts;         // [chunks + 1][digits] of this pass: keys of a chunk with a digit; behind a scan the keys in front of them
+  uint32_t* notes;          // [kEmbedNotes]
+  uint32_t shift, bits, chunks, passes;
   uint4* clear;             // the share of the gradient that this launch clears, in 16-byte pieces, and the bytes behind the last one
   uint64_t clear_pieces;
   uint32_t clear_rest;
@@ -118,34 +123,28 @@ __device__ inline void embed_clear(const EmbedSortArgs& a, uint32_t block, uint3
   if (block == 0 && threadIdx.x < a.clear_rest) reinterpret_cast<unsigned char*>(a.clear + a.clear_pieces)[threadIdx.x] = 0;
 }
 
-// Place of a key: keys of smaller digits, keys of its digit in earlier chunks (both in first[digit]), in earlier waves of its
-// chunk, in earlier lanes of its wave.  A wave finds the lanes that share a digit with one ballot a bit.
-__device__ inline void embed_place(const EmbedSortArgs& a, uint32_t chunk, const uint32_t* first, uint16_t* wave_cnt) {
+// Keys of a chunk in front of this thread's with the same digit: in earlier waves, and in earlier lanes of its wave.  A wave finds the
+// lanes that share a digit with one ballot a bit.  wave_cnt: [16][digits].
+__device__ inline uint32_t embed_rank(uint32_t d, bool valid, uint32_t digits, uint16_t* wave_cnt) {
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const uint32_t words = 16u * a.digits / 2u;
-  for (uint32_t i = tid; i < words; i += 1024u) reinterpret_cast<uint32_t*>(wave_cnt)[i] = 0;
+  for (uint32_t i = tid; i < 8u * digits; i += 1024u) reinterpret_cast<uint32_t*>(wave_cnt)[i] = 0;
   __syncthreads();
-  const uint32_t p = chunk * kEmbedChunk + tid;
-  const bool valid = p < a.e.n;
-  const uint32_t key = valid ? embed_key(a, p) : 0u, d = (key >> a.shift) & (a.digits - 1u);
   unsigned long long same = __builtin_amdgcn_ballot_w64(valid);
-  for (uint32_t bit = 1u; bit < a.digits; bit <<= 1) {
+  for (uint32_t bit = 1u; bit < digits; bit <<= 1) {
     const bool one = d & bit;
     const unsigned long long ones = __builtin_amdgcn_ballot_w64(one);
     same &= one ? ones : ~ones;
   }
-  const uint32_t rank = (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
-  if (valid && rank == 0) wave_cnt[wave * a.digits + d] = (uint16_t)__builtin_popcountll(same);
+  const uint32_t in_wave = (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1ull));
+  if (valid && in_wave == 0) wave_cnt[wave * digits + d] = (uint16_t)__builtin_popcountll(same);
   __syncthreads();
-  if (!valid) return;
-  uint32_t at = first[d] + rank;
+  uint32_t rank = in_wave;
 #pragma unroll
   for (uint32_t w = 0; w < 16; ++w) {
-    const uint32_t c = wave_cnt[w * a.digits + d];
-    at += w < wave ? c : 0u;
+    const uint32_t c = wave_cnt[w * digits + d];
+    rank += w < wave ? c : 0u;
   }
-  a.keys_out[at] = key;
-  a.tokens_out[at] = a.keys ? a.tokens[p] : p;
+  return rank;
 }
 
 // exclusive prefix over values 2 tid, 2 tid + 1 of the workgroup's 1024 threads
@@ -161,61 +160,70 @@ __device__ inline void embed_prefix(uint32_t (&v)[2], uint32_t* waves) {
   v[0] = before;
 }
 
-// The whole pass in one launch: every chunk's workgroup counts all keys, those of earlier chunks apart.  Workgroups behind the
-// chunks clear their share of the gradient meanwhile.
-__global__ __launch_bounds__(1024) void embed_sort_kernel(EmbedSortArgs a) {
+// Up to one chunk of keys: all passes in the LDS, in one launch.
+__global__ __launch_bounds__(1024) void embed_sort_small_kernel(EmbedSortArgs a) {
   extern __shared__ __align__(16) unsigned char lds[];
-  if (blockIdx.x >= a.chunks) return embed_clear(a, blockIdx.x - a.chunks, gridDim.x - a.chunks);
-  uint32_t* all = reinterpret_cast<uint32_t*>(lds);   // keys of a digit; then the first place of this chunk's
-  uint32_t* earlier = all + kEmbedDigits;
-  uint32_t* waves = earlier + kEmbedDigits;
-  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(waves + 16);
-  const uint32_t tid = threadIdx.x, chunk = blockIdx.x;
-  for (uint32_t i = tid; i < kEmbedDigits; i += 1024u) all[i] = earlier[i] = 0;
-  __syncthreads();
-#pragma unroll 4
-  for (uint32_t c = 0; c < a.chunks; ++c) {
-    const uint32_t p = c * kEmbedChunk + tid;
-    const uint32_t d = (embed_key(a, p < a.e.n ? p : a.e.n - 1u) >> a.shift) & (a.digits - 1u);
-    if (p < a.e.n) {
-      atomicAdd(&all[d], 1u);
-      if (c < chunk) atomicAdd(&earlier[d], 1u);
+  if (blockIdx.x >= 1u) return embed_clear(a, blockIdx.x - 1u, gridDim.x - 1u);
+  uint32_t* all = reinterpret_cast<uint32_t*>(lds);   // keys of a digit, then those of smaller ones
+  uint32_t* waves = all + kEmbedDigits;
+  uint32_t* moved = waves + 16;                       // [2][1024] keys and tokens in their new order
+  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(moved + 2048);
+  const uint32_t tid = threadIdx.x, digits = 1u << a.bits;
+  if (tid < kEmbedNotes) a.notes[tid] = 0;
+  const bool valid = tid < a.e.n;
+  uint32_t key = valid ? embed_row(a.e, tid) : 0u, token = tid;
+  for (uint32_t pass = 0; pass < a.passes; ++pass) {
+    const uint32_t d = (key >> (pass * a.bits)) & (digits - 1u);
+    all[tid] = all[tid + 1024u] = 0;
+    const uint32_t rank = embed_rank(d, valid, digits, wave_cnt);  // (its barriers: all is clear, the keys are read)
+    if (valid) atomicAdd(&all[d], 1u);
+    __syncthreads();
+    uint32_t v[2] = {all[2 * tid], all[2 * tid + 1]};
+    embed_prefix(v, waves);
+    all[2 * tid] = v[0];
+    all[2 * tid + 1] = v[1];
+    __syncthreads();
+    if (valid) {
+      const uint32_t at = all[d] + rank;
+      moved[at] = key;
+      moved[1024u + at] = token;
     }
+    __syncthreads();
+    key = moved[tid];
+    token = moved[1024u + tid];
   }
-  __syncthreads();
-  uint32_t v[2] = {all[2 * tid], all[2 * tid + 1]};
-  embed_prefix(v, waves);
-  all[2 * tid] = v[0] + earlier[2 * tid];
-  all[2 * tid + 1] = v[1] + earlier[2 * tid + 1];
-  __syncthreads();
-  embed_place(a, chunk, all, wave_cnt);
+  if (valid) {
+    a.keys_out[tid] = key;
+    a.tokens_out[tid] = token;
+  }
 }
 
-// The same in three launches for more chunks: counts of every chunk, their prefix over the chunks, the places.
+// A pass' digits, chunk by chunk.
 __global__ __launch_bounds__(1024) void embed_count_kernel(EmbedSortArgs a) {
   __shared__ uint32_t cnt[kEmbedDigits];
-  if (blockIdx.x >= a.chunks) return embed_clear(a, blockIdx.x - a.chunks, gridDim.x - a.chunks);
-  const uint32_t tid = threadIdx.x, chunk = blockIdx.x;
-  for (uint32_t i = tid; i < kEmbedDigits; i += 1024u) cnt[i] = 0;
+  const uint32_t tid = threadIdx.x, chunk = blockIdx.x, digits = 1u << a.bits;
+  if (chunk == 0 && tid < kEmbedNotes) a.notes[tid] = 0;
+  cnt[tid] = cnt[tid + 1024u] = 0;
   __syncthreads();
   const uint32_t p = chunk * kEmbedChunk + tid;
-  if (p < a.e.n) atomicAdd(&cnt[(embed_key(a, p) >> a.shift) & (a.digits - 1u)], 1u);
+  if (p < a.e.n) atomicAdd(&cnt[(embed_key(a, p) >> a.shift) & (digits - 1u)], 1u);
   __syncthreads();
-  for (uint32_t i = tid; i < a.digits; i += 1024u) a.counts[(uint64_t)chunk * a.digits + i] = cnt[i];
+  for (uint32_t i = tid; i < digits; i += 1024u) a.counts[((uint64_t)chunk << a.bits) + i] = cnt[i];
 }
+// Many chunks: their counts become the keys of the digit in earlier chunks, and behind them the keys of smaller digits.
 __global__ __launch_bounds__(1024) void embed_scan_kernel(EmbedSortArgs a) {
   __shared__ uint32_t waves[16];
-  const uint32_t tid = threadIdx.x;
+  const uint32_t tid = threadIdx.x, digits = 1u << a.bits;
   uint32_t v[2] = {0u, 0u};
 #pragma unroll
   for (uint32_t h = 0; h < 2; ++h) {
     const uint32_t d = 2u * tid + h;
-    if (d >= a.digits) continue;
+    if (d >= digits) continue;
     uint32_t run = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (uint32_t c = 0; c < a.chunks; ++c) {
-      const uint32_t t = a.counts[(uint64_t)c * a.digits + d];
-      a.counts[(uint64_t)c * a.digits + d] = run;
+      const uint32_t t = a.counts[((uint64_t)c << a.bits) + d];
+      a.counts[((uint64_t)c << a.bits) + d] = run;
       run += t;
     }
     v[h] = run;
@@ -223,16 +231,45 @@ __global__ __launch_bounds__(1024) void embed_scan_kernel(EmbedSortArgs a) {
   embed_prefix(v, waves);
 #pragma unroll
   for (uint32_t h = 0; h < 2; ++h)
-    if (2u * tid + h < a.digits) a.counts[(uint64_t)a.chunks * a.digits + 2u * tid + h] = v[h];
+    if (2u * tid + h < digits) a.counts[((uint64_t)a.chunks << a.bits) + 2u * tid + h] = v[h];
 }
+// Every key to its place.
+template <bool SCANNED>
 __global__ __launch_bounds__(1024) void embed_place_kernel(EmbedSortArgs a) {
   extern __shared__ __align__(16) unsigned char lds[];
+  if (blockIdx.x >= a.chunks) return embed_clear(a, blockIdx.x - a.chunks, gridDim.x - a.chunks);
   uint32_t* first = reinterpret_cast<uint32_t*>(lds);
-  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(first + kEmbedDigits);
-  for (uint32_t i = threadIdx.x; i < a.digits; i += 1024u)
-    first[i] = a.counts[(uint64_t)a.chunks * a.digits + i] + a.counts[(uint64_t)blockIdx.x * a.digits + i];
-  __syncthreads();
-  embed_place(a, blockIdx.x, first, wave_cnt);
+  uint32_t* waves = first + kEmbedDigits;
+  uint16_t* wave_cnt = reinterpret_cast<uint16_t*>(waves + 16);
+  const uint32_t tid = threadIdx.x, chunk = blockIdx.x, digits = 1u << a.bits;
+  const uint32_t p = chunk * kEmbedChunk + tid;
+  const bool valid = p < a.e.n;
+  const uint32_t key = valid ? embed_key(a, p) : 0u, d = (key >> a.shift) & (digits - 1u);
+  if (SCANNED) {
+    for (uint32_t i = tid; i < digits; i += 1024u)
+      first[i] = a.counts[((uint64_t)a.chunks << a.bits) + i] + a.counts[((uint64_t)chunk << a.bits) + i];
+  } else {
+    uint32_t v[2] = {0u, 0u}, earlier[2] = {0u, 0u};
+    if (2u * tid < digits) {
+      const uint2* row = reinterpret_cast<const uint2*>(a.counts) + tid;
+#pragma unroll 8
+      for (uint32_t c = 0; c < a.chunks; ++c) {
+        const uint2 t = row[(uint64_t)c << (a.bits - 1u)];
+        v[0] += t.x;
+        v[1] += t.y;
+        earlier[0] += c < chunk ? t.x : 0u;
+        earlier[1] += c < chunk ? t.y : 0u;
+      }
+    }
+    embed_prefix(v, waves);
+    first[2 * tid] = v[0] + earlier[0];
+    first[2 * tid + 1] = v[1] + earlier[1];
+  }
+  const uint32_t rank = embed_rank(d, valid, digits, wave_cnt);  // (behind its barriers `first` is whole)
+  if (!valid) return;
+  const uint32_t at = first[d] + rank;
+  a.keys_out[at] = key;
+  a.tokens_out[at] = a.keys ? a.tokens[p] : p;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -241,55 +278,60 @@ struct EmbedSumArgs {
   const uint32_t* keys;    // [n], sorted
   const uint32_t* tokens;
   float* parts;            // [runs][2][width]: of a row that reaches into the run, of one that begins in it and reaches out
+  uint32_t* joins;         // [runs] runs whose last row begins in them and has more than kEmbedShort parts, in any order
+  uint32_t* notes;         // the first: how many
   uint32_t run, runs;      // positions of a run
 };
 
 __device__ inline float embed_scale(const EmbedArgs& e, uint32_t row) { return e.scales ? e.scales[row / e.vocab] : e.scale; }
 
-template <typename T, int V>
-__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSumArgs a) {
-  const uint32_t units = a.e.width / V;
-  const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-  const uint32_t r = (uint32_t)(i / units), u = (uint32_t)(i - (uint64_t)r * units);
-  if (r >= a.runs) return;
+// Sums of unit u of run r's rows.  WIDE: the run is the wave's, so that its keys and tokens come by scalar loads.
+template <typename T, int V, bool WIDE>
+__device__ inline void embed_sum_run(const EmbedSumArgs& a, uint32_t r, uint32_t u) {
   const uint32_t none = a.e.n_adapters * a.e.vocab;
   const uint32_t p0 = r * a.run, p1 = p0 + a.run < a.e.n ? p0 + a.run : a.e.n;
-  const T* dy = static_cast<const T*>(a.e.dy);
-  T* out = static_cast<T*>(a.e.out);
+  const T* dy = static_cast<const T*>(a.e.dy) + u * V;
+  T* out = static_cast<T*>(a.e.out) + u * V;
   float sum[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-  uint32_t key = a.keys[p0];
-  bool from_before = p0 > 0 && a.keys[p0 - 1u] == key;
+  const uint32_t behind = p1 < a.e.n ? a.keys[p1] : none + 1u;
+  bool from_before = p0 > 0 && a.keys[p0 - 1u] == a.keys[p0];
   // eight positions at a time: their rows are on the way together
   for (uint32_t p = p0; p < p1; p += 8u) {
-    uint32_t k[9];
+    uint32_t k[9], t[8];
     float f[8][V];
 #pragma unroll
     for (uint32_t x = 0; x < 8; ++x) {
       const uint32_t at = p + x < p1 ? p + x : p1 - 1u;
       k[x] = a.keys[at];
-      EmbedUnit<T, V>::load(dy + (uint64_t)a.tokens[at] * a.e.width + u * V, f[x]);
+      t[x] = a.tokens[at];
     }
-    k[8] = p + 8u < a.e.n ? a.keys[p + 8u] : none + 1u;
+    k[8] = p + 8u < p1 ? a.keys[p + 8u] : behind;
+#pragma unroll
+    for (uint32_t x = 0; x < 8; ++x) EmbedUnit<T, V>::load(dy + (uint64_t)t[x] * a.e.width, f[x]);
 #pragma unroll
     for (uint32_t x = 0; x < 8; ++x) {
       if (p + x >= p1) break;
 #pragma unroll
       for (int j = 0; j < V; ++j) sum[j] += f[x][j];
       const bool last = p + x + 1u == p1;
-      const uint32_t next = last ? (p1 < a.e.n ? a.keys[p1] : none + 1u) : k[x + 1];
+      const uint32_t next = last ? behind : k[x + 1];
       if (next == k[x] && !last) continue;
       if (k[x] < none) {
         if (from_before || next == k[x]) {
           float* part = a.parts + ((uint64_t)r * 2u + (from_before ? 0u : 1u)) * a.e.width + u * V;
 #pragma unroll
           for (int j = 0; j < V; ++j) part[j] = sum[j];
+          if (!from_before && u == 0) {
+            const uint64_t far = (uint64_t)(r + kEmbedShort) * a.run;
+            if (far < a.e.n && a.keys[far] == k[x]) a.joins[atomicAdd(a.notes, 1u)] = r;
+          }
         } else {
           const float s = embed_scale(a.e, k[x]);
 #pragma unroll
           for (int j = 0; j < V; ++j) sum[j] *= s;
-          EmbedUnit<T, V>::store(out + (uint64_t)k[x] * a.e.width + u * V, sum);
+          EmbedUnit<T, V>::store(out + (uint64_t)k[x] * a.e.width, sum);
         }
       }
       from_before = false;
@@ -299,37 +341,90 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSumArgs a) {
   }
 }
 
-// Run r's last row, where it begins in r and goes on behind it: its part there and one of every run that it reaches into.
+template <typename T, int V, bool WIDE>
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedSumArgs a) {
+  const uint32_t units = a.e.width / V;
+  if (WIDE) {  // a wave: 64 units of one run
+    const uint32_t waves = (units + 63u) / 64u, w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
+    const uint32_t r = w / waves, u = (w - r * waves) * 64u + (threadIdx.x & 63u);
+    if (r < a.runs && u < units) embed_sum_run<T, V, true>(a, r, u);
+  } else {
+    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    const uint32_t r = (uint32_t)(i / units), u = (uint32_t)(i - (uint64_t)r * units);
+    if (r < a.runs) embed_sum_run<T, V, false>(a, r, u);
+  }
+}
+
+// The rows that reach over several runs.  Few parts: a thread adds up its unit's, all requested together.  Many: a workgroup takes
+// 16 units, each of a unit's sixteen threads a sixteenth of the parts, then theirs in order.  (A thread for every row walks the 160
+// parts of a padding word one after the other, 33 us; a workgroup for every row with two parts is 28 us of dependent loads.)
 template <typename T, int V>
 __global__ __launch_bounds__(256) void embed_join_kernel(EmbedSumArgs a) {
+  __shared__ float lds[16][16][V];
   const uint32_t units = a.e.width / V;
-  const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-  const uint32_t r = (uint32_t)(i / units), u = (uint32_t)(i - (uint64_t)r * units);
-  if (r + 1u >= a.runs) return;
-  const uint32_t p0 = r * a.run, end = p0 + a.run;  // (a run follows: this one is whole)
-  const uint32_t key = a.keys[end];
-  if (a.keys[end - 1u] != key || key >= a.e.n_adapters * a.e.vocab) return;
-  if (p0 > 0 && a.keys[p0 - 1u] == key) return;  // begins earlier
-  float sum[V];
+  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < (uint64_t)(a.runs - 1u) * units; i += (uint64_t)gridDim.x * 256u) {
+    const uint32_t r = (uint32_t)(i / units), u = (uint32_t)(i - (uint64_t)r * units);
+    const uint32_t end = (r + 1u) * a.run, key = a.keys[end], last = a.keys[end - 1u];  // (a run follows: this one is whole)
+    const uint32_t before = r ? a.keys[r * a.run - 1u] : key + 1u;
+    const uint64_t far = (uint64_t)(r + kEmbedShort) * a.run;
+    if (last != key || before == key || key >= a.e.n_adapters * a.e.vocab || (far < a.e.n && a.keys[far] == key)) continue;
+    float f[kEmbedShort][V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) sum[j] = a.parts[((uint64_t)r * 2u + 1u) * a.e.width + u * V + j];
-  // last position of the row, by bisection: lo holds the key, hi does not
-  uint32_t lo = end, hi = a.e.n;
-  while (hi - lo > 1u) {
-    const uint32_t mid = lo + (hi - lo) / 2u;
-    if (a.keys[mid] == key) lo = mid; else hi = mid;
+    for (uint32_t x = 0; x < kEmbedShort; ++x) {
+      const uint64_t at = (uint64_t)(r + x) * a.run;
+      const bool held = x < 2u || (at < a.e.n && a.keys[at] == key);
+      const float* part = a.parts + ((uint64_t)(r + x) * 2u + (x == 0 ? 1u : 0u)) * a.e.width + u * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[x][j] = held ? part[j] : 0.0f;
+    }
+    float sum[V];
+    const float s = embed_scale(a.e, key);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      sum[j] = f[0][j];
+#pragma unroll
+      for (uint32_t x = 1; x < kEmbedShort; ++x) sum[j] += f[x][j];
+      sum[j] *= s;
+    }
+    EmbedUnit<T, V>::store(static_cast<T*>(a.e.out) + (uint64_t)key * a.e.width + u * V, sum);
   }
-  const uint32_t last = lo / a.run;
-#pragma unroll 8
-  for (uint32_t x = r + 1u; x <= last; ++x) {
-    const float* part = a.parts + (uint64_t)x * 2u * a.e.width + u * V;
+  const uint32_t groups = (units + 15u) / 16u, lane = threadIdx.x & 15u, share = threadIdx.x >> 4;
+  const uint64_t todo = (uint64_t)a.notes[0] * groups;
+  for (uint64_t i = gridDim.x - 1u - blockIdx.x; i < todo; i += gridDim.x) {
+    const uint32_t r = a.joins[i / groups], u = (uint32_t)(i % groups) * 16u + lane;
+    const uint32_t key = a.keys[(r + 1u) * a.run];
+    uint32_t parts = 1u;  // with the runs that begin with the row
+    for (uint32_t more = 256u; more == 256u; parts += more) {
+      const uint64_t at = (uint64_t)(r + parts + threadIdx.x) * a.run;
+      more = (uint32_t)__syncthreads_count(at < a.e.n && a.keys[at] == key);
+    }
+    const uint32_t each = (parts + 15u) / 16u, from = share * each, to = from + each < parts ? from + each : parts;
+    float sum[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] += part[j];
+    for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+    if (u < units) {
+#pragma unroll 4
+      for (uint32_t x = from; x < to; ++x) {
+        const float* part = a.parts + ((uint64_t)(r + x) * 2u + (x == 0 ? 1u : 0u)) * a.e.width + u * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += part[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds[share][lane][j] = sum[j];
+    __syncthreads();
+    if (share == 0 && u < units) {
+#pragma unroll
+      for (uint32_t y = 1; y < 16; ++y)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += lds[y][lane][j];
+      const float s = embed_scale(a.e, key);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] *= s;
+      EmbedUnit<T, V>::store(static_cast<T*>(a.e.out) + (uint64_t)key * a.e.width + u * V, sum);
+    }
+    __syncthreads();
   }
-  const float s = embed_scale(a.e, key);
-#pragma unroll
-  for (int j = 0; j < V; ++j) sum[j] *= s;
-  EmbedUnit<T, V>::store(static_cast<T*>(a.e.out) + (uint64_t)key * a.e.width + u * V, sum);
 }
 
 }  // namespace w8a8
