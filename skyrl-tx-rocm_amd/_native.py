@@ -423,7 +423,9 @@ def host():
                 module = _load_host()
                 for name, fn in (("forward", "forward_v1"), ("linear", "lora_linear_v1"), ("gateup", "rms_gateup_swiglu_v1"),
                                  ("residual", "lora_residual_v1"), ("workspace_bytes", "workspace_bytes"), ("forward_path", "forward_path"),
-                                 ("gq_linear", "gq_linear_v1"), ("gq_workspace_bytes", "gq_workspace_bytes")):
+                                 ("gq_linear", "gq_linear_v1"), ("gq_workspace_bytes", "gq_workspace_bytes"),
+                                 ("bf16_grouped", "bf16_grouped_v1"), ("bf16_grouped_bwd", "bf16_grouped_bwd_v1"), ("embedding", "embedding_v1"),
+                                 ("embedding_bwd", "embedding_bwd_v1"), ("embedding_bwd_workspace_bytes", "embedding_bwd_workspace_bytes")):
                     entry_address[name] = ctypes.cast(getattr(lib, f"mi355_w8a8_{fn}"), ctypes.c_void_p).value
                 _host = module
             except (ImportError, OSError) as e:

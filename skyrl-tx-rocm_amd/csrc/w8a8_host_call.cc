@@ -3,7 +3,7 @@
 // from one call for the next.  The steps take 14 to 16 us in Python beside the 7 us of the entry point's two launches, 4 to 6 here, and a decode
 // call's kernels 11 to 17: 2560 -> 6144, one row, 4 adapters of rank 64 23.3 -> 12.4 us a call; 12288 -> 4096, 16 rows, 4-bit codes 25.2 -> 18.1.
 //
-// Both functions return the output tensor, an int (the entry point's status, not OK), or None for anything out of the ordinary -- a wrong
+// Every function returns the output tensor (grouped_bwd: a tuple of two), an int (the entry point's status, not OK), or None for anything out of the ordinary -- a wrong
 // dtype, shape or device, a tensor subclass or mode, a tensor that is not contiguous, one that requires a gradient, a geometry that
 // the library refuses -- and the caller then goes the general way, which converts, differentiates or raises.
 #define PY_SSIZE_T_CLEAN
@@ -17,7 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include "../../include/mi355_w8a8.h"
+#include "bf16_api.h"
 
 namespace {
 
@@ -206,10 +206,195 @@ PyObject* group_scaled(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   END_HANDLE_TH_ERRORS
 }
 
+// A tensor that the bf16 operators take as it is: plain and, for the kernels' 16-byte loads, aligned.
+bool whole(const at::Tensor* t, at::ScalarType type, c10::Device device, int64_t dim) {
+  return t && plain(*t, type, device) && t->dim() == dim && (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15u) == 0;
+}
+// The device of an ordinary call on t: the current one.
+bool here(const at::Tensor* t) {
+  return t && t->is_cuda() && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+         c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice() == t->device();
+}
+bool grouped_dims(int64_t m, int64_t k, int64_t n, int64_t g) {
+  return m > 0 && m <= (1 << 20) && k > 0 && n > 0 && k % 8 == 0 && n % 8 == 0 && k <= MI355_W8A8_BF16_GROUPED_MAX_FEATURES &&
+         n <= MI355_W8A8_BF16_GROUPED_MAX_FEATURES && g > 0 && g <= 1024;
+}
+
+// grouped(x, weight, group_sizes, flags, entry, stream)
+PyObject* grouped(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  if (argc != 6) { PyErr_SetString(PyExc_TypeError, "grouped takes 6 arguments"); return nullptr; }
+  HANDLE_TH_ERRORS
+  Args arg{argv};
+  const at::Tensor *x = arg.tensor(0), *w = arg.tensor(1), *sizes = arg.tensor(2);
+  const int64_t flags = arg.integer(3);
+  const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_bf16_grouped_problem*, void*)>(arg.address(4));
+  void* const stream = arg.address(5);
+  if (!arg.ok || !entry || !here(x)) Py_RETURN_NONE;
+  const c10::Device device = x->device();
+  if (!whole(x, at::kBFloat16, device, 2) || !whole(w, at::kBFloat16, device, 3) || !sizes || !plain(*sizes, at::kInt, device) || sizes->dim() != 1) Py_RETURN_NONE;
+  const int64_t m = x->size(0), k = x->size(1), n = w->size(2), g = w->size(0);
+  if (w->size(1) != k || sizes->size(0) != g || !grouped_dims(m, k, n, g)) Py_RETURN_NONE;
+  at::Tensor out;
+  int status;
+  {
+    const WithoutGil released;
+    out = at::empty({m, n}, x->options().requires_grad(false));
+    mi355_w8a8_bf16_grouped_problem p{};
+    p.struct_size = sizeof(p);
+    p.flags = (uint32_t)flags;
+    p.m = (uint32_t)m; p.k = (uint32_t)k; p.n = (uint32_t)n; p.n_groups = (uint32_t)g;
+    p.x = x->const_data_ptr(); p.weight = w->const_data_ptr(); p.group_sizes = sizes->const_data_ptr<int32_t>();
+    p.out = out.mutable_data_ptr();
+    status = entry(&p, stream);
+  }
+  return finish(std::move(out), status);
+  END_HANDLE_TH_ERRORS
+}
+
+// grouped_bwd(x, dy, weight, group_sizes, need_dx, need_dw, f32, flags, entry, stream)
+PyObject* grouped_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  if (argc != 10) { PyErr_SetString(PyExc_TypeError, "grouped_bwd takes 10 arguments"); return nullptr; }
+  HANDLE_TH_ERRORS
+  Args arg{argv};
+  const at::Tensor *x = arg.tensor(0), *dy = arg.tensor(1), *w = arg.tensor(2), *sizes = arg.tensor(3);
+  const bool need_dx = argv[4] == Py_True, need_dw = argv[5] == Py_True, f32 = argv[6] == Py_True;
+  const int64_t flags = arg.integer(7);
+  const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_bf16_grouped_bwd_problem*, void*)>(arg.address(8));
+  void* const stream = arg.address(9);
+  if (!arg.ok || !entry || !here(dy) || !x || !w) Py_RETURN_NONE;
+  const c10::Device device = dy->device();
+  if (!whole(dy, at::kBFloat16, device, 2) || !whole(x, at::kBFloat16, device, 2) || !whole(w, at::kBFloat16, device, 3) || !sizes ||
+      !plain(*sizes, at::kInt, device) || sizes->dim() != 1)
+    Py_RETURN_NONE;
+  const int64_t m = dy->size(0), k = w->size(1), n = w->size(2), g = w->size(0);
+  if (dy->size(1) != n || x->size(0) != m || x->size(1) != k || sizes->size(0) != g || !grouped_dims(m, k, n, g)) Py_RETURN_NONE;
+  at::Tensor dx, dw;
+  int status;
+  {
+    const WithoutGil released;
+    if (need_dx) dx = at::empty({m, k}, dy->options().requires_grad(false));
+    if (need_dw) dw = at::empty({g, k, n}, dy->options().requires_grad(false).dtype(f32 ? at::kFloat : at::kBFloat16));
+    mi355_w8a8_bf16_grouped_bwd_problem p{};
+    p.struct_size = sizeof(p);
+    p.flags = (uint32_t)flags | (f32 ? MI355_W8A8_FLAG_BF16_GROUPED_DW_F32 : 0u);
+    p.m = (uint32_t)m; p.k = (uint32_t)k; p.n = (uint32_t)n; p.n_groups = (uint32_t)g;
+    p.x = x->const_data_ptr(); p.dy = dy->const_data_ptr(); p.weight = w->const_data_ptr(); p.group_sizes = sizes->const_data_ptr<int32_t>();
+    p.dx = need_dx ? dx.mutable_data_ptr() : nullptr;
+    p.dw = need_dw ? dw.mutable_data_ptr() : nullptr;
+    status = entry(&p, stream);
+  }
+  if (status) return PyLong_FromLong(status);
+  PyObject* const a = need_dx ? THPVariable_Wrap(std::move(dx)) : (Py_INCREF(Py_None), Py_None);
+  PyObject* const b = need_dw ? THPVariable_Wrap(std::move(dw)) : (Py_INCREF(Py_None), Py_None);
+  return a && b ? Py_BuildValue("(NN)", a, b) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// The index side of an embedding call; false where it is not an ordinary one.  shape: the table's.
+bool embedding_call(const at::Tensor* ids, const at::Tensor* adapters, PyObject* scale, at::IntArrayRef shape, at::ScalarType type, c10::Device device,
+                    mi355_w8a8_embedding_problem& p) {
+  const int64_t dim = (int64_t)shape.size();
+  if ((dim != 2 && dim != 3) || (type != at::kBFloat16 && type != at::kFloat) || !ids) return false;
+  const bool wide = ids->scalar_type() == at::kLong;
+  if (!plain(*ids, wide ? at::kLong : at::kInt, device)) return false;
+  const int64_t n = ids->numel(), vocab = shape[dim - 2], width = shape[dim - 1], adapted = dim == 3 ? shape[0] : 0, rows = adapted ? adapted : 1;
+  if (n <= 0 || n > (1 << 20) || vocab <= 0 || width <= 0 || width > (int64_t)MI355_W8A8_EMBEDDING_MAX_WIDTH || vocab > (int64_t)MI355_W8A8_EMBEDDING_MAX_ROWS ||
+      rows > (int64_t)MI355_W8A8_EMBEDDING_MAX_ROWS / vocab || (dim == 3 && adapted <= 0))
+    return false;
+  if (adapters ? dim != 3 || !plain(*adapters, at::kInt, device) || adapters->numel() != n : adapted > 1) return false;
+  p.scale = 1.0f;
+  if (PyFloat_Check(scale)) {
+    p.scale = (float)PyFloat_AS_DOUBLE(scale);
+    if (!(p.scale - p.scale == 0.0f)) return false;
+  } else if (THPVariable_CheckExact(scale)) {
+    const at::Tensor& t = THPVariable_Unpack(scale);
+    if (dim != 3 || !plain(t, at::kFloat, device) || t.dim() != 1 || t.size(0) != adapted) return false;
+    p.scales = t.const_data_ptr<float>();
+  } else if (scale != Py_None) {
+    return false;
+  }
+  p.struct_size = sizeof(p);
+  p.flags = (type == at::kFloat ? MI355_W8A8_FLAG_EMBEDDING_F32 : 0u) | (wide ? MI355_W8A8_FLAG_EMBEDDING_IDS64 : 0u);
+  p.n_tokens = (uint32_t)n; p.vocab = (uint32_t)vocab; p.width = (uint32_t)width; p.n_adapters = (uint32_t)adapted;
+  p.ids = ids->const_data_ptr();
+  p.adapter_indices = adapters ? adapters->const_data_ptr<int32_t>() : nullptr;
+  return true;
+}
+
+// embedding(table, ids, scale, adapter_indices, entry, stream)
+PyObject* embedding(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  if (argc != 6) { PyErr_SetString(PyExc_TypeError, "embedding takes 6 arguments"); return nullptr; }
+  HANDLE_TH_ERRORS
+  Args arg{argv};
+  const at::Tensor *table = arg.tensor(0), *ids = arg.tensor(1), *adapters = arg.tensor(3);
+  const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_embedding_problem*, void*)>(arg.address(4));
+  void* const stream = arg.address(5);
+  if (!arg.ok || !entry || !here(table) || !plain(*table, table->scalar_type(), table->device())) Py_RETURN_NONE;
+  mi355_w8a8_embedding_problem p{};
+  if (!embedding_call(ids, adapters, argv[2], table->sizes(), table->scalar_type(), table->device(), p)) Py_RETURN_NONE;
+  at::DimVector shape(ids->sizes().begin(), ids->sizes().end());
+  shape.push_back(p.width);
+  at::Tensor out;
+  int status;
+  {
+    const WithoutGil released;
+    out = at::empty(shape, table->options().requires_grad(false));
+    p.table = table->const_data_ptr();
+    p.out = out.mutable_data_ptr();
+    status = entry(&p, stream);
+  }
+  return finish(std::move(out), status);
+  END_HANDLE_TH_ERRORS
+}
+
+// embedding_bwd(d_out, ids, table_shape, scale, adapter_indices, entry, workspace_bytes, stream)
+PyObject* embedding_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  if (argc != 8) { PyErr_SetString(PyExc_TypeError, "embedding_bwd takes 8 arguments"); return nullptr; }
+  HANDLE_TH_ERRORS
+  Args arg{argv};
+  const at::Tensor *d = arg.tensor(0), *ids = arg.tensor(1), *adapters = arg.tensor(4);
+  const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_embedding_problem*, void*)>(arg.address(5));
+  const auto bytes_of = reinterpret_cast<uint64_t (*)(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t)>(arg.address(6));
+  void* const stream = arg.address(7);
+  if (!arg.ok || !entry || !bytes_of || !here(d) || !ids || !plain(*d, d->scalar_type(), d->device()) || !PyTuple_CheckExact(argv[2])) Py_RETURN_NONE;
+  at::DimVector table;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(argv[2]); ++i) {
+    PyObject* const v = PyTuple_GET_ITEM(argv[2], i);
+    if (!PyLong_CheckExact(v)) Py_RETURN_NONE;
+    table.push_back(PyLong_AsLongLong(v));
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+  }
+  mi355_w8a8_embedding_problem p{};
+  if (!embedding_call(ids, adapters, argv[3], table, d->scalar_type(), d->device(), p)) Py_RETURN_NONE;
+  at::DimVector shape(ids->sizes().begin(), ids->sizes().end());
+  shape.push_back(p.width);
+  if (d->sizes() != at::IntArrayRef(shape)) Py_RETURN_NONE;
+  const uint64_t bytes = bytes_of(p.n_tokens, p.vocab, p.width, p.n_adapters, p.flags);
+  if (bytes == 0) Py_RETURN_NONE;
+  at::Tensor out;
+  int status;
+  {
+    const WithoutGil released;
+    out = at::empty(table, d->options().requires_grad(false));
+    const at::Tensor ws = at::empty({(int64_t)bytes}, d->options().requires_grad(false).dtype(at::kByte));
+    p.d_out = d->const_data_ptr();
+    p.out = out.mutable_data_ptr();
+    p.workspace = ws.mutable_data_ptr();
+    p.workspace_bytes = bytes;
+    status = entry(&p, stream);
+  }
+  return finish(std::move(out), status);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"dense", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense)), METH_FASTCALL, "One forward call of the per-channel linear."},
     {"group_scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_scaled)), METH_FASTCALL,
      "One forward call of the group-scaled linear."},
+    {"grouped", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grouped)), METH_FASTCALL, "One call of the bf16 products grouped by expert."},
+    {"grouped_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grouped_bwd)), METH_FASTCALL, "Their two gradients."},
+    {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding)), METH_FASTCALL, "One lookup of embedding rows."},
+    {"embedding_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding_bwd)), METH_FASTCALL, "The table's gradient."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mi355_w8a8_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -65,6 +65,14 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Ten
     """``out[rows of g] = bf16(x[rows of g] @ weight[g])`` with float32 sums: x bf16 [rows, K], weight bf16
     [groups, K, N], group_sizes integers [groups].  Rows behind the last group are zero.  ``flags`` may force the tiles
     (``_native.FLAG_BF16_GROUPED_TILE_*``); by default they follow the sizes."""
+    host = _native.host() if isinstance(x, torch.Tensor) and x.is_cuda else None
+    if host is not None:
+        # an ordinary call goes through the host module; for any other it returns None
+        result = host.grouped(x, weight, group_sizes, flags, _native.entry_address["bf16_grouped"], _stream_ptr(x.device))
+        if type(result) is int:
+            _native.check("mi355_w8a8_bf16_grouped_v1", result)
+        if result is not None:
+            return result
     xc, w = _bf16(x, "x"), _bf16(weight, "weight")
     _same_device(x, weight)
     m, k, n, g, sizes = _geometry(x, "x", 1, weight.shape, group_sizes)
@@ -88,6 +96,14 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
         raise ValueError("dw needs x and dx needs weight")
     if dw_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"dw_dtype must be BF16 or FP32, got {dw_dtype}")
+    host = _native.host() if isinstance(dy, torch.Tensor) and dy.is_cuda else None
+    if host is not None:
+        result = host.grouped_bwd(x, dy, weight, group_sizes, need_dx, need_dw, dw_dtype == torch.float32, flags,
+                                  _native.entry_address["bf16_grouped_bwd"], _stream_ptr(dy.device))
+        if type(result) is int:
+            _native.check("mi355_w8a8_bf16_grouped_bwd_v1", result)
+        if result is not None:
+            return result
     d = _bf16(dy, "dy")
     xc = _bf16(x, "x") if need_dw else None
     w = _bf16(weight, "weight") if need_dx else None

@@ -82,6 +82,14 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale=None, *, adapter_indice
     in float32 and one rounding to the table's type.  ``ids`` int32 or int64 of any shape; ``scale`` a number, or for adapters
     float32 [adapters]; ``adapter_indices`` one entry per id, or per example (a divisor of the ids).  Ids and
     adapters out of range read zeros."""
+    host = _native.host() if isinstance(table, torch.Tensor) and table.is_cuda else None
+    if host is not None:
+        # an ordinary call goes through the host module; for any other it returns None
+        result = host.embedding(table, ids, scale, adapter_indices, _native.entry_address["embedding"], _stream_ptr(table.device))
+        if type(result) is int:
+            _native.check("mi355_w8a8_embedding_v1", result)
+        if result is not None:
+            return result
     _require_cuda(table, "table")
     p, keep = _problem(ids, tuple(table.shape), scale, adapter_indices, table.dtype, table.device)
     t = table.detach().contiguous()
@@ -98,8 +106,16 @@ def lookup_backward(d_out: torch.Tensor, ids: torch.Tensor, table_shape, scale=N
                     adapter_indices: torch.Tensor | None = None) -> torch.Tensor:
     """The table's gradient: ``scale * sum(d_out[t] for ids[t] == v)`` for every row v, in ``d_out``'s type (bf16 or
     float32) from float32 sums in the order of the ids, so that equal inputs give equal bits; zeros for rows that no id names."""
-    _require_cuda(d_out, "d_out")
     shape = tuple(int(s) for s in table_shape)
+    host = _native.host() if isinstance(d_out, torch.Tensor) and d_out.is_cuda else None
+    if host is not None:
+        result = host.embedding_bwd(d_out, ids, shape, scale, adapter_indices, _native.entry_address["embedding_bwd"],
+                                    _native.entry_address["embedding_bwd_workspace_bytes"], _stream_ptr(d_out.device))
+        if type(result) is int:
+            _native.check("mi355_w8a8_embedding_bwd_v1", result)
+        if result is not None:
+            return result
+    _require_cuda(d_out, "d_out")
     p, keep = _problem(ids, shape, scale, adapter_indices, d_out.dtype, d_out.device)
     if tuple(d_out.shape) != (*ids.shape, p.width):
         raise ValueError(f"d_out must have shape {(*ids.shape, p.width)}, got {tuple(d_out.shape)}")
