@@ -327,12 +327,17 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
 
 // ---- gradient norms and clipping -------------------------------------------------------------------------------------
 
-// values of a piece: 64 KiB of bf16, more where an adapter's parts would be more than 2048 (every workgroup of the scaling reads them all)
-uint32_t grad_piece_values(const mi355_w8a8_grad_tensor* t, uint32_t n) {
+// values of a piece: as few as leave the chip 2048 workgroups, at most 64 KiB, so that the last of them end soon after the first; more where an
+// adapter's parts would be more than 4096 (every workgroup of the scaling reads them all)
+uint32_t grad_piece_values(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters) {
   uint64_t values = 0;
-  for (uint32_t i = 0; i < n; ++i) values += t[i].count;
-  uint32_t piece = 32768u;
-  while (values / piece > 2048u && piece < (1u << 28)) piece *= 2u;
+  uint32_t most = 32768u, piece = 2048u;
+  for (uint32_t i = 0; i < n; ++i) {
+    values += t[i].count;
+    if (t[i].type == MI355_W8A8_GRAD_F32) most = 16384u;
+  }
+  while (piece < most && values / piece * adapters > 2048u) piece *= 2u;
+  while (values / piece > 4096u && piece < (1u << 28)) piece *= 2u;
   return piece;
 }
 inline uint64_t pieces_of(uint64_t count, uint32_t piece) { return (count + piece - 1u) / piece; }
@@ -356,9 +361,50 @@ int check_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, 
   return MI355_W8A8_OK;
 }
 
+template <uint32_t TABLE>
+int launch_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const float* limits, float* norms, void* workspace, hipStream_t s) {
+  GradArgs<TABLE> a{};
+  a.parts = static_cast<double*>(workspace);
+  a.limits = limits;
+  a.norms = norms;
+  a.piece = grad_piece_values(t, n, adapters);
+  uint64_t total = 0;
+  for (uint32_t i = 0; i < n; ++i) total += pieces_of(t[i].count, a.piece);
+  a.parts_ld = a.parts_used = (uint32_t)total;
+  // The table's share of a launch each, first to last for the norm, last to first for the scaling.
+  auto fill = [&](uint32_t from) {  // -> the first tensor behind the launch
+    a.tensors = a.pieces = 0;
+    uint32_t i = from;
+    for (; i < n && a.tensors < TABLE; ++i) {
+      if (t[i].count == 0) continue;
+      a.tensor[a.tensors++] = GradTensor{t[i].grad, t[i].out, t[i].count, a.pieces, t[i].type == MI355_W8A8_GRAD_F32};
+      a.pieces += (uint32_t)pieces_of(t[i].count, a.piece);
+    }
+    return i;
+  };
+  uint32_t first[MI355_W8A8_GRAD_MAX_TENSORS / TABLE + 1], parts[MI355_W8A8_GRAD_MAX_TENSORS / TABLE + 1], launches = 0;
+  int st;
+  for (uint32_t i = 0, part = 0; i < n; part += a.pieces) {
+    first[launches] = i;
+    parts[launches] = a.part0 = part;
+    i = fill(i);
+    if (a.pieces == 0) break;  // (none of the last tensors holds a value)
+    ++launches;
+    hipLaunchKernelGGL(grad_norm_kernel<TABLE>, dim3(a.pieces, adapters), dim3(256), 0, s, a);
+    if ((st = launch_status())) return st;
+  }
+  for (uint32_t l = limits ? launches : 1u; l-- > 0;) {
+    if (launches > 1u || a.pieces == 0) fill(first[l]);
+    a.part0 = parts[l];
+    hipLaunchKernelGGL(grad_scale_kernel<TABLE>, dim3(limits ? a.pieces : 1u, adapters), dim3(256), 0, s, a);
+    if ((st = launch_status())) return st;
+  }
+  return MI355_W8A8_OK;
+}
+
 int run_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const float* limits, float* norms, void* workspace, uint64_t workspace_bytes,
               hipStream_t s, bool scale) {
-  int st = check_grads(t, n, adapters, norms, scale);
+  const int st = check_grads(t, n, adapters, norms, scale);
   if (st) return st;
   if (scale && !limits) return MI355_W8A8_ERR_NULL;
   if (!aligned(limits, 4)) return MI355_W8A8_ERR_ALIGN;
@@ -369,44 +415,21 @@ int run_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, co
   if (overlaps(workspace, need, norms, adapters * 4ull) || overlaps(workspace, need, limits, adapters * 4ull) ||
       overlaps(norms, adapters * 4ull, limits, limits ? adapters * 4ull : 0ull))
     return MI355_W8A8_ERR_ALIAS;
+  bool any = false;
   for (uint32_t i = 0; i < n; ++i) {
+    any |= t[i].count != 0;
     const uint64_t bytes = t[i].count * adapters * (t[i].type == MI355_W8A8_GRAD_F32 ? 4u : 2u);
     if (overlaps(workspace, need, t[i].grad, bytes) ||
         (scale && (overlaps(workspace, need, t[i].out, bytes) || overlaps(limits, adapters * 4ull, t[i].out, bytes))))
       return MI355_W8A8_ERR_ALIAS;
   }
-  GradArgs a{};
-  a.parts = static_cast<double*>(workspace);
-  a.limits = scale ? limits : nullptr;
-  a.norms = norms;
-  a.piece = grad_piece_values(t, n);
-  uint64_t total = 0;
-  for (uint32_t i = 0; i < n; ++i) total += pieces_of(t[i].count, a.piece);
-  a.parts_ld = a.parts_used = (uint32_t)total;
   (void)hipGetLastError();
-  if (total == 0) {  // no values: the norms are zero
-    a.pieces = 0;
+  if (!any) {  // no values: the norms are zero
     hipLaunchKernelGGL(grad_zero_norms_kernel, dim3((adapters + 255u) / 256u), dim3(256), 0, s, norms, adapters);
     return launch_status();
   }
-  for (int phase = 0; phase < 2; ++phase) {
-    uint32_t i = 0, part = 0;
-    while (i < n) {
-      a.tensors = a.pieces = 0;
-      a.part0 = part;
-      for (; i < n && a.tensors < kGradTable; ++i) {
-        if (t[i].count == 0) continue;
-        a.tensor[a.tensors++] = GradTensor{t[i].grad, t[i].out, t[i].count, a.pieces, t[i].type == MI355_W8A8_GRAD_F32};
-        a.pieces += (uint32_t)pieces_of(t[i].count, a.piece);
-      }
-      if (a.pieces == 0) break;
-      part += a.pieces;
-      if (phase == 0) hipLaunchKernelGGL(grad_norm_kernel, dim3(a.pieces, adapters), dim3(256), 0, s, a);
-      else if (scale || a.part0 == 0) hipLaunchKernelGGL(grad_scale_kernel, dim3(scale ? a.pieces : 1u, adapters), dim3(256), 0, s, a);
-      if ((st = launch_status())) return st;
-    }
-  }
-  return MI355_W8A8_OK;
+  if (n <= kGradShortTable) return launch_grads<kGradShortTable>(t, n, adapters, scale ? limits : nullptr, norms, workspace, s);
+  return launch_grads<kGradTable>(t, n, adapters, scale ? limits : nullptr, norms, workspace, s);
 }
 
 }  // namespace
@@ -435,7 +458,7 @@ uint64_t mi355_w8a8_grad_workspace_bytes(const mi355_w8a8_grad_tensor* tensors, 
   if (!tensors || n_tensors == 0 || n_tensors > MI355_W8A8_GRAD_MAX_TENSORS || n_adapters == 0 || n_adapters > 65535u) return 0;
   for (uint32_t i = 0; i < n_tensors; ++i)
     if (tensors[i].count > (1ull << 40) / n_adapters) return 0;
-  const uint32_t piece = grad_piece_values(tensors, n_tensors);
+  const uint32_t piece = grad_piece_values(tensors, n_tensors, n_adapters);
   uint64_t pieces = 0;
   for (uint32_t i = 0; i < n_tensors; ++i) pieces += pieces_of(tensors[i].count, piece);
   return pieces > 0x7fffffffu ? 0u : align256((pieces ? pieces : 1u) * n_adapters * 8u);

@@ -18,7 +18,7 @@
 
 namespace w8a8 {
 
-constexpr uint32_t kGradTable = 120;
+constexpr uint32_t kGradTable = 120, kGradShortTable = 16;  // (a call of few tensors does not hand over 4 KiB: eight tensors of 6.8 MB: 12.4 / 10.0 us)
 
 struct GradTensor {
   const void* grad;
@@ -27,8 +27,9 @@ struct GradTensor {
   uint32_t first_piece;   // among the launch's pieces of one adapter
   uint32_t f32;
 };
+template <uint32_t TABLE>
 struct GradArgs {
-  GradTensor tensor[kGradTable];
+  GradTensor tensor[TABLE];
   double* parts;          // [adapters][parts_ld]
   const float* limits;    // [adapters]
   float* norms;           // [adapters]
@@ -37,9 +38,16 @@ struct GradArgs {
   uint32_t piece;         // values of a piece
 };
 
+typedef uint32_t v4whole __attribute__((ext_vector_type(4)));
+typedef uint32_t v4unaligned __attribute__((ext_vector_type(4), aligned(2)));  // (out may lie at another offset from 16 than grad)
+// (pointers out of a table are to any memory for the compiler: its flat accesses look at the LDS too)
+template <typename T>
+__device__ inline __attribute__((address_space(1))) T* in_memory(T* p) { return (__attribute__((address_space(1))) T*)p; }
+
 struct GradPiece { const GradTensor* t; uint64_t at; uint32_t count; };  // at: first value, in the whole tensor
 
-__device__ inline GradPiece grad_piece(const GradArgs& a, uint32_t adapter, uint32_t piece) {
+template <uint32_t TABLE>
+__device__ inline GradPiece grad_piece(const GradArgs<TABLE>& a, uint32_t adapter, uint32_t piece) {
   uint32_t lo = 0, hi = a.tensors;  // the last tensor whose first piece is not behind this one
   while (hi - lo > 1u) {
     const uint32_t mid = (lo + hi) / 2u;
@@ -86,21 +94,21 @@ template <> struct GradUnit<float> {
 template <typename T>
 __device__ inline double grad_squares(const GradPiece& p) {
   constexpr uint32_t N = GradUnit<T>::kN;
-  const T* g = static_cast<const T*>(p.t->grad) + p.at;
+  const auto* g = in_memory(static_cast<const T*>(p.t->grad) + p.at);
   const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T);
   const uint32_t head = off ? (N - off < p.count ? N - off : p.count) : 0u, units = (p.count - head) / N;
   double sum = 0.0;
-  auto add = [&](float v) { sum += (double)v * (double)v; };
+  auto add = [&](float v) { sum = __builtin_fma((double)v, (double)v, sum); };
   if (threadIdx.x < head) add(GradUnit<T>::one(g[threadIdx.x]));
-  const uint4* u = reinterpret_cast<const uint4*>(g + head);
+  const auto* u = reinterpret_cast<const __attribute__((address_space(1))) v4whole*>(g + head);
   for (uint32_t i = threadIdx.x; i < units; i += 1024u) {
-    uint4 r[4];
+    v4whole r[4];
 #pragma unroll
-    for (uint32_t x = 0; x < 4; ++x) r[x] = i + x * 256u < units ? u[i + x * 256u] : make_uint4(0u, 0u, 0u, 0u);
+    for (uint32_t x = 0; x < 4; ++x) r[x] = i + x * 256u < units ? u[i + x * 256u] : v4whole{0u, 0u, 0u, 0u};
 #pragma unroll
     for (uint32_t x = 0; x < 4; ++x) {
       float f[N];
-      GradUnit<T>::open(r[x], f);
+      GradUnit<T>::open(make_uint4(r[x][0], r[x][1], r[x][2], r[x][3]), f);
 #pragma unroll
       for (uint32_t j = 0; j < N; ++j) add(f[j]);
     }
@@ -120,7 +128,8 @@ __device__ inline double grad_block_sum(double v) {
   return s;
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
+template <uint32_t TABLE>
+__global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs<TABLE> a) {
   const uint32_t adapter = blockIdx.y, piece = blockIdx.x;
   const GradPiece p = grad_piece(a, adapter, piece);
   const double s = grad_block_sum(p.t->f32 ? grad_squares<float>(p) : grad_squares<uint16_t>(p));
@@ -130,34 +139,37 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs a) {
 template <typename T>
 __device__ inline void grad_scale(const GradPiece& p, float factor) {
   constexpr uint32_t N = GradUnit<T>::kN;
-  const T* g = static_cast<const T*>(p.t->grad) + p.at;
-  T* o = static_cast<T*>(p.t->out) + p.at;
-  if (factor == 1.0f && g == o) return;
+  if (factor == 1.0f && p.t->grad == p.t->out) return;
+  const auto* g = in_memory(static_cast<const T*>(p.t->grad) + p.at);
+  auto* o = in_memory(static_cast<T*>(p.t->out) + p.at);
   const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T);
   const uint32_t head = off ? (N - off < p.count ? N - off : p.count) : 0u, units = (p.count - head) / N;
   if (threadIdx.x < head) o[threadIdx.x] = GradUnit<T>::back(GradUnit<T>::one(g[threadIdx.x]) * factor);
-  const uint4* u = reinterpret_cast<const uint4*>(g + head);
-  unsigned char* w = reinterpret_cast<unsigned char*>(o + head);
+  const auto* u = reinterpret_cast<const __attribute__((address_space(1))) v4whole*>(g + head);
+  auto* w = reinterpret_cast<__attribute__((address_space(1))) v4unaligned*>(o + head);
   for (uint32_t i = threadIdx.x; i < units; i += 1024u) {
-    uint4 r[4];
+    v4whole r[4];
 #pragma unroll
-    for (uint32_t x = 0; x < 4; ++x) r[x] = i + x * 256u < units ? u[i + x * 256u] : make_uint4(0u, 0u, 0u, 0u);
+    for (uint32_t x = 0; x < 4; ++x) r[x] = i + x * 256u < units ? u[i + x * 256u] : v4whole{0u, 0u, 0u, 0u};
 #pragma unroll
     for (uint32_t x = 0; x < 4; ++x) {
       float f[N];
-      GradUnit<T>::open(r[x], f);
+      GradUnit<T>::open(make_uint4(r[x][0], r[x][1], r[x][2], r[x][3]), f);
 #pragma unroll
       for (uint32_t j = 0; j < N; ++j) f[j] *= factor;
       const uint4 v = GradUnit<T>::close(f);
-      if (i + x * 256u < units) __builtin_memcpy(w + (uint64_t)(i + x * 256u) * 16u, &v, 16);  // (out may lie at another offset from 16)
+      // past the caches, which the next norm's reads would have to wait for: 32 tensors of 838 MB in all 234 us, 211 so
+      if (i + x * 256u < units) __builtin_nontemporal_store(v4unaligned{v.x, v.y, v.z, v.w}, w + i + x * 256u);
     }
   }
   const uint32_t done = head + units * N;
   if (threadIdx.x < p.count - done) o[done + threadIdx.x] = GradUnit<T>::back(GradUnit<T>::one(g[done + threadIdx.x]) * factor);
 }
 
-__global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs a) {
-  const uint32_t adapter = blockIdx.y, piece = blockIdx.x;
+template <uint32_t TABLE>
+__global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs<TABLE> a) {
+  // from the last piece to the first: what the norm read last is in the caches yet
+  const uint32_t adapter = gridDim.y - 1u - blockIdx.y, piece = gridDim.x - 1u - blockIdx.x;
   double s = 0.0;
   for (uint32_t i = threadIdx.x; i < a.parts_used; i += 256u) s += a.parts[(uint64_t)adapter * a.parts_ld + i];
   const double norm = sqrt(grad_block_sum(s));
