@@ -13,8 +13,10 @@ or eager fallback.
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ... import _native
 from .w8a8_lora import _on, _require_cuda, _stream_ptr
@@ -124,15 +126,50 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
     return dx, dw
 
 
+class _LeafUse:
+    """One use of a leaf in an autograd graph; lives as long as the graph."""
+
+    __slots__ = ("leaf", "stream", "__weakref__")
+
+    def __init__(self, leaf, stream):
+        self.leaf, self.stream = weakref.ref(leaf), stream
+
+
+_leaf_uses: weakref.WeakSet = weakref.WeakSet()
+
+
+def note_leaves(*tensors: torch.Tensor) -> list:
+    """Uses of those ``tensors`` that are leaves, for the graph to keep and ``check_capture`` to look at."""
+    uses = [_LeafUse(t, _stream_ptr(t.device)) for t in tensors if t.requires_grad and t.is_leaf]
+    _leaf_uses.update(uses)
+    return uses
+
+
+def check_capture(uses: list) -> None:
+    """Refuse a backward pass under stream capture while another graph of the same leaves, made on another stream, lives.  Autograd
+    adds to a leaf's gradient on the stream of the leaf's first use among the living graphs: that stream would be drawn into the
+    capture, which ends the process when it is the default one."""
+    if not uses or not torch.cuda.is_current_stream_capturing():
+        return
+    for other in list(_leaf_uses):
+        leaf = other.leaf()
+        if leaf is not None and any(use.leaf() is leaf and use.stream != other.stream for use in uses):
+            raise RuntimeError("a backward pass is captured while a graph of the same parameters, made on another stream, lives: "
+                               "let go of its outputs (the last loss, say) first, or run it on the capture's stream")
+
+
 class _GroupedMatmulFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group_sizes):
+        ctx.uses = note_leaves(x, weight)
         ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None, group_sizes)
         ctx.shape = tuple(weight.shape)
         return grouped_matmul(x, weight, group_sizes)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
+        check_capture(ctx.uses)
         x, weight, group_sizes = ctx.saved_tensors
         dx, dw = grouped_matmul_backward(x, dy, weight, group_sizes, need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
         return dx, dw, None

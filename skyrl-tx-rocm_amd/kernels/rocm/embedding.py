@@ -11,8 +11,10 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ... import _native
+from .bf16_grouped_linear import check_capture, note_leaves
 from .w8a8_lora import _on, _require_cuda, _stream_ptr
 
 MAX_TOKENS = 1 << 20
@@ -135,12 +137,15 @@ def lookup_backward(d_out: torch.Tensor, ids: torch.Tensor, table_shape, scale=N
 class _LookupFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, adapter_indices):
+        ctx.uses = note_leaves(table)
         ctx.save_for_backward(ids, adapter_indices, scale if isinstance(scale, torch.Tensor) else None)
         ctx.shape, ctx.scale = tuple(table.shape), None if isinstance(scale, torch.Tensor) else scale
         return lookup(table, ids, scale, adapter_indices=adapter_indices)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out):
+        check_capture(ctx.uses)
         ids, adapter_indices, scales = ctx.saved_tensors
         grad = lookup_backward(d_out, ids, ctx.shape, ctx.scale if scales is None else scales, adapter_indices=adapter_indices)
         return grad, None, None, None

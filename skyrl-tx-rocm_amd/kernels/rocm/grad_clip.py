@@ -25,8 +25,9 @@ class GradClipPlan:
     current stream that neither allocates nor synchronizes, so it can be captured in a HIP graph.
 
     ``grads`` are contiguous bf16 or float32 tensors, read at every run where they lie: a loop whose backward writes the same
-    buffers each step (``BackwardPlan``) builds the plan once.  ``max_norm`` is a number or a float32 tensor (one value, or
-    [adapters] with ``per_adapter``), read at every run; None: only norms.  ``out`` names the tensors that the scaled gradients go
+    buffers each step (``BackwardPlan``) builds the plan once.  ``max_norm`` is a number or a tensor (one value, or [adapters]
+    with ``per_adapter``); None: only norms.  A contiguous float32 [adapters] tensor on the gradients' device is read at every
+    run where it lies, any other form is copied when the plan is made.  ``out`` names the tensors that the scaled gradients go
     to, of the same shapes and types; the gradients themselves scale in place."""
 
     def __init__(self, grads, max_norm=None, *, per_adapter: bool = False, out=None):
@@ -70,6 +71,8 @@ class GradClipPlan:
                 raise ValueError(f"max_norm must be a number or have shape ({adapters},), got {tuple(limits.shape)}")
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), t.data_ptr()) for t in {id(t): t for t in (*grads, *(outs or ()))}.values()
                        if t.numel()) if outs is not None else []
+        if outs is not None and len({o.data_ptr() for o in outs if o.numel()}) != sum(1 for o in outs if o.numel()):
+            raise ValueError("two outputs lie at the same place (a gradient given twice cannot be scaled in place)")
         pairs = {(g.data_ptr(), o.data_ptr()) for g, o in zip(grads, outs)} if outs is not None else set()
         for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
             if start < end and not (a == b and (a, b) in pairs):

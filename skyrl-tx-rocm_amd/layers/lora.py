@@ -1,10 +1,12 @@
-"""LoRA layer modules of the reference on W8A8 frozen weights.
+"""LoRA layer modules of the reference on W8A8 frozen weights, and those that keep their weights in bf16.
 
 Mirrors the call surface of ``skyrl/tx/layers/lora.py``: ``LoRALinear.__call__(x,
 adapter_indices=None)`` (:226-268), ``FusedLoRALinear.__call__ -> tuple`` with
 ``fuse``/``split`` (:271-351), ``LoRAExpert.__call__(x, group_sizes,
 adapter_indices_sorted=None, *, group_offset=None)`` (:354-444) and
-``init_lora_adapter`` (:447-501).  The frozen kernel is a ``GroupQuantizedWeight`` with one
+``init_lora_adapter`` (:447-501).  ``LoRAEmbed`` and a ``LoRAExpert`` with ``load_dense`` hold bf16 weights and run on
+the ragged bf16 products and the embedding lookup; ``clip_adapter_gradients`` closes a training step over the
+adapters of any of them.  The frozen kernel is a ``GroupQuantizedWeight`` with one
 group over K (int8 codes, one float32 scale per output channel) instead of a dense matrix;
 the forward runs on the HIP kernels.  Parameters are plain torch tensors on the GPU: the
 reference's flax/NNX containers, sharding annotations and RNG plumbing are not part of the path.
@@ -17,7 +19,10 @@ import math
 import torch
 
 from ..kernels import quantized_lora as ql
+from ..kernels.rocm import embedding as emb
+from ..kernels.rocm import grad_clip
 from ..kernels.rocm import w8a8_lora as w8
+from ..kernels.rocm.bf16_grouped_linear import bf16_grouped_linear
 
 
 class LoRAMixin:
@@ -164,6 +169,65 @@ class FusedLoRALinear(LoRALinear):
         return tuple(out)
 
 
+def _whole_units(t: torch.Tensor, dim: int) -> torch.Tensor:
+    """``t`` with zeros behind ``dim`` up to a multiple of 8, which is what the ragged bf16 products take."""
+    spare = -t.shape[dim] % 8
+    if not spare:
+        return t
+    shape = list(t.shape)
+    shape[dim] = spare
+    return torch.cat([t, t.new_zeros(shape)], dim)
+
+
+class LoRAEmbed(LoRAMixin):
+    """Embedding table with multi-adapter LoRA: ``table[id] + s[a] * A[a, id] @ B[a]``.
+
+    ``adapter_indices`` holds one adapter per example (leading dimension of ``ids``).  The A rows are looked up in adapter
+    order, scaled and rounded to bf16, multiplied by their adapter's B in one ragged product, put back and added to the table's
+    rows.  Differentiable in the table and the adapters: A's gradient is a sum by sorted tokens.  Ids and adapters out of range
+    read zeros (an adapter out of range: the table's row alone).
+    """
+
+    def __init__(self, num_embeddings: int, features: int, *, embedding: torch.Tensor | None = None, max_lora_adapters: int = 0,
+                 max_lora_rank: int = 8, device="cuda:0", **_unused_reference_keywords):
+        self.num_embeddings, self.features = int(num_embeddings), int(features)
+        self.device = torch.device(device)
+        self.embedding = None
+        if embedding is not None:
+            self.load_dense(embedding)
+        self.init_lora(max_lora_adapters=max_lora_adapters, max_lora_rank=max_lora_rank,
+                       shape_A=(max_lora_adapters, num_embeddings, max_lora_rank),
+                       shape_B=(max_lora_adapters, max_lora_rank, features), device=self.device)
+
+    def load_dense(self, table: torch.Tensor) -> None:
+        """A [num_embeddings, features] table, kept as bf16."""
+        if tuple(table.shape) != (self.num_embeddings, self.features):
+            raise ValueError(f"table must be {(self.num_embeddings, self.features)}, got {tuple(table.shape)}")
+        self.embedding = table.to(device=self.device, dtype=torch.bfloat16).contiguous()
+
+    def __call__(self, ids: torch.Tensor, adapter_indices: torch.Tensor | None = None) -> torch.Tensor:
+        if self.embedding is None:
+            raise RuntimeError("the table is not loaded: call load_dense()")
+        out = emb.embed(self.embedding, ids)
+        if not self._lora_active(adapter_indices):
+            return out
+        if ids.ndim == 0 or adapter_indices.ndim != 1 or adapter_indices.shape[0] != ids.shape[0]:
+            raise ValueError("adapter_indices must hold one entry per example (leading axis of ids)")
+        n_ad = self.max_lora_adapters
+        flat = ids.reshape(-1)
+        adapters = adapter_indices.clamp(-1, n_ad).to(device=flat.device, dtype=torch.int32).repeat_interleave(flat.numel() // adapter_indices.shape[0])
+        order = None
+        sizes = torch.full((1,), flat.numel(), dtype=torch.int32, device=flat.device)
+        if n_ad > 1:
+            _, sizes, order, _, _ = w8.moe_dispatch(None, adapters, n_ad)
+            flat, adapters = flat[order], adapters[order]
+        z = emb.embed(self.lora_A, flat, self.lora_scaling, adapter_indices=adapters)
+        delta = bf16_grouped_linear(_whole_units(z, 1), _whole_units(self.lora_B, 1), sizes)
+        if order is not None:
+            delta = torch.zeros_like(delta).index_copy(0, order.long(), delta)
+        return out + delta.reshape(out.shape)
+
+
 class LoRAExpert(LoRAMixin):
     """Expert layer (ragged per-expert linear) with multi-adapter LoRA (lora.py:354-444).
 
@@ -171,7 +235,8 @@ class LoRAExpert(LoRAMixin):
     pairs are indexed ``expert * max_lora_adapters + adapter`` (lora.py:414-431): rows are
     stably re-sorted by that combined index, run through the grouped kernel with
     ``max_lora_adapters`` LoRA groups per expert weight, and put back.  Differentiable: the backward
-    is one native grouped call for all experts and adapters.
+    is one native grouped call for all experts and adapters.  With ``load_dense`` the kernels stay bf16 (and
+    differentiable): the base and the two low-rank factors are ragged bf16 products.
     """
 
     def __init__(self, num_experts: int, in_features: int, out_features: int, *,
@@ -180,6 +245,7 @@ class LoRAExpert(LoRAMixin):
         self.num_experts, self.in_features, self.out_features = int(num_experts), int(in_features), int(out_features)
         self.device = torch.device(device)
         self.weight = weight
+        self.dense = None
         self.init_lora(max_lora_adapters=max_lora_adapters, max_lora_rank=max_lora_rank,
                        shape_A=(max_lora_adapters, num_experts, in_features, max_lora_rank),
                        shape_B=(max_lora_adapters, num_experts, max_lora_rank, out_features), device=self.device)
@@ -189,15 +255,25 @@ class LoRAExpert(LoRAMixin):
         if tuple(codes.shape) != (self.num_experts, self.in_features, self.out_features):
             raise ValueError(f"codes must be {(self.num_experts, self.in_features, self.out_features)}")
         self.weight = w8.prepare_grouped_weight(codes.to(self.device), scales.to(self.device))
+        self.dense = None
+
+    def load_dense(self, kernels: torch.Tensor) -> None:
+        """[E, in, out] kernels, kept as bf16 instead of codes."""
+        if tuple(kernels.shape) != (self.num_experts, self.in_features, self.out_features):
+            raise ValueError(f"kernels must be {(self.num_experts, self.in_features, self.out_features)}, got {tuple(kernels.shape)}")
+        self.dense = kernels.to(device=self.device, dtype=torch.bfloat16).contiguous()
+        self.weight = None
 
     def __call__(self, x: torch.Tensor, group_sizes: torch.Tensor, adapter_indices_sorted: torch.Tensor | None = None,
                  *, group_offset: torch.Tensor | None = None) -> torch.Tensor:
-        if self.weight is None:
-            raise RuntimeError("the expert kernels are not loaded: call load_quantized()")
+        if self.weight is None and self.dense is None:
+            raise RuntimeError("the expert kernels are not loaded: call load_quantized() or load_dense()")
         if group_offset is not None and int(torch.as_tensor(group_offset).reshape(-1)[0]) != 0:
             raise NotImplementedError("expert shards (group_offset != 0) belong to the multi-GPU dispatch, "
                                       "which this one-GPU build leaves out")
         if not self._lora_active(adapter_indices_sorted):
+            if self.dense is not None:
+                return bf16_grouped_linear(x, self.dense, group_sizes)
             return w8.grouped_lora_linear(x, group_sizes, self.weight)
         n_ad, n_exp = self.max_lora_adapters, self.num_experts
         gs = group_sizes.to(device=x.device, dtype=torch.int64)
@@ -217,6 +293,11 @@ class LoRAExpert(LoRAMixin):
         a = self.lora_A.transpose(0, 1).reshape(n_exp * n_ad, self.in_features, self.max_lora_rank)
         b = self.lora_B.transpose(0, 1).reshape(n_exp * n_ad, self.max_lora_rank, self.out_features)
         scaling = self.lora_scaling.repeat(n_exp)
+        if self.dense is not None:
+            z = bf16_grouped_linear(x[order], _whole_units(a, 2), sizes)
+            factor = scaling[combined[order].clamp(max=n_exp * n_ad - 1)]
+            delta = bf16_grouped_linear((z.float() * factor[:, None]).to(torch.bfloat16), _whole_units(b, 1), sizes)
+            return bf16_grouped_linear(x, self.dense, group_sizes) + torch.zeros_like(delta).index_copy(0, order, delta)
         out_sorted = w8.grouped_lora_linear(x[order], sizes, self.weight, a.contiguous(), b.contiguous(), scaling,
                                             groups_per_weight=n_ad)
         return torch.zeros_like(out_sorted).index_copy(0, order, out_sorted)
@@ -245,3 +326,22 @@ def init_lora_adapter(layer: LoRAMixin, adapter_index: int, *, rank: int, alpha:
     a[..., effective:] = 0.0
     layer.lora_A[adapter_index] = a.to(device=layer.lora_A.device, dtype=torch.bfloat16)
     layer.lora_B[adapter_index] = 0
+
+
+def clip_adapter_gradients(layers, max_norm) -> torch.Tensor:
+    """Scale the adapters' gradients in place so that, for each adapter, their norm over all ``layers`` does not exceed
+    ``max_norm`` (a number, or float32 [max_lora_adapters]: each adapter is another model that trains beside the others).
+    Returns the float32 norms [max_lora_adapters] before scaling.  Layers whose adapters have no gradient are left out, a layer or
+    parameter that is named twice counts once."""
+    grads, seen = [], set()
+    for layer in layers:
+        for p in (layer.lora_A, layer.lora_B):
+            if p is None or p.grad is None or id(p) in seen:  # (shared parameters count once)
+                continue
+            seen.add(id(p))
+            if not p.grad.is_contiguous():
+                p.grad = p.grad.contiguous()
+            grads.append(p.grad)
+    if not grads:
+        raise ValueError("none of the layers has adapter gradients")
+    return grad_clip.clip_grad_norm_(grads, max_norm, per_adapter=True)

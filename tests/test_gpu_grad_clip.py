@@ -130,3 +130,14 @@ def test_plan_reads_its_buffers_at_every_run_and_replays(gc):
         want, wn = gc.clip_grad_norm(grads, limits, per_adapter=True)
         torch.cuda.synchronize()
         assert torch.equal(norms, wn) and all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_a_gradient_given_twice(gc):
+    grad = torch.ones(4, 8, device=DEV)
+    with pytest.raises(ValueError, match="twice"):
+        gc.clip_grad_norm_([grad, grad], 1.0)
+    with pytest.raises(ValueError, match="twice|overlap"):
+        gc.clip_grad_norm_([grad, grad[0]], 1.0)
+    (one, two), norm = gc.clip_grad_norm([grad, grad], 4.0)
+    assert float(norm) == 8.0 and torch.equal(one, two) and one.data_ptr() != two.data_ptr() and float(one[0, 0]) == 0.5
+    assert float(gc.grad_norm([grad, grad])) == 8.0
