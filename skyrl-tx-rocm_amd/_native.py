@@ -71,7 +71,8 @@ EXPORTS = (
 # called by the torch mirror alone (csrc/w8a8_gq_bwd_api.h, csrc/bf16_api.h)
 PRIVATE_EXPORTS = (
     "mi355_w8a8_gq_bwd_workspace_bytes", "mi355_w8a8_gq_linear_bwd_v1",
-    "mi355_w8a8_bf16_grouped_v1", "mi355_w8a8_bf16_grouped_bwd_v1",
+    "mi355_w8a8_bf16_grouped_workspace_bytes", "mi355_w8a8_bf16_grouped_bwd_workspace_bytes", "mi355_w8a8_bf16_grouped_v1",
+    "mi355_w8a8_bf16_grouped_bwd_v1",
     "mi355_w8a8_embedding_v1", "mi355_w8a8_embedding_bwd_workspace_bytes", "mi355_w8a8_embedding_bwd_v1",
     "mi355_w8a8_grad_workspace_bytes", "mi355_w8a8_grad_norm_v1", "mi355_w8a8_grad_clip_v1",
 )
@@ -231,7 +232,7 @@ class Bf16GroupedProblem(ctypes.Structure):
 
     _fields_ = [
         ("struct_size", _u32), ("flags", _u32), ("m", _u32), ("k", _u32), ("n", _u32), ("n_groups", _u32),
-        ("x", _vp), ("weight", _vp), ("group_sizes", _vp), ("out", _vp),
+        ("x", _vp), ("weight", _vp), ("group_sizes", _vp), ("out", _vp), ("workspace", _vp), ("workspace_bytes", _u64),
     ]
 
 
@@ -240,7 +241,8 @@ class Bf16GroupedBwdProblem(ctypes.Structure):
 
     _fields_ = [
         ("struct_size", _u32), ("flags", _u32), ("m", _u32), ("k", _u32), ("n", _u32), ("n_groups", _u32),
-        ("x", _vp), ("dy", _vp), ("weight", _vp), ("group_sizes", _vp), ("dx", _vp), ("dw", _vp),
+        ("x", _vp), ("dy", _vp), ("weight", _vp), ("group_sizes", _vp), ("dx", _vp), ("dw", _vp), ("workspace", _vp),
+        ("workspace_bytes", _u64),
     ]
 
 
@@ -361,6 +363,10 @@ def _bind(lib: ctypes.CDLL) -> None:
         fn = getattr(lib, f"mi355_w8a8_{name}_v1")
         fn.restype = ctypes.c_int
         fn.argtypes = (ctypes.POINTER(struct), _vp)
+    lib.mi355_w8a8_bf16_grouped_workspace_bytes.restype = _u64
+    lib.mi355_w8a8_bf16_grouped_workspace_bytes.argtypes = (_u32,) * 5
+    lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes.restype = _u64
+    lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes.argtypes = (_u32,) * 7
     lib.mi355_w8a8_embedding_bwd_workspace_bytes.restype = _u64
     lib.mi355_w8a8_embedding_bwd_workspace_bytes.argtypes = (_u32,) * 5
     lib.mi355_w8a8_grad_workspace_bytes.restype = _u64
@@ -425,6 +431,8 @@ def host():
                                  ("residual", "lora_residual_v1"), ("workspace_bytes", "workspace_bytes"), ("forward_path", "forward_path"),
                                  ("gq_linear", "gq_linear_v1"), ("gq_workspace_bytes", "gq_workspace_bytes"),
                                  ("bf16_grouped", "bf16_grouped_v1"), ("bf16_grouped_bwd", "bf16_grouped_bwd_v1"), ("embedding", "embedding_v1"),
+                                 ("bf16_grouped_workspace_bytes", "bf16_grouped_workspace_bytes"),
+                                 ("bf16_grouped_bwd_workspace_bytes", "bf16_grouped_bwd_workspace_bytes"),
                                  ("embedding_bwd", "embedding_bwd_v1"), ("embedding_bwd_workspace_bytes", "embedding_bwd_workspace_bytes")):
                     entry_address[name] = ctypes.cast(getattr(lib, f"mi355_w8a8_{fn}"), ctypes.c_void_p).value
                 _host = module

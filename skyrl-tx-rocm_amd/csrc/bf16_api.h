@@ -32,6 +32,8 @@ typedef struct mi355_w8a8_bf16_grouped_problem {
   const void* weight;       /* bf16 [n_groups, k, n] */
   const int32_t* group_sizes; /* int32 [n_groups] */
   void* out;                /* bf16 [m, n] */
+  void* workspace;          /* 256-byte aligned device scratch; may be NULL where no bytes are needed */
+  uint64_t workspace_bytes; /* >= mi355_w8a8_bf16_grouped_workspace_bytes(...) */
 } mi355_w8a8_bf16_grouped_problem;
 #define MI355_W8A8_FLAG_BF16_GROUPED_DW_F32 1u /* dw is float32 */
 typedef struct mi355_w8a8_bf16_grouped_bwd_problem {
@@ -44,7 +46,13 @@ typedef struct mi355_w8a8_bf16_grouped_bwd_problem {
   const int32_t* group_sizes; /* int32 [n_groups] */
   void* dx;                 /* bf16 [m, k], or NULL: not wanted */
   void* dw;                 /* bf16 or float32 [n_groups, k, n], or NULL: not wanted */
+  void* workspace;          /* as above, for what dx and dw need one after the other */
+  uint64_t workspace_bytes; /* >= mi355_w8a8_bf16_grouped_bwd_workspace_bytes(...) */
 } mi355_w8a8_bf16_grouped_bwd_problem;
+/* Scratch of a call: nothing, or the parts of a long contraction that few tiles share.  0 also for sizes that a call refuses. */
+uint64_t mi355_w8a8_bf16_grouped_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags);
+uint64_t mi355_w8a8_bf16_grouped_bwd_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags, uint32_t want_dx,
+                                                     uint32_t want_dw);
 int mi355_w8a8_bf16_grouped_v1(const mi355_w8a8_bf16_grouped_problem* problem, void* stream);
 int mi355_w8a8_bf16_grouped_bwd_v1(const mi355_w8a8_bf16_grouped_bwd_problem* problem, void* stream);
 

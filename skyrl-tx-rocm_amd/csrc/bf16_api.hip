@@ -55,12 +55,17 @@ int launch_grouped_tiles(const BgArgs& g, hipStream_t s) {
   auto kernel = &bf16_grouped_kernel<KIND, TM, TN, WM, WN, STAGES, LOADERS, F32>;
   const uint32_t lds = (TM + TN) * kBgDepth * 2u * STAGES + (kBgScratch + 2u * (g.groups + 2u)) * 4u;
   if (!allow_lds(kernel, lds)) return MI355_W8A8_ERR_LAUNCH;
-  const uint64_t n_tiles = (g.cols + TN - 1u) / TN;
+  const uint64_t n_tiles = (g.cols + TN - 1u) / TN * g.splits;
   const uint64_t tiles = n_tiles * (KIND == kGroupedDw ? (uint64_t)g.groups * ((g.rows + TM - 1u) / TM) : most_row_tiles(g.m, g.groups + 1u, TM));
   const uint32_t grid = (uint32_t)(tiles < 256u ? (tiles + 7u) / 8u * 8u : 256u);  // (one workgroup a CU: its stages fill the LDS)
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * (WM * WN + LOADERS)), lds, s, g);
   return launch_status();
 }
+
+struct GroupedPlan {
+  uint32_t tile;    // one of kGroupedTiles
+  uint32_t splits;  // of the contraction
+};
 
 // Which tiles.  A call costs the rounds of its tiles on the 256 CUs times what a round takes: 4 units for 256 x 256, 2.2 for 128 x 256 and
 // 1.15 for 64 x 128 (half and an eighth of the products; 32768 rows of 4096 -> 12288 in 8 groups 2740, 3060 and 6100 us).  Groups end
@@ -68,29 +73,79 @@ int launch_grouped_tiles(const BgArgs& g, hipStream_t s) {
 // weights come from memory for few rows.  us, 256 x 256 / 128 x 256 / 64 x 128, 2048 -> 1536, 128 groups of uneven sizes: forward 16384 rows 235 / 197 /
 // 250, 8192 224 / 176 / 194, 512 172 / 142 / 146, 64 100 / 70 / 60, dW 16384 rows 259 / 245 / 373, 8192 180 / 194 / 286; 4096 -> 4096, 4 groups,
 // 2048 rows 91 / 109 / 133; 1024 -> 1024, 8 groups, 4096 rows 31 / 23 / 29.
-template <int KIND, bool F32 = false>
-int launch_grouped(const BgArgs& g, uint32_t forced, hipStream_t s) {
-  auto cost = [&](uint32_t tm, uint32_t tn, float round) {
-    const float held = (float)(g.groups < g.m ? g.groups : g.m);
-    const float row_tiles = KIND == kGroupedDw ? (float)((uint64_t)g.groups * ((g.rows + tm - 1u) / tm)) : fmaxf((float)g.m / tm + 0.5f * held, held);
-    return ceilf(row_tiles * ((g.cols + tn - 1u) / tn) / 256.0f) * round;
+// rows: of C a group (dW); depth: contraction of forward and dx.
+GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols, uint32_t depth, uint32_t forced) {
+  if (forced) return {forced, 1u};
+  const float held = (float)(groups < m ? groups : m);
+  auto tiles = [&](uint32_t tm, uint32_t tn) {
+    const float row_tiles = kind == kGroupedDw ? (float)((uint64_t)groups * ((rows + tm - 1u) / tm)) : fmaxf((float)m / tm + 0.5f * held, held);
+    return row_tiles * ((cols + tn - 1u) / tn);
   };
-  if (forced == MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
-  if (forced == MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
-  if (forced) return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
-  const float large = cost(256u, 256u, 4.0f), middle = cost(128u, 256u, 2.2f), small = cost(64u, 128u, 1.15f);
+  const float large = ceilf(tiles(256u, 256u) / 256.0f) * 4.0f, middle = ceilf(tiles(128u, 256u) / 256.0f) * 2.2f;
+  const float small_tiles = tiles(64u, 128u), small = ceilf(small_tiles / 256.0f) * 1.15f;
+  uint32_t tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128;
+  float round_us = 0.47f;  // a round's time for each stage
   // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 23 / 20.5)
-  if (KIND == kGroupedDw && large == 4.0f && g.m / g.groups < 8u * kBgDepth) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
-  if (large <= middle && large <= small) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
-  if (middle <= small) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
+  const bool shallow = kind == kGroupedDw && large == 4.0f && m / groups < 8u * kBgDepth;
+  if (!shallow && large <= middle && large <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256, round_us = large / 4.0f * 1.7f;
+  else if (shallow || middle <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256, round_us = middle / 2.2f * 0.95f;
+  else round_us *= small / 1.15f;
+  // Few tiles of a long contraction leave most CUs idle: then parts of it are products of their own, of small tiles with float32 results,
+  // that a second launch adds up (4 us, and the parts written and read).  Neither is faster than the operands come from memory.
+  const uint32_t stages = bg_stages(kind == kGroupedDw ? (uint32_t)((float)m / held) : depth);
+  const float bytes = kind == kGroupedDw ? (float)m * (rows + cols) * 2.0f : (held * cols + (float)m) * depth * 2.0f;
+  const float values = kind == kGroupedDw ? (float)groups * rows * cols : (float)m * cols, memory_us = bytes / 5.0e6f;
+  float best = 0.9f * fmaxf(round_us * (stages + 3.0f), memory_us);
+  uint32_t splits = 1;
+  for (uint32_t n = 2; n <= 64u && n * 2u <= stages && small_tiles * n <= 1024.0f; ++n) {
+    const uint32_t each = (stages + n - 1u) / n;
+    const float us = fmaxf(ceilf(small_tiles * n / 256.0f) * 0.47f * (each + 3.0f), memory_us) + 4.0f + values * n * 8.0f / 5.0e6f;
+    if (us < best) best = us, splits = n;
+  }
+  return {splits > 1u ? MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128 : tile, splits};
+}
+
+inline uint64_t grouped_plane(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols) {
+  return kind == kGroupedDw ? (uint64_t)groups * rows * cols : (uint64_t)m * cols;
+}
+uint64_t grouped_workspace(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols, uint32_t depth, uint32_t forced) {
+  const GroupedPlan plan = plan_grouped(kind, m, groups, rows, cols, depth, forced);
+  return plan.splits > 1u ? plan.splits * grouped_plane(kind, m, groups, rows, cols) * 4u : 0u;
+}
+
+template <int KIND, bool F32 = false>
+int launch_grouped(BgArgs g, uint32_t forced, void* workspace, hipStream_t s) {
+  const GroupedPlan plan = plan_grouped((GroupedKind)KIND, g.m, g.groups, g.rows, g.cols, g.depth, forced);
+  g.splits = plan.splits;
+  if (plan.splits > 1u) {
+    void* const out = g.out;
+    g.out = workspace;
+    g.plane = grouped_plane((GroupedKind)KIND, g.m, g.groups, g.rows, g.cols);
+    const int st = launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, true>(g, s);
+    if (st) return st;
+    hipLaunchKernelGGL(bg_join_kernel<F32>, dim3((uint32_t)((g.plane / 4u + 255u) / 256u)), dim3(256), 0, s, static_cast<const float*>(workspace), out, g.plane,
+                       g.splits);
+    return launch_status();
+  }
+  if (plan.tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
+  if (plan.tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
   return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
+}
+
+int check_grouped_workspace(const void* workspace, uint64_t given, uint64_t needed) {
+  if (needed && (!workspace || given < needed)) return MI355_W8A8_ERR_WORKSPACE;
+  return workspace && !aligned(workspace, 256) ? MI355_W8A8_ERR_ALIGN : MI355_W8A8_OK;
+}
+uint64_t grouped_bwd_workspace(uint32_t m, uint32_t k, uint32_t n, uint32_t groups, uint32_t forced, bool dx, bool dw) {  // (one after the other)
+  const uint64_t a = dx ? grouped_workspace(kGroupedDx, m, groups, 0u, k, n, forced) : 0u, b = dw ? grouped_workspace(kGroupedDw, m, groups, k, n, 0u, forced) : 0u;
+  return a > b ? a : b;
 }
 
 int run_grouped(const mi355_w8a8_bf16_grouped_problem* p, hipStream_t s) {
   if (!p) return MI355_W8A8_ERR_NULL;
   if (p->struct_size != sizeof(mi355_w8a8_bf16_grouped_problem)) return MI355_W8A8_ERR_STRUCT;
   if ((p->flags & ~kGroupedTiles) || !one_bit_at_most(p->flags)) return MI355_W8A8_ERR_SHAPE;
-  const int st = check_grouped_dims(p->m, p->k, p->n, p->n_groups);
+  int st = check_grouped_dims(p->m, p->k, p->n, p->n_groups);
   if (st) return st;
   if (!p->x || !p->weight || !p->group_sizes || !p->out) return MI355_W8A8_ERR_NULL;
   if (!aligned(p->x, 16) || !aligned(p->weight, 16) || !aligned(p->out, 16) || !aligned(p->group_sizes, 4)) return MI355_W8A8_ERR_ALIGN;
@@ -99,13 +154,18 @@ int run_grouped(const mi355_w8a8_bf16_grouped_problem* p, hipStream_t s) {
       overlaps(p->out, out_bytes, p->weight, (uint64_t)p->n_groups * p->k * p->n * 2u) ||
       overlaps(p->out, out_bytes, p->group_sizes, (uint64_t)p->n_groups * 4u))
     return MI355_W8A8_ERR_ALIAS;
+  const uint64_t needed = grouped_workspace(kGroupedFwd, p->m, p->n_groups, 0u, p->n, p->k, p->flags);
+  if ((st = check_grouped_workspace(p->workspace, p->workspace_bytes, needed))) return st;
+  if (overlaps(p->workspace, needed, p->out, out_bytes) || overlaps(p->workspace, needed, p->x, (uint64_t)p->m * p->k * 2u) ||
+      overlaps(p->workspace, needed, p->weight, (uint64_t)p->n_groups * p->k * p->n * 2u) || overlaps(p->workspace, needed, p->group_sizes, (uint64_t)p->n_groups * 4u))
+    return MI355_W8A8_ERR_ALIAS;
   (void)hipGetLastError();
   BgArgs g{};
   g.a = static_cast<const uint16_t*>(p->x); g.b = static_cast<const uint16_t*>(p->weight);
   g.sizes = p->group_sizes; g.out = p->out;
   g.m = p->m; g.rows_ld = p->k; g.cols_ld = p->n; g.depth = p->k; g.cols = p->n; g.groups = p->n_groups;
   g.b_group = (uint64_t)p->k * p->n;
-  return launch_grouped<kGroupedFwd>(g, p->flags, s);
+  return launch_grouped<kGroupedFwd>(g, p->flags, p->workspace, s);
 }
 
 int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s) {
@@ -122,14 +182,16 @@ int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s)
   const bool f32 = p->flags & MI355_W8A8_FLAG_BF16_GROUPED_DW_F32;
   const uint64_t x_bytes = (uint64_t)p->m * p->k * 2u, dy_bytes = (uint64_t)p->m * p->n * 2u, sizes_bytes = (uint64_t)p->n_groups * 4u;
   const uint64_t values = (uint64_t)p->n_groups * p->k * p->n, dw_bytes = values * (f32 ? 4u : 2u);
-  const void* outs[2] = {p->dx, p->dw};
-  const uint64_t bytes[2] = {x_bytes, dw_bytes};
-  for (int i = 0; i < 2; ++i) {
+  const uint64_t needed = grouped_bwd_workspace(p->m, p->k, p->n, p->n_groups, forced, p->dx, p->dw);
+  if ((st = check_grouped_workspace(p->workspace, p->workspace_bytes, needed))) return st;
+  const void* outs[3] = {p->dx, p->dw, p->workspace};
+  const uint64_t bytes[3] = {x_bytes, dw_bytes, needed};
+  for (int i = 0; i < 3; ++i) {
     if (overlaps(outs[i], bytes[i], p->dy, dy_bytes) || overlaps(outs[i], bytes[i], p->x, x_bytes) ||
         overlaps(outs[i], bytes[i], p->weight, values * 2u) || overlaps(outs[i], bytes[i], p->group_sizes, sizes_bytes))
       return MI355_W8A8_ERR_ALIAS;
   }
-  if (overlaps(p->dx, x_bytes, p->dw, dw_bytes)) return MI355_W8A8_ERR_ALIAS;
+  if (overlaps(p->dx, x_bytes, p->dw, dw_bytes) || overlaps(p->workspace, needed, p->dx, x_bytes) || overlaps(p->workspace, needed, p->dw, dw_bytes)) return MI355_W8A8_ERR_ALIAS;
   (void)hipGetLastError();
   BgArgs g{};
   g.sizes = p->group_sizes; g.m = p->m; g.groups = p->n_groups;
@@ -137,13 +199,13 @@ int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s)
     g.a = static_cast<const uint16_t*>(p->dy); g.b = static_cast<const uint16_t*>(p->weight); g.out = p->dx;
     g.rows_ld = p->n; g.cols_ld = p->n; g.depth = p->n; g.cols = p->k;
     g.b_group = (uint64_t)p->k * p->n;
-    if ((st = launch_grouped<kGroupedDx>(g, forced, s))) return st;
+    if ((st = launch_grouped<kGroupedDx>(g, forced, p->workspace, s))) return st;
   }
   if (p->dw) {
     g.a = static_cast<const uint16_t*>(p->x); g.b = static_cast<const uint16_t*>(p->dy); g.out = p->dw;
     g.rows_ld = p->k; g.cols_ld = p->n; g.depth = 0; g.cols = p->n; g.rows = p->k;
     g.out_group = (uint64_t)p->k * p->n;
-    st = f32 ? launch_grouped<kGroupedDw, true>(g, forced, s) : launch_grouped<kGroupedDw>(g, forced, s);
+    st = f32 ? launch_grouped<kGroupedDw, true>(g, forced, p->workspace, s) : launch_grouped<kGroupedDw>(g, forced, p->workspace, s);
   }
   return st;
 }
@@ -436,6 +498,13 @@ int run_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, co
 
 extern "C" {
 
+uint64_t mi355_w8a8_bf16_grouped_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags) {
+  return check_grouped_dims(m, k, n, n_groups) ? 0u : grouped_workspace(kGroupedFwd, m, n_groups, 0u, n, k, flags & kGroupedTiles);
+}
+uint64_t mi355_w8a8_bf16_grouped_bwd_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags, uint32_t want_dx,
+                                                     uint32_t want_dw) {
+  return check_grouped_dims(m, k, n, n_groups) ? 0u : grouped_bwd_workspace(m, k, n, n_groups, flags & kGroupedTiles, want_dx, want_dw);
+}
 int mi355_w8a8_bf16_grouped_v1(const mi355_w8a8_bf16_grouped_problem* problem, void* stream) {
   return run_grouped(problem, static_cast<hipStream_t>(stream));
 }

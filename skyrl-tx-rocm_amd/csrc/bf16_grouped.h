@@ -47,6 +47,8 @@ struct BgArgs {
   uint32_t cols, rows;           // columns of C; rows of C a group (dW)
   uint32_t groups;
   uint64_t b_group, out_group;   // elements between groups of b and of C (forward, dx: of b alone)
+  uint32_t splits;               // float32 results: parts of the contraction, each with a C of its own ..
+  uint64_t plane;                // .. this many elements behind the one before (1 part: C itself)
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -78,7 +80,7 @@ __device__ inline void buffer_store_16(v4i v, v4i rsrc, uint32_t voff) {
 }
 
 // (a tile without products has one stage, of zeros)
-__device__ inline uint32_t bg_stages(uint32_t depth) { return depth ? (depth + kBgDepth - 1u) / kBgDepth : 1u; }
+__host__ __device__ inline uint32_t bg_stages(uint32_t depth) { return depth ? (depth + kBgDepth - 1u) / kBgDepth : 1u; }
 
 // Tables of a call in the LDS, made by every workgroup from the sizes: the first row and the first tile of every group (and of the rows
 // behind the last one, which are a group of their own for the forward and dx).
@@ -226,23 +228,29 @@ struct BgOperand {
                        __builtin_amdgcn_readfirstlane(lds + index * 1024u));
   }
   __device__ inline void next() { base += ALONG ? BK * 2u : BK * ld_bytes; }
-  // the lane's eight contraction values 32 step + 8 (lane / 16) .. of fragment f
-  __device__ static inline v8bf fragment(const unsigned char* tile, uint32_t first, int f, int step, uint32_t lane) {
-    const uint32_t i = lane & 15u, q = lane >> 4;
+  // Where the lane reads, from the tile's place in the LDS, for fragment 0 of the rows or columns that begin at `first` and step 0.
+  __device__ static inline uint32_t lane_place(uint32_t first, uint32_t lane) {
+    const uint32_t i = lane & 15u, q = lane >> 4, c = i & 3u;
     if constexpr (ALONG) {
-      const uint32_t row = first + (PAIRED ? 32u * (f >> 1) + 8u * (i >> 2) + 4u * ((f ^ (i >> 2)) & 1u) + (i & 3u) : 16u * f + i);
-      const uint32_t unit = (4u * step + q) ^ bg_unit_along<BK, PAIRED>(row);
-      return *reinterpret_cast<const v8bf*>(tile + row * (BK * 2u) + unit * 16u);
+      const uint32_t row = first + (PAIRED ? 8u * (i >> 2) + 4u * ((i >> 2) & 1u) + c : i);
+      return row * (BK * 2u) + (q ^ bg_unit_along<BK, PAIRED>(row)) * 16u;
+    } else {
+      const uint32_t t = 8u * q + (i >> 2), col = first + (PAIRED ? 8u * c + 4u * (c & 1u) : 4u * c);
+      return t * (T * 2u) + ((col >> 3) ^ (bg_unit_across<PAIRED>(t) % (T / 8u))) * 16u + (col & 4u) * 2u;
+    }
+  }
+  // The lane's eight contraction values 32 step + 8 (lane / 16) .. of fragment f; `at`: the tile's place and the lane's.  Fragments lie an exclusive
+  // or or a constant apart (no permutation depends on f, step or the wave), so that a lane keeps one register of addresses an operand.
+  __device__ static inline v8bf fragment(uint32_t at, int f, int step) {
+    if constexpr (ALONG) {
+      typedef __attribute__((address_space(3))) const v8bf* lds_v8bf;
+      return PAIRED ? *(lds_v8bf)(uintptr_t)((at ^ (512u * (f & 1) + 64u * step)) + 4096u * (f >> 1)) : *(lds_v8bf)(uintptr_t)((at ^ (64u * step)) + 2048u * f);
     } else {
       typedef __attribute__((address_space(3))) v4s* lds_v4s;
-      const uint32_t c = i & 3u, col = first + (PAIRED ? 32u * (f >> 1) + 8u * c + 4u * ((f ^ c) & 1u) : 16u * f + 4u * c);
+      const uint32_t place = at ^ (PAIRED ? 64u * (f >> 1) + 8u * (f & 1) : 32u * f);
       v4s h[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t t = 32u * step + 8u * q + 4u * u + (i >> 2);
-        const uint32_t unit = (col >> 3) ^ (bg_unit_across<PAIRED>(t) % (T / 8u));
-        h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(tile + t * (T * 2u) + unit * 16u + (col & 4u) * 2u));
-      }
+      for (int u = 0; u < 2; ++u) h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(uintptr_t)(place + (32u * step + 4u * u) * (T * 2u)));
       typedef short v8s __attribute__((ext_vector_type(8)));
       const v8s v = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
       return __builtin_bit_cast(v8bf, v);
@@ -253,6 +261,9 @@ struct BgOperand {
 // One tile of a call.
 struct BgTile {
   uint32_t group, start, row0, col0, rows, depth;  // rows: of the tile's group from row0 on (at least one); start: the group's first row
+  uint32_t split, first;  // part of the contraction; its first index (depth: of the part)
+  uint32_t number;        // of the tile in its group (and part)
+  bool empty;             // the group has no rows
 };
 
 // TM x TN tiles, WM x WN waves, STAGES stages of 64 in the LDS.  LOADERS: waves that do nothing but request the stages (0: every wave its
@@ -279,9 +290,12 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
   const uint32_t held = KIND == kGroupedDw ? g.groups : g.groups + 1u;
   const BgShare share = bg_tables<64 * (kWaves + LOADERS)>(
       g, held, tab, scratch,
-      [&](uint32_t rows) { return ((KIND == kGroupedDw ? g.rows : rows) + TM - 1u) / TM * n_tiles; },
+      [&](uint32_t rows) { return ((KIND == kGroupedDw ? g.rows : rows) + TM - 1u) / TM * n_tiles * (F32 ? g.splits : 1u); },
       // (a tile's results take about as long to store as three of its stages to compute)
-      [&](uint32_t group, uint32_t rows) { return 3u + bg_stages(KIND == kGroupedDw ? rows : (group < g.groups ? g.depth : 0u)); });
+      [&](uint32_t group, uint32_t rows) {
+        const uint32_t stages = bg_stages(KIND == kGroupedDw ? rows : (group < g.groups ? g.depth : 0u));
+        return 3u + (F32 ? (stages + g.splits - 1u) / g.splits : stages);
+      });
   const uint32_t stride = gridDim.x >> 3, end = share.end;
   uint32_t tile = share.first + (blockIdx.x >> 3);
   if (tile >= end) return;
@@ -291,16 +305,26 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
     d.group = __builtin_amdgcn_readfirstlane(bg_group_of(tab.tile, held, t, lane));
     d.start = __builtin_amdgcn_readfirstlane(tab.start[d.group]);
     const uint32_t size = __builtin_amdgcn_readfirstlane(tab.start[d.group + 1u]) - d.start;
-    const uint32_t in_group = t - __builtin_amdgcn_readfirstlane(tab.tile[d.group]);
+    uint32_t in_group = t - __builtin_amdgcn_readfirstlane(tab.tile[d.group]);
     // the row tiles of a group in bands of eight, in a band column by column: workgroups that run side by side share both operands
     const uint32_t m_tiles = ((KIND == kGroupedDw ? g.rows : size) + TM - 1u) / TM;
+    d.depth = KIND == kGroupedDw ? size : (d.group == g.groups ? 0u : g.depth);
+    d.split = d.first = 0;
+    if (F32 && g.splits > 1u) {  // part by part, whole stages each
+      const uint32_t each = (bg_stages(d.depth) + g.splits - 1u) / g.splits * BK;
+      d.split = in_group / (m_tiles * n_tiles);
+      in_group -= d.split * m_tiles * n_tiles;
+      d.first = d.split * each < d.depth ? d.split * each : d.depth;
+      d.depth = d.depth - d.first < each ? d.depth - d.first : each;
+    }
+    d.number = in_group;
+    d.empty = size == 0u;
     const uint32_t band = in_group / (8u * n_tiles), in_band = in_group - band * 8u * n_tiles;
     const uint32_t band_tiles = m_tiles - band * 8u < 8u ? m_tiles - band * 8u : 8u;
     const uint32_t tn = in_band / band_tiles;
     d.row0 = (band * 8u + in_band - tn * band_tiles) * TM;
     d.col0 = tn * TN;
     d.rows = (KIND == kGroupedDw ? g.rows : size) - d.row0;
-    d.depth = KIND == kGroupedDw ? size : (d.group == g.groups ? 0u : g.depth);
     return d;
   };
   OpA a;
@@ -312,12 +336,12 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
     const BgTile d = describe(t);
     left = d.depth;
     if constexpr (KIND == kGroupedDw) {
-      a.open(g.a + (uint64_t)d.start * g.rows_ld + d.row0, d.rows);
-      b.open(g.b + (uint64_t)d.start * g.cols_ld + d.col0, g.cols - d.col0);
+      a.open(g.a + (uint64_t)(d.start + d.first) * g.rows_ld + d.row0, d.rows);
+      b.open(g.b + (uint64_t)(d.start + d.first) * g.cols_ld + d.col0, g.cols - d.col0);
     } else {
       const uint16_t* w = g.b + (uint64_t)(d.group == g.groups ? 0u : d.group) * g.b_group;
-      a.open(g.a + (uint64_t)(d.start + d.row0) * g.rows_ld, d.rows);
-      b.open(w + (KIND == kGroupedFwd ? (uint64_t)d.col0 : (uint64_t)d.col0 * g.cols_ld), g.cols - d.col0);
+      a.open(g.a + (uint64_t)(d.start + d.row0) * g.rows_ld + d.first, d.rows);
+      b.open(w + (KIND == kGroupedFwd ? (uint64_t)d.first * g.cols_ld + d.col0 : (uint64_t)d.col0 * g.cols_ld + d.first), g.cols - d.col0);
     }
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr_t)lds, loader = LOADERS ? wave - kWaves : wave;
@@ -365,10 +389,11 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
   const uint32_t wm = wave / WN, wn = wave % WN;
   v4f acc[FM][FN];
   v8bf fa[2][FM], fb[2][FN];
+  const uint32_t place_a = lds0 + OpA::lane_place(wm * (TM / WM), lane), place_b = lds0 + OpA::kBytes + OpB::lane_place(wn * (TN / WN), lane);
   auto fetch = [&](uint32_t s, int step, int f) {  // columns' fragments first
-    const unsigned char* at = lds + (s % STAGES) * kStage;
-    if (f < FN) fb[step][f] = OpB::fragment(at + OpA::kBytes, wn * (TN / WN), f, step, lane);
-    else fa[step][f - FN] = OpA::fragment(at, wm * (TM / WM), f - FN, step, lane);
+    const uint32_t at = (s % STAGES) * kStage;
+    if (f < FN) fb[step][f] = OpB::fragment(at + place_b, f, step);
+    else fa[step][f - FN] = OpA::fragment(at + place_a, f - FN, step);
   };
   // Half of a stage's products, and between them, so that neither waits for the other, the fragments of the next half out of the LDS
   // and (LOAD) the requests of the stage after next.  A wave issues in order: with the reads and requests in front of
@@ -402,14 +427,17 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
   // bytes of either half of a row's 128-byte line; lanes eight rows apart exchange one, and an instruction stores eight whole lines.
   auto store = [&](const BgTile& d) {
     constexpr uint32_t size = F32 ? 4u : 2u, kLine = 128u / size;
-    const uint64_t at = (KIND == kGroupedDw ? d.group * g.out_group : (uint64_t)d.start * g.cols) + (uint64_t)d.row0 * g.cols + d.col0;
+    const uint64_t at = (KIND == kGroupedDw ? d.group * g.out_group : (uint64_t)d.start * g.cols) + (uint64_t)d.row0 * g.cols + d.col0 +
+                        (F32 ? d.split * g.plane : 0u);
     const v4i out = buffer_of(static_cast<unsigned char*>(g.out) + at * size);
     // A dW is larger than the caches and leaves x and dy there no room: it is streamed where its rows are whole lines (us, streamed /
     // not, 768 -> 2048, 128 groups, 32768 rows: bf16 162 / 184, float32 205 / 269; parts of lines are not joined on that way: 712 ->
     // 1096, 13 groups, 1003 rows, float32 28 / 23).
-    const bool stream = KIND == kGroupedDw && g.cols * size % 128u == 0u;
-    const bool high = lane & 8u;
-    const uint32_t row = lane & 7u, col = (lane >> 4) * (16u / size) + (high ? kLine / 2u : 0u), voff = (row * g.cols + col) * size;
+    const bool stream = KIND == kGroupedDw && g.cols * size % 128u == 0u && !(F32 && g.splits > 1u);
+    uint32_t own = lane;
+    asm volatile("" : "+v"(own));  // (offsets are made anew for every tile: kept over the products they would be spilled)
+    const bool high = own & 8u;
+    const uint32_t row = own & 7u, col = (own >> 4) * (16u / size) + (high ? kLine / 2u : 0u), voff = (row * g.cols + col) * size;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const uint32_t r0 = wm * (TM / WM) + 16u * i;
@@ -451,6 +479,25 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
     }
   };
 
+  // The dW of a group without rows is one stretch of zeros (whole lines: K and N are multiples of 8), a tile's share of it as many bytes as a
+  // tile holds: the same stores, but line after line.
+  auto clear = [&](const BgTile& d) {
+    constexpr uint32_t size = F32 ? 4u : 2u;
+    const uint64_t all = (uint64_t)g.rows * g.cols * size, from = (uint64_t)d.number * (TM * TN * size);
+    const uint64_t left_bytes = from < all ? all - from : 0u;
+    const uint32_t held_bytes = left_bytes < TM * TN * size ? (uint32_t)left_bytes : TM * TN * size;
+    const v4i out = buffer_of(static_cast<unsigned char*>(g.out) + (d.group * g.out_group + (F32 ? d.split * g.plane : 0u)) * size + from);
+    const bool stream = !(F32 && g.splits > 1u);
+    uint32_t own = lane;
+    asm volatile("" : "+v"(own));
+#pragma nounroll
+    for (uint32_t i = 0; i < kStores; ++i) {
+      const uint32_t at = (wave * kStores + i) * 1024u + own * 16u;
+      if (stream) buffer_store_16<true>(v4i{0, 0, 0, 0}, out, at < held_bytes ? at : kOutside);
+      else buffer_store_16<false>(v4i{0, 0, 0, 0}, out, at < held_bytes ? at : kOutside);
+    }
+  };
+
   constexpr std::integral_constant<int, 0> first{};
   constexpr std::integral_constant<int, 1> second{};
   if constexpr (!LOADERS) {
@@ -481,10 +528,26 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
       half(second, s + 1u, std::true_type{}, s + STAGES, std::false_type{});
       if constexpr (!LOADERS) requested();
     }
-    store(d);
+    if (KIND == kGroupedDw && d.empty) clear(d);
+    else store(d);
     stored = true;
   }
   if constexpr (!LOADERS) wait_vmcnt0();
+}
+
+// The parts of a split contraction: C = their sum in order, with the one rounding.  A thread four values of C.
+template <bool F32>
+__global__ __launch_bounds__(256) void bg_join_kernel(const float* parts, void* out, uint64_t plane, uint32_t splits) {
+  const uint64_t i = ((uint64_t)blockIdx.x * 256u + threadIdx.x) * 4u;
+  if (i >= plane) return;
+  float4 sum = *reinterpret_cast<const float4*>(parts + i);
+#pragma unroll 8
+  for (uint32_t s = 1; s < splits; ++s) {
+    const float4 p = *reinterpret_cast<const float4*>(parts + s * plane + i);
+    sum.x += p.x; sum.y += p.y; sum.z += p.z; sum.w += p.w;
+  }
+  if constexpr (F32) *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = sum;
+  else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
 }
 
 }  // namespace w8a8

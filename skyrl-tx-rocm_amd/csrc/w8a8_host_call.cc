@@ -220,21 +220,22 @@ bool grouped_dims(int64_t m, int64_t k, int64_t n, int64_t g) {
          n <= MI355_W8A8_BF16_GROUPED_MAX_FEATURES && g > 0 && g <= 1024;
 }
 
-// grouped(x, weight, group_sizes, flags, entry, stream)
+// grouped(x, weight, group_sizes, flags, entry, workspace_bytes, stream)
 PyObject* grouped(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
-  if (argc != 6) { PyErr_SetString(PyExc_TypeError, "grouped takes 6 arguments"); return nullptr; }
+  if (argc != 7) { PyErr_SetString(PyExc_TypeError, "grouped takes 7 arguments"); return nullptr; }
   HANDLE_TH_ERRORS
   Args arg{argv};
   const at::Tensor *x = arg.tensor(0), *w = arg.tensor(1), *sizes = arg.tensor(2);
   const int64_t flags = arg.integer(3);
   const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_bf16_grouped_problem*, void*)>(arg.address(4));
-  void* const stream = arg.address(5);
-  if (!arg.ok || !entry || !here(x)) Py_RETURN_NONE;
+  const auto bytes_of = reinterpret_cast<uint64_t (*)(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t)>(arg.address(5));
+  void* const stream = arg.address(6);
+  if (!arg.ok || !entry || !bytes_of || !here(x)) Py_RETURN_NONE;
   const c10::Device device = x->device();
   if (!whole(x, at::kBFloat16, device, 2) || !whole(w, at::kBFloat16, device, 3) || !sizes || !plain(*sizes, at::kInt, device) || sizes->dim() != 1) Py_RETURN_NONE;
   const int64_t m = x->size(0), k = x->size(1), n = w->size(2), g = w->size(0);
   if (w->size(1) != k || sizes->size(0) != g || !grouped_dims(m, k, n, g)) Py_RETURN_NONE;
-  at::Tensor out;
+  at::Tensor out, ws;
   int status;
   {
     const WithoutGil released;
@@ -245,30 +246,36 @@ PyObject* grouped(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     p.m = (uint32_t)m; p.k = (uint32_t)k; p.n = (uint32_t)n; p.n_groups = (uint32_t)g;
     p.x = x->const_data_ptr(); p.weight = w->const_data_ptr(); p.group_sizes = sizes->const_data_ptr<int32_t>();
     p.out = out.mutable_data_ptr();
+    p.workspace_bytes = bytes_of(p.m, p.k, p.n, p.n_groups, p.flags);
+    if (p.workspace_bytes) {
+      ws = at::empty({(int64_t)p.workspace_bytes}, x->options().requires_grad(false).dtype(at::kByte));
+      p.workspace = ws.mutable_data_ptr();
+    }
     status = entry(&p, stream);
   }
   return finish(std::move(out), status);
   END_HANDLE_TH_ERRORS
 }
 
-// grouped_bwd(x, dy, weight, group_sizes, need_dx, need_dw, f32, flags, entry, stream)
+// grouped_bwd(x, dy, weight, group_sizes, need_dx, need_dw, f32, flags, entry, workspace_bytes, stream)
 PyObject* grouped_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
-  if (argc != 10) { PyErr_SetString(PyExc_TypeError, "grouped_bwd takes 10 arguments"); return nullptr; }
+  if (argc != 11) { PyErr_SetString(PyExc_TypeError, "grouped_bwd takes 11 arguments"); return nullptr; }
   HANDLE_TH_ERRORS
   Args arg{argv};
   const at::Tensor *x = arg.tensor(0), *dy = arg.tensor(1), *w = arg.tensor(2), *sizes = arg.tensor(3);
   const bool need_dx = argv[4] == Py_True, need_dw = argv[5] == Py_True, f32 = argv[6] == Py_True;
   const int64_t flags = arg.integer(7);
   const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_bf16_grouped_bwd_problem*, void*)>(arg.address(8));
-  void* const stream = arg.address(9);
-  if (!arg.ok || !entry || !here(dy) || !x || !w) Py_RETURN_NONE;
+  const auto bytes_of = reinterpret_cast<uint64_t (*)(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t)>(arg.address(9));
+  void* const stream = arg.address(10);
+  if (!arg.ok || !entry || !bytes_of || !here(dy) || !x || !w) Py_RETURN_NONE;
   const c10::Device device = dy->device();
   if (!whole(dy, at::kBFloat16, device, 2) || !whole(x, at::kBFloat16, device, 2) || !whole(w, at::kBFloat16, device, 3) || !sizes ||
       !plain(*sizes, at::kInt, device) || sizes->dim() != 1)
     Py_RETURN_NONE;
   const int64_t m = dy->size(0), k = w->size(1), n = w->size(2), g = w->size(0);
   if (dy->size(1) != n || x->size(0) != m || x->size(1) != k || sizes->size(0) != g || !grouped_dims(m, k, n, g)) Py_RETURN_NONE;
-  at::Tensor dx, dw;
+  at::Tensor dx, dw, ws;
   int status;
   {
     const WithoutGil released;
@@ -281,6 +288,11 @@ PyObject* grouped_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     p.x = x->const_data_ptr(); p.dy = dy->const_data_ptr(); p.weight = w->const_data_ptr(); p.group_sizes = sizes->const_data_ptr<int32_t>();
     p.dx = need_dx ? dx.mutable_data_ptr() : nullptr;
     p.dw = need_dw ? dw.mutable_data_ptr() : nullptr;
+    p.workspace_bytes = bytes_of(p.m, p.k, p.n, p.n_groups, p.flags, need_dx, need_dw);
+    if (p.workspace_bytes) {
+      ws = at::empty({(int64_t)p.workspace_bytes}, dy->options().requires_grad(false).dtype(at::kByte));
+      p.workspace = ws.mutable_data_ptr();
+    }
     status = entry(&p, stream);
   }
   if (status) return PyLong_FromLong(status);

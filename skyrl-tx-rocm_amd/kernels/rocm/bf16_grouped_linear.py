@@ -70,7 +70,8 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Ten
     host = _native.host() if isinstance(x, torch.Tensor) and x.is_cuda else None
     if host is not None:
         # an ordinary call goes through the host module; for any other it returns None
-        result = host.grouped(x, weight, group_sizes, flags, _native.entry_address["bf16_grouped"], _stream_ptr(x.device))
+        result = host.grouped(x, weight, group_sizes, flags, _native.entry_address["bf16_grouped"],
+                              _native.entry_address["bf16_grouped_workspace_bytes"], _stream_ptr(x.device))
         if type(result) is int:
             _native.check("mi355_w8a8_bf16_grouped_v1", result)
         if result is not None:
@@ -79,10 +80,12 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Ten
     _same_device(x, weight)
     m, k, n, g, sizes = _geometry(x, "x", 1, weight.shape, group_sizes)
     out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+    lib = _native.load()
+    ws = torch.empty(lib.mi355_w8a8_bf16_grouped_workspace_bytes(m, k, n, g, flags), dtype=torch.uint8, device=x.device)
     p = _native.Bf16GroupedProblem(ctypes.sizeof(_native.Bf16GroupedProblem), flags, m, k, n, g, xc.data_ptr(), w.data_ptr(),
-                                   sizes.data_ptr(), out.data_ptr())
+                                   sizes.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel())
     with _on(x.device):
-        status = _native.load().mi355_w8a8_bf16_grouped_v1(ctypes.byref(p), _stream_ptr(x.device))
+        status = lib.mi355_w8a8_bf16_grouped_v1(ctypes.byref(p), _stream_ptr(x.device))
     _native.check("mi355_w8a8_bf16_grouped_v1", status)
     return out
 
@@ -101,7 +104,8 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
     host = _native.host() if isinstance(dy, torch.Tensor) and dy.is_cuda else None
     if host is not None:
         result = host.grouped_bwd(x, dy, weight, group_sizes, need_dx, need_dw, dw_dtype == torch.float32, flags,
-                                  _native.entry_address["bf16_grouped_bwd"], _stream_ptr(dy.device))
+                                  _native.entry_address["bf16_grouped_bwd"], _native.entry_address["bf16_grouped_bwd_workspace_bytes"],
+                                  _stream_ptr(dy.device))
         if type(result) is int:
             _native.check("mi355_w8a8_bf16_grouped_bwd_v1", result)
         if result is not None:
@@ -116,12 +120,15 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
         raise ValueError(f"x must be [{m}, {k}], got {tuple(x.shape)}")
     dx = torch.empty((m, k), dtype=torch.bfloat16, device=dy.device) if need_dx else None
     dw = torch.empty((g, k, n), dtype=dw_dtype, device=dy.device) if need_dw else None
+    lib = _native.load()
+    ws = torch.empty(lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes(m, k, n, g, flags, need_dx, need_dw), dtype=torch.uint8, device=dy.device)
     p = _native.Bf16GroupedBwdProblem(ctypes.sizeof(_native.Bf16GroupedBwdProblem),
                                       flags | (_native.FLAG_BF16_GROUPED_DW_F32 if dw_dtype == torch.float32 else 0), m, k, n, g,
                                       xc.data_ptr() if need_dw else None, d.data_ptr(), w.data_ptr() if need_dx else None,
-                                      sizes.data_ptr(), dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None)
+                                      sizes.data_ptr(), dx.data_ptr() if need_dx else None, dw.data_ptr() if need_dw else None,
+                                      ws.data_ptr(), ws.numel())
     with _on(dy.device):
-        status = _native.load().mi355_w8a8_bf16_grouped_bwd_v1(ctypes.byref(p), _stream_ptr(dy.device))
+        status = lib.mi355_w8a8_bf16_grouped_bwd_v1(ctypes.byref(p), _stream_ptr(dy.device))
     _native.check("mi355_w8a8_bf16_grouped_bwd_v1", status)
     return dx, dw
 

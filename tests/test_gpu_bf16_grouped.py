@@ -108,6 +108,26 @@ def test_longest_depths(gl):
         check(gl, x, w, dy, st, sizes, torch.float32)
 
 
+@pytest.mark.parametrize("rows,k,n,sizes,parts", [
+    (1, 4096, 512, [0, 1, 0], "f"), (1, 512, 4104, [1], "d"), (8, 704, 8952, [0, 2, 1, 0, 5, 0], "d"), (70, 4168, 72, [9, 0, 30, 1, 20], "f"),
+    (200, 72, 4232, [9, 0, 130, 1, 20], "d"), (9000, 8, 520, [9000], "w"), (9100, 264, 40, [5000, 0, 4000], "w"), (4100, 4096, 8, [1000, 2000, 0, 1000], "f"),
+    (64, 4096, 4096, [1, 0, 63], "fd"), (300, 65536, 16, [100, 7, 150], "f")])
+def test_parts_of_a_long_contraction(gl, rows, k, n, sizes, parts):
+    lib = load_package()._native.load()
+    m, g = rows, len(sizes)
+    assert ("f" in parts) == (lib.mi355_w8a8_bf16_grouped_workspace_bytes(m, k, n, g, 0) > 0)
+    assert ("d" in parts) == (lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes(m, k, n, g, 0, 1, 0) > 0)
+    assert ("w" in parts) == (lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes(m, k, n, g, 0, 0, 1) > 0)
+    assert lib.mi355_w8a8_bf16_grouped_workspace_bytes(m, k, n, g, 16) == 0
+    x, w, dy, st = make(rows, k, n, sizes, seed=5)
+    check(gl, x, w, dy, st, sizes)
+    check(gl, x, w, dy, st, sizes, torch.float32)
+    first = gl.grouped_matmul(x, w, st), *gl.grouped_matmul_backward(x, dy, w, st)
+    assert all(torch.equal(a, b) for a, b in zip(first, (gl.grouped_matmul(x, w, st), *gl.grouped_matmul_backward(x, dy, w, st))))
+    if sum(sizes) < rows:
+        assert not first[0][sum(sizes):].any() and not first[1][sum(sizes):].any()
+
+
 @pytest.mark.parametrize("flags", [0, 4, 8, 16])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_values_of_other_rows_stay_there(gl, bad, flags):

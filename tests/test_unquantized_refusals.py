@@ -50,6 +50,25 @@ def test_grouped_backward_call(native, change, status):
     assert native.load().mi355_w8a8_bf16_grouped_bwd_v1(ctypes.byref(p), None) == status
 
 
+def test_grouped_workspace(native):
+    lib = native.load()
+    sizes = dict(m=1, k=4096, n=4096, n_groups=8)
+    need = lib.mi355_w8a8_bf16_grouped_workspace_bytes(1, 4096, 4096, 8, 0)
+    back = lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes(1, 4096, 4096, 8, 0, 1, 1)
+    assert need >= 2 * 4096 * 4 and back >= 2 * 4096 * 4
+    assert lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes(1, 4096, 4096, 8, 0, 0, 0) == 0 and lib.mi355_w8a8_bf16_grouped_workspace_bytes(1, 12, 8, 8, 0) == 0
+    W = A + 9 * STEP
+    for change, status in ((dict(), -5), (dict(workspace=W, workspace_bytes=need - 1), -5), (dict(workspace=W + 64, workspace_bytes=need), -3),
+                           (dict(workspace=A + 3 * STEP, workspace_bytes=need), -4), (dict(workspace=A + STEP, workspace_bytes=need), -4)):
+        p = fill(native.Bf16GroupedProblem, **{**sizes, **dict(x=A, weight=A + STEP, group_sizes=A + 8 * STEP, out=A + 3 * STEP), **change})
+        assert lib.mi355_w8a8_bf16_grouped_v1(ctypes.byref(p), None) == status, change
+    for change, status in ((dict(), -5), (dict(workspace=W, workspace_bytes=back - 1), -5), (dict(workspace=W + 64, workspace_bytes=back), -3),
+                           (dict(workspace=A + 5 * STEP, workspace_bytes=back), -4), (dict(workspace=A + 3 * STEP, workspace_bytes=back), -4)):
+        p = fill(native.Bf16GroupedBwdProblem, **{**sizes, **dict(x=A, dy=A + STEP, weight=A + 3 * STEP, dx=A + 2 * STEP, dw=A + 5 * STEP,
+                                                                  group_sizes=A + 8 * STEP), **change})
+        assert lib.mi355_w8a8_bf16_grouped_bwd_v1(ctypes.byref(p), None) == status, change
+
+
 @pytest.mark.parametrize("change,status", [
     (dict(struct_size=8), -8), (dict(flags=4), -2), (dict(n_tokens=0), -2), (dict(vocab=0), -2), (dict(width=0), -2),
     (dict(n_tokens=(1 << 20) + 1), -7), (dict(width=65537), -7), (dict(vocab=(1 << 30) + 1), -7), (dict(n_adapters=2), -1),
