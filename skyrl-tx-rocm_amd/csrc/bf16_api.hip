@@ -252,8 +252,8 @@ int run_embedding(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
   const uint64_t out_bytes = (uint64_t)p->n_tokens * p->width * size;
   if (overlaps(p->out, out_bytes, p->table, embedding_rows(p) * p->width * size) || overlaps_indices(p, p->out, out_bytes)) return MI355_W8A8_ERR_ALIAS;
   const EmbedArgs e = embed_args(p);
-  const bool wide = p->width % (16u / size) == 0 && aligned(p->table, 16) && aligned(p->out, 16);
-  const uint64_t threads = (uint64_t)p->n_tokens * (wide ? p->width / (16u / size) : p->width);
+  const bool wide = p->width >= 16u / size;
+  const uint64_t threads = (uint64_t)p->n_tokens * embed_units(p->width, wide ? 16u / size : 1u);
   const dim3 grid(blocks_of(threads)), block(256);
   (void)hipGetLastError();
   if (size == 4u) {
@@ -280,7 +280,7 @@ EmbedLayout embed_layout(uint32_t n, uint64_t rows, uint32_t width, uint32_t fla
   L.bits = (bits + L.passes - 1u) / L.passes;
   L.chunks = (n + kEmbedChunk - 1u) / kEmbedChunk;
   const uint32_t vec = flags & MI355_W8A8_FLAG_EMBEDDING_F32 ? 4u : 8u;
-  const uint64_t units = width % vec ? width : width / vec;
+  const uint64_t units = embed_units(width, width >= vec ? vec : 1u);
   L.run = 8;
   while (L.run < 256u && (uint64_t)n * units / (L.run * 2u) >= 524288u) L.run *= 2u;
   L.runs = (n + L.run - 1u) / L.run;
@@ -300,15 +300,16 @@ EmbedLayout embed_layout(uint32_t n, uint64_t rows, uint32_t width, uint32_t fla
 
 template <typename T, int V>
 int launch_embed_sums(const EmbedSumArgs& a, hipStream_t s) {
-  const uint32_t units = a.e.width / V;
+  const uint32_t units = embed_units(a.e.width, V);
   const dim3 block(256);
   const dim3 grid(blocks_of((uint64_t)a.runs * (units >= 64u ? (units + 63u) / 64u * 64u : units)));
   if (units >= 64u) hipLaunchKernelGGL((embed_sum_kernel<T, V, true>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((embed_sum_kernel<T, V, false>), grid, block, 0, s, a);
   const int st = launch_status();
   if (st || a.runs < 2u) return st;
-  const uint64_t most = ((uint64_t)a.runs * units + 255u) / 256u;
-  hipLaunchKernelGGL((embed_join_kernel<T, V>), dim3((uint32_t)(most < 2048u ? most : 2048u)), block, 0, s, a);
+  constexpr int kJoin = V < 4 ? V : 4;
+  const uint64_t most = ((uint64_t)a.runs * embed_units(a.e.width, kJoin) + 255u) / 256u;
+  hipLaunchKernelGGL((embed_join_kernel<T, kJoin>), dim3((uint32_t)(most < 2048u ? most * 2u : 2048u + kEmbedLongs)), block, 0, s, a);
   return launch_status();
 }
 
@@ -331,11 +332,14 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
   a.e = embed_args(p);
   a.bits = L.bits; a.passes = L.passes; a.chunks = L.chunks;
   a.notes = words(L.notes);
-  // the launches that place the keys clear a share of the gradient each
+  // the launches that count clear a share of the gradient each (in those that place the reads would wait behind so many stores: 20 MB beside
+  // 32768 tokens 12 us instead of 9), by 256 workgroups (they write 6.0 TB/s, 2048 of them 5.5), and past the caches where
+  // the last one, 256 MiB, does not hold it (the rows of dy stay there then: 778 MB 193 us in all, 199 through the caches; 102 MB 26 and 23)
   const uint64_t pieces = out_bytes / 16u;
   const bool small = L.chunks == 1u;
   const uint32_t launches = small ? 1u : L.passes;
   uint32_t launched = 0, clearing = 0;
+  a.stream = out_bytes > (256u << 20);
   auto share = [&] {
     const uint64_t each = pieces / launches;
     const bool last = launched + 1u == launches;
@@ -343,7 +347,7 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
     a.clear_pieces = last ? pieces - launched * each : each;
     a.clear_rest = last ? (uint32_t)(out_bytes % 16u) : 0u;
     const uint64_t wanted = (a.clear_pieces + 4095u) / 4096u + (a.clear_rest ? 1u : 0u);
-    clearing = (uint32_t)(wanted < 2048u ? wanted : 2048u);
+    clearing = (uint32_t)(wanted < 256u ? wanted : 256u);
     ++launched;
   };
   const uint32_t place_lds = (kEmbedDigits + 16u) * 4u + (32u << L.bits), small_lds = place_lds + 8192u;
@@ -364,15 +368,15 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
       a.keys_out = words(L.keys[pass & 1u]);
       a.tokens_out = words(L.tokens[pass & 1u]);
       a.shift = pass * L.bits;
-      hipLaunchKernelGGL(embed_count_kernel, dim3(L.chunks), dim3(1024), 0, s, a);
+      share();
+      hipLaunchKernelGGL(embed_count_kernel, dim3(L.chunks + clearing), dim3(1024), 0, s, a);
       if ((st = launch_status())) return st;
       if (scan) {
         hipLaunchKernelGGL(embed_scan_kernel, dim3(1), dim3(1024), 0, s, a);
         if ((st = launch_status())) return st;
       }
-      share();
-      if (scan) hipLaunchKernelGGL(embed_place_kernel<true>, dim3(L.chunks + clearing), dim3(1024), place_lds, s, a);
-      else hipLaunchKernelGGL(embed_place_kernel<false>, dim3(L.chunks + clearing), dim3(1024), place_lds, s, a);
+      if (scan) hipLaunchKernelGGL(embed_place_kernel<true>, dim3(L.chunks), dim3(1024), place_lds, s, a);
+      else hipLaunchKernelGGL(embed_place_kernel<false>, dim3(L.chunks), dim3(1024), place_lds, s, a);
       if ((st = launch_status())) return st;
     }
   }
@@ -382,7 +386,7 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
   b.parts = reinterpret_cast<float*>(ws + L.parts);
   b.joins = words(L.joins); b.notes = a.notes;
   b.run = L.run; b.runs = L.runs;
-  const bool wide = p->width % (16u / size) == 0 && aligned(p->d_out, 16);
+  const bool wide = p->width >= 16u / size;
   if (size == 4u) return wide ? launch_embed_sums<float, 4>(b, s) : launch_embed_sums<float, 1>(b, s);
   return wide ? launch_embed_sums<uint16_t, 8>(b, s) : launch_embed_sums<uint16_t, 1>(b, s);
 }

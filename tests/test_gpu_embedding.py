@@ -114,6 +114,30 @@ def test_gradient_of_adapters(em, n_ad, vocab, width, n):
     check_grad(em, torch.randn(n, width, generator=g, device=DEV).to(BF16), ids, (n_ad, vocab, width), scale, index)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("width", [5, 9, 15, 513, 3415])
+def test_rows_that_begin_anywhere(em, dtype, width):
+    """Widths that are no multiple of 16 bytes, from views that begin in the middle of a buffer; the values around them stay."""
+    g = gen(7)
+    for vocab, n, hot in ((700, 1500, 0.5), (40, 700, 0.0)):
+        ids = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+        ids[torch.rand(n, generator=g, device=DEV) < hot] = 3
+        buffer = torch.randn(n * width + 9, generator=g, device=DEV).to(dtype)
+        dy = buffer[3:3 + n * width].view(n, width)
+        check_grad(em, dy, ids, (vocab, width), -0.7)
+        assert torch.equal(em.lookup(dy, ids % n, 3.0), (dy[ids % n].float() * 3.0).to(dtype))
+
+
+@pytest.mark.parametrize("n", [20000, 300000])
+def test_a_row_of_very_many_tokens(em, n):
+    """One word nearly everywhere: parts by the thousand; whole numbers, whose float32 sums are exact in any order."""
+    ids = torch.full((n,), 17, device=DEV)
+    ids[:: 1000] = torch.arange(n // 1000, device=DEV) % 50
+    dy = torch.randint(-3, 4, (n, 24), generator=gen(8), device=DEV).float()
+    got = em.lookup_backward(dy, ids, (60, 24))
+    assert torch.equal(got, torch.zeros(60, 24, device=DEV, dtype=torch.float64).index_add_(0, ids, dy.double()).float())
+
+
 def test_more_bits_than_two_passes(em):
     """2^25 table rows: three passes of the sort."""
     g = gen(4)
