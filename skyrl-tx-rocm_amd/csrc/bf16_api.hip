@@ -81,8 +81,9 @@ GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t
     const float row_tiles = kind == kGroupedDw ? (float)((uint64_t)groups * ((rows + tm - 1u) / tm)) : fmaxf((float)m / tm + 0.5f * held, held);
     return row_tiles * ((cols + tn - 1u) / tn);
   };
-  const float large = ceilf(tiles(256u, 256u) / 256.0f) * 4.0f, middle = ceilf(tiles(128u, 256u) / 256.0f) * 2.2f;
-  const float small_tiles = tiles(64u, 128u), small = ceilf(small_tiles / 256.0f) * 1.15f;
+  auto rounds = [](float n) { return n <= 256.0f ? 1.0f : n / 256.0f + 0.5f; };  // (how many tiles the groups make is not known, nor whether they fill the last round)
+  const float small_tiles = tiles(64u, 128u), middle_tiles = tiles(128u, 256u);
+  const float large = rounds(tiles(256u, 256u)) * 4.0f, middle = rounds(middle_tiles) * 2.2f, small = rounds(small_tiles) * 1.15f;
   uint32_t tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128;
   float round_us = 0.47f;  // a round's time for each stage
   // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 23 / 20.5)
@@ -90,19 +91,25 @@ GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t
   if (!shallow && large <= middle && large <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256, round_us = large / 4.0f * 1.7f;
   else if (shallow || middle <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256, round_us = middle / 2.2f * 0.95f;
   else round_us *= small / 1.15f;
-  // Few tiles of a long contraction leave most CUs idle: then parts of it are products of their own, of small tiles with float32 results,
-  // that a second launch adds up (4 us, and the parts written and read).  Neither is faster than the operands come from memory.
+  // Few tiles of a long contraction leave most CUs idle: then parts of it are products of their own, with float32 results
+  // that a second launch adds up (4 us, and the parts written and read).  Neither is faster than the operands come from memory.  us, whole / in
+  // parts: 1 row of 4096 -> 4096 28 / 14.7, 8 rows of 8952 -> 704 in 6 groups 81 / 29, 64 rows of 4096 -> 64 in 16 groups 29 / 12.7; dW of 272 -> 1696
+  // in 4 groups of 28533 rows 97 / 55.
   const uint32_t stages = bg_stages(kind == kGroupedDw ? (uint32_t)((float)m / held) : depth);
   const float bytes = kind == kGroupedDw ? (float)m * (rows + cols) * 2.0f : (held * cols + (float)m) * depth * 2.0f;
   const float values = kind == kGroupedDw ? (float)groups * rows * cols : (float)m * cols, memory_us = bytes / 5.0e6f;
   float best = 0.9f * fmaxf(round_us * (stages + 3.0f), memory_us);
   uint32_t splits = 1;
-  for (uint32_t n = 2; n <= 64u && n * 2u <= stages && small_tiles * n <= 1024.0f; ++n) {
-    const uint32_t each = (stages + n - 1u) / n;
-    const float us = fmaxf(ceilf(small_tiles * n / 256.0f) * 0.47f * (each + 3.0f), memory_us) + 4.0f + values * n * 8.0f / 5.0e6f;
-    if (us < best) best = us, splits = n;
+  for (uint32_t n = 2; n <= 64u && n * 2u <= stages && middle_tiles * n <= 1024.0f; ++n) {
+    const float each = (float)((stages + n - 1u) / n) + 3.0f;
+    const float s = ceilf(small_tiles * n / 256.0f) * 0.47f * each, m2 = ceilf(middle_tiles * n / 256.0f) * 0.95f * each;
+    const float us = fmaxf(s < m2 ? s : m2, memory_us) + 4.0f + values * n * 8.0f / 5.0e6f;
+    if (us >= best) continue;
+    best = us;
+    splits = n;
+    tile = s < m2 ? MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128 : MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256;
   }
-  return {splits > 1u ? MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128 : tile, splits};
+  return {tile, splits};
 }
 
 inline uint64_t grouped_plane(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols) {
@@ -121,7 +128,8 @@ int launch_grouped(BgArgs g, uint32_t forced, void* workspace, hipStream_t s) {
     void* const out = g.out;
     g.out = workspace;
     g.plane = grouped_plane((GroupedKind)KIND, g.m, g.groups, g.rows, g.cols);
-    const int st = launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, true>(g, s);
+    const int st = plan.tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128 ? launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, true>(g, s)
+                                                                         : launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, true>(g, s);
     if (st) return st;
     hipLaunchKernelGGL(bg_join_kernel<F32>, dim3((uint32_t)((g.plane / 4u + 255u) / 256u)), dim3(256), 0, s, static_cast<const float*>(workspace), out, g.plane,
                        g.splits);

@@ -111,7 +111,8 @@ def test_longest_depths(gl):
 @pytest.mark.parametrize("rows,k,n,sizes,parts", [
     (1, 4096, 512, [0, 1, 0], "f"), (1, 512, 4104, [1], "d"), (8, 704, 8952, [0, 2, 1, 0, 5, 0], "d"), (70, 4168, 72, [9, 0, 30, 1, 20], "f"),
     (200, 72, 4232, [9, 0, 130, 1, 20], "d"), (9000, 8, 520, [9000], "w"), (9100, 264, 40, [5000, 0, 4000], "w"), (4100, 4096, 8, [1000, 2000, 0, 1000], "f"),
-    (64, 4096, 4096, [1, 0, 63], "fd"), (300, 65536, 16, [100, 7, 150], "f")])
+    (64, 4096, 4096, [1, 0, 63], "fd"), (300, 65536, 16, [100, 7, 150], "f"), (520, 8200, 1032, [300, 200], "f"), (520, 1032, 8200, [17, 503], "d"),
+    (20000, 272, 1696, [7000, 0, 12000, 900], "w")])
 def test_parts_of_a_long_contraction(gl, rows, k, n, sizes, parts):
     lib = load_package()._native.load()
     m, g = rows, len(sizes)
