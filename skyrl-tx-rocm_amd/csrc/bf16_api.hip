@@ -68,11 +68,11 @@ struct GroupedPlan {
 };
 
 // Which tiles.  A call costs the rounds of its tiles on the 256 CUs times what a round takes: 4 units for 256 x 256, 2.2 for 128 x 256 and
-// 1.15 for 64 x 128 (half and an eighth of the products; 32768 rows of 4096 -> 12288 in 8 groups 2740, 3060 and 6100 us).  Groups end
+// 1.15 for 64 x 128 (half and an eighth of the products; 32768 rows of 4096 -> 12288 in 8 groups 2640, 3000 and 6020 us).  Groups end
 // in the middle of a tile, half a tile on average.  The smaller tiles have room for more stages, which is what counts where the
-// weights come from memory for few rows.  us, 256 x 256 / 128 x 256 / 64 x 128, 2048 -> 1536, 128 groups of uneven sizes: forward 16384 rows 235 / 197 /
-// 250, 8192 224 / 176 / 194, 512 172 / 142 / 146, 64 100 / 70 / 60, dW 16384 rows 259 / 245 / 373, 8192 180 / 194 / 286; 4096 -> 4096, 4 groups,
-// 2048 rows 91 / 109 / 133; 1024 -> 1024, 8 groups, 4096 rows 31 / 23 / 29.
+// weights come from memory for few rows.  us, 256 x 256 / 128 x 256 / 64 x 128, 2048 -> 1536, 128 groups of uneven sizes: forward 16384 rows 242 / 212 /
+// 242, 8192 226 / 179 / 195, 512 165 / 129 / 138, 64 91 / 60 / 53, dW 16384 rows 217 / 218 / 335, 8192 172 / 178 / 269; 4096 -> 4096, 4 groups,
+// 2048 rows 96 / 70 / 126; 1024 -> 1024, 8 groups, 4096 rows 27 / 19 / 19; 512 -> 512, 16 groups, 16384 rows 21 / 17 / 21.5.
 // rows: of C a group (dW); depth: contraction of forward and dx.
 GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols, uint32_t depth, uint32_t forced) {
   if (forced) return {forced, 1u};
@@ -86,15 +86,15 @@ GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t
   const float large = rounds(tiles(256u, 256u)) * 4.0f, middle = rounds(middle_tiles) * 2.2f, small = rounds(small_tiles) * 1.15f;
   uint32_t tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128;
   float round_us = 0.47f;  // a round's time for each stage
-  // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 23 / 20.5)
+  // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 22 / 18)
   const bool shallow = kind == kGroupedDw && large == 4.0f && m / groups < 8u * kBgDepth;
   if (!shallow && large <= middle && large <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256, round_us = large / 4.0f * 1.7f;
   else if (shallow || middle <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256, round_us = middle / 2.2f * 0.95f;
   else round_us *= small / 1.15f;
   // Few tiles of a long contraction leave most CUs idle: then parts of it are products of their own, with float32 results
   // that a second launch adds up (4 us, and the parts written and read).  Neither is faster than the operands come from memory.  us, whole / in
-  // parts: 1 row of 4096 -> 4096 28 / 14.7, 8 rows of 8952 -> 704 in 6 groups 81 / 29, 64 rows of 4096 -> 64 in 16 groups 29 / 12.7; dW of 272 -> 1696
-  // in 4 groups of 28533 rows 97 / 55.
+  // parts: 1 row of 4096 -> 4096 27 / 14.4, 8 rows of 8952 -> 704 in 6 groups 52 / 22, 64 rows of 4096 -> 64 in 16 groups 27 / 13, dW of 272 -> 1696
+  // in 4 groups of 28533 rows 78 / 57.
   const uint32_t stages = bg_stages(kind == kGroupedDw ? (uint32_t)((float)m / held) : depth);
   const float bytes = kind == kGroupedDw ? (float)m * (rows + cols) * 2.0f : (held * cols + (float)m) * depth * 2.0f;
   const float values = kind == kGroupedDw ? (float)groups * rows * cols : (float)m * cols, memory_us = bytes / 5.0e6f;

@@ -398,7 +398,7 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
   // Half of a stage's products, and between them, so that neither waits for the other, the fragments of the next half out of the LDS
   // and (LOAD) the requests of the stage after next.  A wave issues in order: with the reads and requests in front of
   // the products both waves of a SIMD, which the barrier holds together, left the matrix unit idle meanwhile (32768 rows of 4096 ->
-  // 12288 in 8 groups 2840 us, 2660 this way).
+  // 12288 in 8 groups 2840 us, 2660 this way, and 2600 with the addresses of OpA and OpB::fragment).
   auto half = [&](auto step_c, uint32_t s_fetch, auto load_c, uint32_t s_load, auto fresh_c) {  // FRESH: a tile's first sums
     constexpr int step = step_c.value, next = 1 - step;
     constexpr bool load = load_c.value, fresh = fresh_c.value;
@@ -431,8 +431,8 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
                         (F32 ? d.split * g.plane : 0u);
     const v4i out = buffer_of(static_cast<unsigned char*>(g.out) + at * size);
     // A dW is larger than the caches and leaves x and dy there no room: it is streamed where its rows are whole lines (us, streamed /
-    // not, 768 -> 2048, 128 groups, 32768 rows: bf16 162 / 184, float32 205 / 269; parts of lines are not joined on that way: 712 ->
-    // 1096, 13 groups, 1003 rows, float32 28 / 23).
+    // not, 768 -> 2048, 128 groups, 32768 rows: bf16 171 / 207, float32 210 / 275; parts of lines are not joined on that way: 712 ->
+    // 1096, 13 groups, 1003 rows, float32 28 / 23 when it was tried).
     const bool stream = KIND == kGroupedDw && g.cols * size % 128u == 0u && !(F32 && g.splits > 1u);
     uint32_t own = lane;
     asm volatile("" : "+v"(own));  // (offsets are made anew for every tile: kept over the products they would be spilled)
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
   };
 
   // The dW of a group without rows is one stretch of zeros (whole lines: K and N are multiples of 8), a tile's share of it as many bytes as a
-  // tile holds: the same stores, but line after line.
+  // tile holds: the same stores, but line after line (1616 -> 10504, 56 of 78 groups empty, 756 us -> 540).
   auto clear = [&](const BgTile& d) {
     constexpr uint32_t size = F32 ? 4u : 2u;
     const uint64_t all = (uint64_t)g.rows * g.cols * size, from = (uint64_t)d.number * (TM * TN * size);

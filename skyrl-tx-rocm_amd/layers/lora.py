@@ -4,7 +4,7 @@ Mirrors the call surface of ``skyrl/tx/layers/lora.py``: ``LoRALinear.__call__(x
 adapter_indices=None)`` (:226-268), ``FusedLoRALinear.__call__ -> tuple`` with
 ``fuse``/``split`` (:271-351), ``LoRAExpert.__call__(x, group_sizes,
 adapter_indices_sorted=None, *, group_offset=None)`` (:354-444) and
-``init_lora_adapter`` (:447-501).  ``LoRAEmbed`` and a ``LoRAExpert`` with ``load_dense`` hold bf16 weights and run on
+``init_lora_adapter`` (:447-501).  ``LoRAEmbed`` and a ``LoRAExpert`` with ``load_unquantized`` hold bf16 weights and run on
 the ragged bf16 products and the embedding lookup; ``clip_adapter_gradients`` closes a training step over the
 adapters of any of them.  The frozen kernel is a ``GroupQuantizedWeight`` with one
 group over K (int8 codes, one float32 scale per output channel) instead of a dense matrix;
@@ -194,12 +194,12 @@ class LoRAEmbed(LoRAMixin):
         self.device = torch.device(device)
         self.embedding = None
         if embedding is not None:
-            self.load_dense(embedding)
+            self.load_unquantized(embedding)
         self.init_lora(max_lora_adapters=max_lora_adapters, max_lora_rank=max_lora_rank,
                        shape_A=(max_lora_adapters, num_embeddings, max_lora_rank),
                        shape_B=(max_lora_adapters, max_lora_rank, features), device=self.device)
 
-    def load_dense(self, table: torch.Tensor) -> None:
+    def load_unquantized(self, table: torch.Tensor) -> None:
         """A [num_embeddings, features] table, kept as bf16."""
         if tuple(table.shape) != (self.num_embeddings, self.features):
             raise ValueError(f"table must be {(self.num_embeddings, self.features)}, got {tuple(table.shape)}")
@@ -207,7 +207,7 @@ class LoRAEmbed(LoRAMixin):
 
     def __call__(self, ids: torch.Tensor, adapter_indices: torch.Tensor | None = None) -> torch.Tensor:
         if self.embedding is None:
-            raise RuntimeError("the table is not loaded: call load_dense()")
+            raise RuntimeError("the table is not loaded: call load_unquantized()")
         out = emb.embed(self.embedding, ids)
         if not self._lora_active(adapter_indices):
             return out
@@ -235,7 +235,7 @@ class LoRAExpert(LoRAMixin):
     pairs are indexed ``expert * max_lora_adapters + adapter`` (lora.py:414-431): rows are
     stably re-sorted by that combined index, run through the grouped kernel with
     ``max_lora_adapters`` LoRA groups per expert weight, and put back.  Differentiable: the backward
-    is one native grouped call for all experts and adapters.  With ``load_dense`` the kernels stay bf16 (and
+    is one native grouped call for all experts and adapters.  With ``load_unquantized`` the kernels stay bf16 (and
     differentiable): the base and the two low-rank factors are ragged bf16 products.
     """
 
@@ -245,7 +245,7 @@ class LoRAExpert(LoRAMixin):
         self.num_experts, self.in_features, self.out_features = int(num_experts), int(in_features), int(out_features)
         self.device = torch.device(device)
         self.weight = weight
-        self.dense = None
+        self.unquantized = None
         self.init_lora(max_lora_adapters=max_lora_adapters, max_lora_rank=max_lora_rank,
                        shape_A=(max_lora_adapters, num_experts, in_features, max_lora_rank),
                        shape_B=(max_lora_adapters, num_experts, max_lora_rank, out_features), device=self.device)
@@ -255,25 +255,25 @@ class LoRAExpert(LoRAMixin):
         if tuple(codes.shape) != (self.num_experts, self.in_features, self.out_features):
             raise ValueError(f"codes must be {(self.num_experts, self.in_features, self.out_features)}")
         self.weight = w8.prepare_grouped_weight(codes.to(self.device), scales.to(self.device))
-        self.dense = None
+        self.unquantized = None
 
-    def load_dense(self, kernels: torch.Tensor) -> None:
+    def load_unquantized(self, kernels: torch.Tensor) -> None:
         """[E, in, out] kernels, kept as bf16 instead of codes."""
         if tuple(kernels.shape) != (self.num_experts, self.in_features, self.out_features):
             raise ValueError(f"kernels must be {(self.num_experts, self.in_features, self.out_features)}, got {tuple(kernels.shape)}")
-        self.dense = kernels.to(device=self.device, dtype=torch.bfloat16).contiguous()
+        self.unquantized = kernels.to(device=self.device, dtype=torch.bfloat16).contiguous()
         self.weight = None
 
     def __call__(self, x: torch.Tensor, group_sizes: torch.Tensor, adapter_indices_sorted: torch.Tensor | None = None,
                  *, group_offset: torch.Tensor | None = None) -> torch.Tensor:
-        if self.weight is None and self.dense is None:
-            raise RuntimeError("the expert kernels are not loaded: call load_quantized() or load_dense()")
+        if self.weight is None and self.unquantized is None:
+            raise RuntimeError("the expert kernels are not loaded: call load_quantized() or load_unquantized()")
         if group_offset is not None and int(torch.as_tensor(group_offset).reshape(-1)[0]) != 0:
             raise NotImplementedError("expert shards (group_offset != 0) belong to the multi-GPU dispatch, "
                                       "which this one-GPU build leaves out")
         if not self._lora_active(adapter_indices_sorted):
-            if self.dense is not None:
-                return bf16_grouped_linear(x, self.dense, group_sizes)
+            if self.unquantized is not None:
+                return bf16_grouped_linear(x, self.unquantized, group_sizes)
             return w8.grouped_lora_linear(x, group_sizes, self.weight)
         n_ad, n_exp = self.max_lora_adapters, self.num_experts
         gs = group_sizes.to(device=x.device, dtype=torch.int64)
@@ -293,11 +293,11 @@ class LoRAExpert(LoRAMixin):
         a = self.lora_A.transpose(0, 1).reshape(n_exp * n_ad, self.in_features, self.max_lora_rank)
         b = self.lora_B.transpose(0, 1).reshape(n_exp * n_ad, self.max_lora_rank, self.out_features)
         scaling = self.lora_scaling.repeat(n_exp)
-        if self.dense is not None:
+        if self.unquantized is not None:
             z = bf16_grouped_linear(x[order], _whole_units(a, 2), sizes)
             factor = scaling[combined[order].clamp(max=n_exp * n_ad - 1)]
             delta = bf16_grouped_linear((z.float() * factor[:, None]).to(torch.bfloat16), _whole_units(b, 1), sizes)
-            return bf16_grouped_linear(x, self.dense, group_sizes) + torch.zeros_like(delta).index_copy(0, order, delta)
+            return bf16_grouped_linear(x, self.unquantized, group_sizes) + torch.zeros_like(delta).index_copy(0, order, delta)
         out_sorted = w8.grouped_lora_linear(x[order], sizes, self.weight, a.contiguous(), b.contiguous(), scaling,
                                             groups_per_weight=n_ad)
         return torch.zeros_like(out_sorted).index_copy(0, order, out_sorted)

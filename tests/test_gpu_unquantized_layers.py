@@ -73,17 +73,17 @@ def test_dense_experts(lora, n_exp, n_ad, k, n, rank, sizes):
     print(f"[case] {n_exp} experts, {n_ad} adapters, {k} -> {n}", flush=True)
     g = torch.Generator(device=DEV).manual_seed(4)
     layer = lora.LoRAExpert(n_exp, k, n, max_lora_adapters=n_ad, max_lora_rank=rank)
-    layer.load_dense(torch.randn(n_exp, k, n, generator=g, device=DEV) * k ** -0.5)
+    layer.load_unquantized(torch.randn(n_exp, k, n, generator=g, device=DEV) * k ** -0.5)
     fill(layer, g)
     rows = sum(sizes) + 2  # (two rows of no expert)
     x = torch.randn(rows, k, generator=g, device=DEV).to(BF16).requires_grad_()
     st = torch.tensor(sizes, dtype=torch.int32, device=DEV)
     index = torch.randint(0, n_ad, (rows,), generator=g, device=DEV)
-    layer.dense.requires_grad_()
+    layer.unquantized.requires_grad_()
     plain, out = layer(x, st), layer(x, st, index)
     expert = torch.repeat_interleave(torch.arange(n_exp, device=DEV), st.long())
     held = expert.numel()
-    xd, w = x.detach().double()[:held], layer.dense.detach().double()[expert]
+    xd, w = x.detach().double()[:held], layer.unquantized.detach().double()[expert]
     a, b = layer.lora_A.detach().double()[index[:held], expert], layer.lora_B.detach().double()[index[:held], expert]
     s = layer.lora_scaling.double()[index[:held]][:, None]
     mul = lambda v, m: torch.matmul(v[:, None], m)[:, 0]
@@ -105,7 +105,7 @@ def test_dense_experts(lora, n_exp, n_ad, k, n, rank, sizes):
     pairs = n_ad * n_exp
     assert off_by(layer.lora_A.grad.reshape(pairs, k, rank), sum_of(outer(xd, dz), pairs, spot), sum_of(outer(xd.abs(), dz_m), pairs, spot), 3) <= 0
     assert off_by(layer.lora_B.grad.reshape(pairs, rank, n), sum_of(outer(z, d), pairs, spot), sum_of(outer(z_m, d.abs()), pairs, spot), 3) <= 0
-    assert off_by(layer.dense.grad, sum_of(outer(xd, d), n_exp, expert), sum_of(outer(xd.abs(), d.abs()), n_exp, expert), 1) <= 0
+    assert off_by(layer.unquantized.grad, sum_of(outer(xd, d), n_exp, expert), sum_of(outer(xd.abs(), d.abs()), n_exp, expert), 1) <= 0
 
 
 def test_a_training_step(lora):
@@ -116,7 +116,7 @@ def test_a_training_step(lora):
     n_ad, n_exp, top_k, hidden = 3, 8, 2, 64
     embed = lora.LoRAEmbed(500, hidden, embedding=torch.randn(500, hidden, generator=g, device=DEV), max_lora_adapters=n_ad, max_lora_rank=8)
     up = lora.LoRAExpert(n_exp, hidden, 96, max_lora_adapters=n_ad, max_lora_rank=8)
-    up.load_dense(torch.randn(n_exp, hidden, 96, generator=g, device=DEV) * 0.1)
+    up.load_unquantized(torch.randn(n_exp, hidden, 96, generator=g, device=DEV) * 0.1)
     for layer in (embed, up):
         fill(layer, g)
     ids = torch.randint(0, 500, (6, 13), generator=g, device=DEV)
@@ -150,17 +150,17 @@ def test_a_training_step(lora):
 
 def test_refusals(lora):
     layer = lora.LoRAEmbed(10, 16, max_lora_adapters=2)
-    with pytest.raises(RuntimeError, match="load_dense"):
+    with pytest.raises(RuntimeError, match="load_unquantized"):
         layer(torch.zeros(2, dtype=torch.int64, device=DEV))
     with pytest.raises(ValueError, match="table"):
-        layer.load_dense(torch.zeros(10, 8, device=DEV))
-    layer.load_dense(torch.zeros(10, 16, device=DEV))
+        layer.load_unquantized(torch.zeros(10, 8, device=DEV))
+    layer.load_unquantized(torch.zeros(10, 16, device=DEV))
     with pytest.raises(ValueError, match="one entry per example"):
         layer(torch.zeros(2, 3, dtype=torch.int64, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV))
     with pytest.raises(ValueError, match="no|none"):
         lora.clip_adapter_gradients([layer], 1.0)
     with pytest.raises(ValueError, match="kernels"):
-        lora.LoRAExpert(2, 8, 8).load_dense(torch.zeros(2, 8, 16, device=DEV))
+        lora.LoRAExpert(2, 8, 8).load_unquantized(torch.zeros(2, 8, 16, device=DEV))
     for bad in (torch.zeros((), dtype=torch.int32, device=DEV), torch.zeros((2, 1), dtype=torch.int32, device=DEV)):
         with pytest.raises(ValueError, match="one entry per example"):
             layer(torch.zeros(2, dtype=torch.int64, device=DEV), bad)
@@ -186,7 +186,7 @@ def test_new_adapters_leave_the_layers_as_they_are(lora):
     g = torch.Generator(device=DEV).manual_seed(7)
     embed = lora.LoRAEmbed(90, 24, embedding=torch.randn(90, 24, generator=g, device=DEV), max_lora_adapters=2, max_lora_rank=8)
     experts = lora.LoRAExpert(4, 24, 32, max_lora_adapters=2, max_lora_rank=8)
-    experts.load_dense(torch.randn(4, 24, 32, generator=g, device=DEV))
+    experts.load_unquantized(torch.randn(4, 24, 32, generator=g, device=DEV))
     for layer, rank in ((embed, 6), (experts, 16)):
         lora.init_lora_adapter(layer, 1, rank=rank, alpha=16.0)
         kept = rank if layer is embed else rank // 4
