@@ -213,6 +213,8 @@ class LoRAEmbed(LoRAMixin):
             return out
         if ids.ndim == 0 or adapter_indices.ndim != 1 or adapter_indices.shape[0] != ids.shape[0]:
             raise ValueError("adapter_indices must hold one entry per example (leading axis of ids)")
+        if adapter_indices.dtype.is_floating_point or adapter_indices.dtype == torch.bool:
+            raise TypeError(f"adapter_indices must be integers, got {adapter_indices.dtype}")
         n_ad = self.max_lora_adapters
         flat = ids.reshape(-1)
         adapters = adapter_indices.clamp(-1, n_ad).to(device=flat.device, dtype=torch.int32).repeat_interleave(flat.numel() // adapter_indices.shape[0])

@@ -219,3 +219,59 @@ def test_same_bits_at_every_call(gl):
     for _ in range(3):
         again = gl.grouped_matmul(x, w, st), *gl.grouped_matmul_backward(x, dy, w, st, dw_dtype=torch.float32)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("k,n", [(4096, 8), (8, 4096)])
+def test_rows_beyond_32_bits(gl, k, n):
+    """The last of 600000 rows lie 4.9 GB behind the first; small whole numbers, whose sums are exact."""
+    rows, sizes = 600000, [1, 299999, 0, 299000]
+    print(f"[case] {rows} rows, {k} -> {n}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(7)
+    whole = lambda *s: torch.randint(-2, 3, s, generator=g, device=DEV, dtype=torch.int8).to(torch.bfloat16)
+    x, dy, w, st = whole(rows, k), whole(rows, n), whole(4, k, n), torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    out = gl.grouped_matmul(x, w, st)
+    dx, _ = gl.grouped_matmul_backward(x, dy, w, st, need_dw=False)
+    for r, e in ((slice(0, 1), 0), (slice(299990, 300000), 1), (slice(300000, 300010), 3), (slice(598990, 599000), 3)):
+        assert torch.equal(out[r].double(), (x[r].double() @ w[e].double()).to(torch.bfloat16).double())
+        assert torch.equal(dx[r].double(), (dy[r].double() @ w[e].double().T).to(torch.bfloat16).double())
+    assert not out[599000:].any() and not dx[599000:].any()
+    _, dw = gl.grouped_matmul_backward(x, dy, w, st, need_dx=False, dw_dtype=torch.float32)  # (at most 1.2 million: exact)
+    assert torch.equal(dw[3], x[300000:599000].float().T @ dy[300000:599000].float()) and not dw[2].any()
+
+
+def test_weights_beyond_32_bits(gl):
+    """The last of 70 groups lie 4.6 GB behind the first."""
+    groups, k, n, rows = 70, 4096, 8192, 140
+    print(f"[case] {groups} groups, {k} -> {n}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    x, dy = (torch.randn(rows, c, generator=g, device=DEV).to(torch.bfloat16) for c in (k, n))
+    w = torch.empty(groups, k, n, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    sizes = torch.full((groups,), 2, dtype=torch.int32, device=DEV)
+    sizes[40], sizes[69] = 0, 4
+    out = gl.grouped_matmul(x, w, sizes)
+    dx, dw = gl.grouped_matmul_backward(x, dy, w, sizes)
+    for e, r in ((0, slice(0, 2)), (66, slice(130, 132)), (69, slice(136, 140))):
+        xd, dd, wd = x[r].double(), dy[r].double(), w[e].double()
+        close(out[r], xd @ wd, xd.abs() @ wd.abs(), k)
+        close(dx[r], dd @ wd.T, dd.abs() @ wd.abs().T, n)
+        close(dw[e], xd.T @ dd, xd.abs().T @ dd.abs(), 4)
+    assert not dw[40].any()
+
+
+def test_the_most_groups_and_rows(gl):
+    sizes = torch.full((1024,), 1023, dtype=torch.int32, device=DEV)
+    sizes[1000] = 0
+    rows = 1 << 20
+    x, dy = (torch.randint(-1, 2, (rows, 8), device=DEV, dtype=torch.int8).to(torch.bfloat16) for _ in range(2))
+    w = torch.randint(-1, 2, (1024, 8, 8), device=DEV, dtype=torch.int8).to(torch.bfloat16)
+    group = torch.repeat_interleave(torch.arange(1024, device=DEV), sizes.long())
+    held = group.numel()
+    want = (x[:held, :, None].float() * w[group].float()).sum(1)
+    out = gl.grouped_matmul(x, w, sizes)
+    assert torch.equal(out[:held].float(), want) and not out[held:].any()
+    dx, dw = gl.grouped_matmul_backward(x, dy, w, sizes, dw_dtype=torch.float32)
+    assert torch.equal(dx[:held].float(), (dy[:held, None, :].float() * w[group].float()).sum(2)) and not dx[held:].any()
+    outer = torch.zeros(1024, 8, 8, device=DEV).index_add_(0, group, x[:held, :, None].float() * dy[:held, None, :].float())  # (whole numbers: exact)
+    assert torch.equal(dw, outer)
+    with pytest.raises(ValueError, match="at most"):
+        gl.grouped_matmul(torch.zeros(rows + 1, 8, dtype=torch.bfloat16, device=DEV), w, sizes)

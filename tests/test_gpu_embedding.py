@@ -205,3 +205,30 @@ def test_graph_replays(em, n):
         eager = em.lookup_backward(dy, ids, (3000, 32))
         torch.cuda.synchronize()
         assert torch.equal(grad, eager) and torch.equal(rows, em.lookup(eager, ids, 0.5))
+
+
+def test_the_most_tokens(em):
+    """2^20 tokens; the last rows of the output lie 4.3 GB behind the first."""
+    n, vocab = 1 << 20, 5000
+    g = gen(9)
+    table = torch.randn(vocab, 2056, generator=g, device=DEV).to(BF16)
+    ids = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    out = em.lookup(table, ids)
+    for r in (slice(0, 10), slice(n // 2, n // 2 + 10), slice(n - 10, n)):
+        assert torch.equal(out[r], table[ids[r]])
+    del out
+    dy = torch.randint(-3, 4, (n, 9), generator=g, device=DEV).float()
+    want = torch.zeros(vocab, 9, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())
+    assert torch.equal(em.lookup_backward(dy, ids, (vocab, 9)), want.float())
+    with pytest.raises(ValueError, match="at most"):
+        em.lookup(table, torch.zeros(n + 1, dtype=torch.int64, device=DEV))
+
+
+def test_the_widest_rows(em):
+    g = gen(10)
+    ids = torch.tensor([3, 0, 3, 2, 3], device=DEV)
+    for width in (65536, 65535):
+        dy = torch.randint(-3, 4, (5, width), generator=g, device=DEV).to(BF16)
+        want = torch.zeros(5, width, device=DEV).index_add_(0, ids, dy.float())
+        grad = em.lookup_backward(dy, ids, (5, width))
+        assert torch.equal(grad.float(), want) and torch.equal(em.lookup(grad, ids).float(), want[ids])

@@ -141,3 +141,30 @@ def test_a_gradient_given_twice(gc):
     (one, two), norm = gc.clip_grad_norm([grad, grad], 4.0)
     assert float(norm) == 8.0 and torch.equal(one, two) and one.data_ptr() != two.data_ptr() and float(one[0, 0]) == 0.5
     assert float(gc.grad_norm([grad, grad])) == 8.0
+
+
+def test_a_tensor_beyond_32_bits(gc):
+    """2^31 + 8 ones: the norm's square is exact in float64, the scaled values are powers of two."""
+    n = (1 << 31) + 8
+    grad = torch.ones(n, dtype=torch.bfloat16, device=DEV)
+    grad[-8:] = 0
+    norm = gc.clip_grad_norm_([grad], (2.0 ** 31) ** 0.5 / 4)
+    assert abs(float(norm) - (2.0 ** 31) ** 0.5) <= (2.0 ** 31) ** 0.5 * 2.0 ** -24
+    assert torch.equal(grad[:1000], torch.full((1000,), 0.25, dtype=torch.bfloat16, device=DEV))
+    assert torch.equal(grad[-1008:-8], torch.full((1000,), 0.25, dtype=torch.bfloat16, device=DEV)) and not grad[-8:].any()
+
+
+def test_two_plans_at_once(gc):
+    g = torch.Generator(device=DEV).manual_seed(11)
+    sets = [[torch.randn(2, c, generator=g, device=DEV) for c in (100000, 77, 300001)] for _ in range(2)]
+    want = [gc.clip_grad_norm(s, 1.0, per_adapter=True) for s in sets]
+    plans = [gc.GradClipPlan(s, 1.0, per_adapter=True) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        for plan, stream in zip(plans, streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                plan.run()
+    torch.cuda.synchronize()
+    for plan, (out, norms) in zip(plans, want):
+        assert torch.equal(plan.norms, norms) and all(torch.equal(a, b) for a, b in zip(plan.out, out))

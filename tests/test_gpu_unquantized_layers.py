@@ -161,6 +161,8 @@ def test_refusals(lora):
         lora.clip_adapter_gradients([layer], 1.0)
     with pytest.raises(ValueError, match="kernels"):
         lora.LoRAExpert(2, 8, 8).load_unquantized(torch.zeros(2, 8, 16, device=DEV))
+    with pytest.raises(TypeError, match="integers"):
+        layer(torch.zeros(2, dtype=torch.int64, device=DEV), torch.zeros(2, device=DEV))
     for bad in (torch.zeros((), dtype=torch.int32, device=DEV), torch.zeros((2, 1), dtype=torch.int32, device=DEV)):
         with pytest.raises(ValueError, match="one entry per example"):
             layer(torch.zeros(2, dtype=torch.int64, device=DEV), bad)
