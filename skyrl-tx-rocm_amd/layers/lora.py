@@ -179,6 +179,20 @@ def _whole_units(t: torch.Tensor, dim: int) -> torch.Tensor:
     return torch.cat([t, t.new_zeros(shape)], dim)
 
 
+class _Reorder(torch.autograd.Function):
+    """Rows in another order: ``t[order]``; ``back`` is the inverse permutation, so that the gradient is a gather too."""
+
+    @staticmethod
+    def forward(ctx, t, order, back):
+        ctx.save_for_backward(order, back)
+        return t.index_select(0, order)
+
+    @staticmethod
+    def backward(ctx, d):
+        order, back = ctx.saved_tensors
+        return _Reorder.apply(d, back, order), None, None
+
+
 class LoRAEmbed(LoRAMixin):
     """Embedding table with multi-adapter LoRA: ``table[id] + s[a] * A[a, id] @ B[a]``.
 
@@ -218,15 +232,15 @@ class LoRAEmbed(LoRAMixin):
         n_ad = self.max_lora_adapters
         flat = ids.reshape(-1)
         adapters = adapter_indices.clamp(-1, n_ad).to(device=flat.device, dtype=torch.int32).repeat_interleave(flat.numel() // adapter_indices.shape[0])
-        order = None
+        order = back = None
         sizes = torch.full((1,), flat.numel(), dtype=torch.int32, device=flat.device)
         if n_ad > 1:
-            _, sizes, order, _, _ = w8.moe_dispatch(None, adapters, n_ad)
-            flat, adapters = flat[order], adapters[order]
+            _, sizes, order, back, _ = w8.moe_dispatch(None, adapters, n_ad)
+            flat, adapters = flat.index_select(0, order), adapters.index_select(0, order)
         z = emb.embed(self.lora_A, flat, self.lora_scaling, adapter_indices=adapters)
         delta = bf16_grouped_linear(_whole_units(z, 1), _whole_units(self.lora_B, 1), sizes)
         if order is not None:
-            delta = torch.zeros_like(delta).index_copy(0, order.long(), delta)
+            delta = _Reorder.apply(delta, back, order)
         return out + delta.reshape(out.shape)
 
 
@@ -296,10 +310,11 @@ class LoRAExpert(LoRAMixin):
         b = self.lora_B.transpose(0, 1).reshape(n_exp * n_ad, self.max_lora_rank, self.out_features)
         scaling = self.lora_scaling.repeat(n_exp)
         if self.unquantized is not None:
-            z = bf16_grouped_linear(x[order], _whole_units(a, 2), sizes)
+            back = torch.empty_like(order).scatter_(0, order, rows)
+            z = bf16_grouped_linear(_Reorder.apply(x, order, back), _whole_units(a, 2), sizes)
             factor = scaling[combined[order].clamp(max=n_exp * n_ad - 1)]
             delta = bf16_grouped_linear((z.float() * factor[:, None]).to(torch.bfloat16), _whole_units(b, 1), sizes)
-            return bf16_grouped_linear(x, self.unquantized, group_sizes) + torch.zeros_like(delta).index_copy(0, order, delta)
+            return bf16_grouped_linear(x, self.unquantized, group_sizes) + _Reorder.apply(delta, back, order)
         out_sorted = w8.grouped_lora_linear(x[order], sizes, self.weight, a.contiguous(), b.contiguous(), scaling,
                                             groups_per_weight=n_ad)
         return torch.zeros_like(out_sorted).index_copy(0, order, out_sorted)
