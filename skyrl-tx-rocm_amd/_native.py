@@ -40,6 +40,7 @@ FLAG_BF16_GROUPED_TILE_256X256, FLAG_BF16_GROUPED_TILE_128X256, FLAG_BF16_GROUPE
 FLAG_EMBEDDING_F32 = 1        # mi355_w8a8_embedding_problem.flags
 FLAG_EMBEDDING_IDS64 = 2
 GRAD_BF16, GRAD_F32 = 0, 1    # mi355_w8a8_grad_tensor.type
+FLAG_GRAD_TABLE_KEPT = 1      # mi355_w8a8_grad_norm_v1, mi355_w8a8_grad_clip_v1
 STATIC_WORKSPACE_BYTES = 32 << 20
 PATH_NAMES = {1: "skinny", 2: "skinny-chunks", 3: "tiled-256x128", 4: "tiled-256x256", 5: "tiled-128x128",
               6: "tiled-256x128-pair"}
@@ -372,9 +373,9 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mi355_w8a8_grad_workspace_bytes.restype = _u64
     lib.mi355_w8a8_grad_workspace_bytes.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32)
     lib.mi355_w8a8_grad_norm_v1.restype = ctypes.c_int
-    lib.mi355_w8a8_grad_norm_v1.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32, _vp, _vp, _u64, _vp)
+    lib.mi355_w8a8_grad_norm_v1.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32, _vp, _vp, _u64, _u32, _vp)
     lib.mi355_w8a8_grad_clip_v1.restype = ctypes.c_int
-    lib.mi355_w8a8_grad_clip_v1.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32, _vp, _vp, _vp, _u64, _vp)
+    lib.mi355_w8a8_grad_clip_v1.argtypes = (ctypes.POINTER(GradTensor), _u32, _u32, _vp, _vp, _vp, _u64, _u32, _vp)
 
 
 def load() -> ctypes.CDLL:

@@ -95,10 +95,12 @@ int mi355_w8a8_embedding_bwd_v1(const mi355_w8a8_embedding_problem* problem, voi
  * clipping:
  *   norms[a] = sqrt(sum over the tensors of sum(grad[a]^2))        (double sums, the same bits at every call)
  *   out[a]   = grad[a] * (norms[a] > limits[a] ? limits[a] / norms[a] : 1)
- * out may be grad itself; other overlaps are refused.  Where a norm or a limit is NaN that adapter's gradients stay as they are, a
+ * A tensor's out may be its grad itself, other overlaps of the two are refused; different tensors must not overlap where one is written.  Where a norm or a limit is NaN that adapter's gradients stay as they are, a
  * negative limit counts as zero.  The tensor table is host memory and is read before the call returns; limits and norms are device
- * memory.
+ * memory.  More than 16 tensors are found by the kernels in a table that the call writes into the workspace;
+ * MI355_W8A8_FLAG_GRAD_TABLE_KEPT says that it is still there from an earlier call on the same workspace with the same tensors, in order.
  */
+#define MI355_W8A8_FLAG_GRAD_TABLE_KEPT 1u
 #define MI355_W8A8_GRAD_BF16 0u
 #define MI355_W8A8_GRAD_F32 1u
 #define MI355_W8A8_GRAD_MAX_TENSORS 65536u
@@ -111,8 +113,8 @@ typedef struct mi355_w8a8_grad_tensor {
 } mi355_w8a8_grad_tensor;
 uint64_t mi355_w8a8_grad_workspace_bytes(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters);
 int mi355_w8a8_grad_norm_v1(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters, float* norms,
-                            void* workspace, uint64_t workspace_bytes, void* stream);
+                            void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream);
 int mi355_w8a8_grad_clip_v1(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters, const float* limits,
-                            float* norms, void* workspace, uint64_t workspace_bytes, void* stream);
+                            float* norms, void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream);
 
 }  // extern "C"

@@ -435,51 +435,66 @@ int check_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, 
   return MI355_W8A8_OK;
 }
 
+// where the table of many tensors lies behind the parts
+inline uint64_t grad_parts_bytes(uint64_t pieces, uint32_t adapters) { return align256((pieces ? pieces : 1u) * adapters * 8u); }
+inline uint64_t grad_table_bytes(uint32_t n) { return n > kGradShortTable ? align256((uint64_t)n * (sizeof(GradTensor) + 4u)) : 0u; }
+
 template <uint32_t TABLE>
-int launch_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const float* limits, float* norms, void* workspace, hipStream_t s) {
+int launch_grads(GradArgs<TABLE>& a, uint32_t adapters, hipStream_t s) {
+  hipLaunchKernelGGL(grad_norm_kernel<TABLE>, dim3(a.pieces, adapters), dim3(256), 0, s, a);
+  const int st = launch_status();
+  if (st) return st;
+  hipLaunchKernelGGL(grad_scale_kernel<TABLE>, dim3(a.limits ? a.pieces : 1u, adapters), dim3(256), 0, s, a);
+  return launch_status();
+}
+
+// entry(i, the tensor with its first piece) for every tensor that holds values
+template <class Entry>
+void each_grad(const mi355_w8a8_grad_tensor* t, uint32_t n, GradCall& c, Entry entry) {
+  c.tensors = c.pieces = 0;
+  for (uint32_t i = 0; i < n; ++i) {
+    if (t[i].count == 0) continue;
+    entry(c.tensors++, GradTensor{t[i].grad, t[i].out, t[i].count, c.pieces, t[i].type == MI355_W8A8_GRAD_F32});
+    c.pieces += (uint32_t)pieces_of(t[i].count, c.piece);
+  }
+}
+template <uint32_t TABLE>
+int launch_grads_from_arguments(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const GradCall& call, hipStream_t s) {
   GradArgs<TABLE> a{};
-  a.parts = static_cast<double*>(workspace);
-  a.limits = limits;
-  a.norms = norms;
-  a.piece = grad_piece_values(t, n, adapters);
-  uint64_t total = 0;
-  for (uint32_t i = 0; i < n; ++i) total += pieces_of(t[i].count, a.piece);
-  a.parts_ld = a.parts_used = (uint32_t)total;
-  // The table's share of a launch each, first to last for the norm, last to first for the scaling.
-  auto fill = [&](uint32_t from) {  // -> the first tensor behind the launch
-    a.tensors = a.pieces = 0;
-    uint32_t i = from;
-    for (; i < n && a.tensors < TABLE; ++i) {
-      if (t[i].count == 0) continue;
-      a.tensor[a.tensors++] = GradTensor{t[i].grad, t[i].out, t[i].count, a.pieces, t[i].type == MI355_W8A8_GRAD_F32};
-      a.pieces += (uint32_t)pieces_of(t[i].count, a.piece);
+  static_cast<GradCall&>(a) = call;
+  each_grad(t, n, a, [&](uint32_t i, const GradTensor& g) { a.tensor[i] = g; });
+  return launch_grads(a, adapters, s);
+}
+int launch_grads_from_table(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const GradCall& call, void* table, bool kept, hipStream_t s) {
+  GradArgs<0> a{};
+  static_cast<GradCall&>(a) = call;
+  GradTableArgs w{};
+  w.table = static_cast<GradTensor*>(table);
+  w.first = reinterpret_cast<uint32_t*>(w.table + n);
+  a.tensor = w.table; a.first = w.first;
+  int st = MI355_W8A8_OK;
+  auto write = [&] {
+    if (w.tensors && !kept && !st) {
+      hipLaunchKernelGGL(grad_table_kernel, dim3(1), dim3(128), 0, s, w);
+      st = launch_status();
     }
-    return i;
+    w.table += w.tensors;
+    w.first += w.tensors;
+    w.tensors = 0;
   };
-  uint32_t first[MI355_W8A8_GRAD_MAX_TENSORS / TABLE + 1], parts[MI355_W8A8_GRAD_MAX_TENSORS / TABLE + 1], launches = 0;
-  int st;
-  for (uint32_t i = 0, part = 0; i < n; part += a.pieces) {
-    first[launches] = i;
-    parts[launches] = a.part0 = part;
-    i = fill(i);
-    if (a.pieces == 0) break;  // (none of the last tensors holds a value)
-    ++launches;
-    hipLaunchKernelGGL(grad_norm_kernel<TABLE>, dim3(a.pieces, adapters), dim3(256), 0, s, a);
-    if ((st = launch_status())) return st;
-  }
-  for (uint32_t l = limits ? launches : 1u; l-- > 0;) {
-    if (launches > 1u || a.pieces == 0) fill(first[l]);
-    a.part0 = parts[l];
-    hipLaunchKernelGGL(grad_scale_kernel<TABLE>, dim3(limits ? a.pieces : 1u, adapters), dim3(256), 0, s, a);
-    if ((st = launch_status())) return st;
-  }
-  return MI355_W8A8_OK;
+  each_grad(t, n, a, [&](uint32_t, const GradTensor& g) {
+    w.tensor[w.tensors++] = g;
+    if (w.tensors == kGradTable) write();
+  });
+  write();
+  return st ? st : launch_grads(a, adapters, s);
 }
 
 int run_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, const float* limits, float* norms, void* workspace, uint64_t workspace_bytes,
-              hipStream_t s, bool scale) {
+              uint32_t flags, hipStream_t s, bool scale) {
   const int st = check_grads(t, n, adapters, norms, scale);
   if (st) return st;
+  if (flags & ~MI355_W8A8_FLAG_GRAD_TABLE_KEPT) return MI355_W8A8_ERR_SHAPE;
   if (scale && !limits) return MI355_W8A8_ERR_NULL;
   if (!aligned(limits, 4)) return MI355_W8A8_ERR_ALIGN;
   const uint64_t need = mi355_w8a8_grad_workspace_bytes(t, n, adapters);
@@ -502,8 +517,14 @@ int run_grads(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters, co
     hipLaunchKernelGGL(grad_zero_norms_kernel, dim3((adapters + 255u) / 256u), dim3(256), 0, s, norms, adapters);
     return launch_status();
   }
-  if (n <= kGradShortTable) return launch_grads<kGradShortTable>(t, n, adapters, scale ? limits : nullptr, norms, workspace, s);
-  return launch_grads<kGradTable>(t, n, adapters, scale ? limits : nullptr, norms, workspace, s);
+  GradCall call{};
+  call.parts = static_cast<double*>(workspace);
+  call.limits = scale ? limits : nullptr;
+  call.norms = norms;
+  call.piece = grad_piece_values(t, n, adapters);
+  if (n <= kGradShortTable) return launch_grads_from_arguments<kGradShortTable>(t, n, adapters, call, s);
+  return launch_grads_from_table(t, n, adapters, call, static_cast<unsigned char*>(workspace) + need - grad_table_bytes(n),
+                                 flags & MI355_W8A8_FLAG_GRAD_TABLE_KEPT, s);
 }
 
 }  // namespace
@@ -542,15 +563,15 @@ uint64_t mi355_w8a8_grad_workspace_bytes(const mi355_w8a8_grad_tensor* tensors, 
   const uint32_t piece = grad_piece_values(tensors, n_tensors, n_adapters);
   uint64_t pieces = 0;
   for (uint32_t i = 0; i < n_tensors; ++i) pieces += pieces_of(tensors[i].count, piece);
-  return pieces > 0x7fffffffu ? 0u : align256((pieces ? pieces : 1u) * n_adapters * 8u);
+  return pieces > 0x7fffffffu ? 0u : grad_parts_bytes(pieces, n_adapters) + grad_table_bytes(n_tensors);
 }
 int mi355_w8a8_grad_norm_v1(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters, float* norms, void* workspace,
-                            uint64_t workspace_bytes, void* stream) {
-  return run_grads(tensors, n_tensors, n_adapters, nullptr, norms, workspace, workspace_bytes, static_cast<hipStream_t>(stream), false);
+                            uint64_t workspace_bytes, uint32_t flags, void* stream) {
+  return run_grads(tensors, n_tensors, n_adapters, nullptr, norms, workspace, workspace_bytes, flags, static_cast<hipStream_t>(stream), false);
 }
 int mi355_w8a8_grad_clip_v1(const mi355_w8a8_grad_tensor* tensors, uint32_t n_tensors, uint32_t n_adapters, const float* limits, float* norms,
-                            void* workspace, uint64_t workspace_bytes, void* stream) {
-  return run_grads(tensors, n_tensors, n_adapters, limits, norms, workspace, workspace_bytes, static_cast<hipStream_t>(stream), true);
+                            void* workspace, uint64_t workspace_bytes, uint32_t flags, void* stream) {
+  return run_grads(tensors, n_tensors, n_adapters, limits, norms, workspace, workspace_bytes, flags, static_cast<hipStream_t>(stream), true);
 }
 
 }  // extern "C"

@@ -11,32 +11,48 @@
 //   grad_norm_kernel   a workgroup per piece of one tensor's adapter: the sum of its squares
 //   grad_scale_kernel  a workgroup per piece: the parts of its adapter added up, then the piece scaled
 //
-// The tensors come in the kernels' arguments, kGradTable to a launch: no table in device memory that a captured graph could find
-// overwritten, no copy.
+// Up to kGradShortTable tensors come in the kernels' arguments.  More lie in a table in the workspace, written by launches whose arguments they
+// are (grad_table_kernel, 120 a launch) once for all calls on it: two launches for any number of tensors.  Norm and scaling of 204 tensors
+// of 2.6 MB in all 19.1 us as two launches each with the tensors as arguments, 9.5 so; 64 of 24 KB 8.6 and 7.2 us (4 KiB of arguments take
+// their time), where the table has to be written first 7.3 and 8.5.
 #pragma once
 #include "w8a8_device.h"
 
 namespace w8a8 {
 
-constexpr uint32_t kGradTable = 120, kGradShortTable = 16;  // (a call of few tensors does not hand over 4 KiB: eight tensors of 6.8 MB: 12.4 / 10.0 us)
+constexpr uint32_t kGradTable = 120, kGradShortTable = 16;
 
 struct GradTensor {
   const void* grad;
   void* out;
   uint64_t count;         // values of one adapter
-  uint32_t first_piece;   // among the launch's pieces of one adapter
+  uint32_t first_piece;   // among the pieces of one adapter
   uint32_t f32;
 };
-template <uint32_t TABLE>
-struct GradArgs {
-  GradTensor tensor[TABLE];
-  double* parts;          // [adapters][parts_ld]
+struct GradCall {
+  double* parts;          // [adapters][pieces]
   const float* limits;    // [adapters]
   float* norms;           // [adapters]
-  uint32_t tensors, pieces;        // of this launch, for one adapter
-  uint32_t part0, parts_ld, parts_used;  // first part of this launch; parts in all
+  uint32_t tensors, pieces;  // pieces of one adapter
   uint32_t piece;         // values of a piece
 };
+template <uint32_t TABLE> struct GradArgs : GradCall { GradTensor tensor[TABLE]; };
+template <> struct GradArgs<0> : GradCall {
+  const GradTensor* tensor;  // [tensors]
+  const uint32_t* first;     // [tensors] their first pieces
+};
+
+struct GradTableArgs {
+  GradTensor tensor[kGradTable];
+  GradTensor* table;
+  uint32_t* first;
+  uint32_t tensors;
+};
+__global__ __launch_bounds__(128) void grad_table_kernel(GradTableArgs a) {
+  if (threadIdx.x >= a.tensors) return;
+  a.table[threadIdx.x] = a.tensor[threadIdx.x];
+  a.first[threadIdx.x] = a.tensor[threadIdx.x].first_piece;
+}
 
 typedef uint32_t v4whole __attribute__((ext_vector_type(4)));
 typedef uint32_t v4unaligned __attribute__((ext_vector_type(4), aligned(2)));  // (out may lie at another offset from 16 than grad)
@@ -49,9 +65,18 @@ struct GradPiece { const GradTensor* t; uint64_t at; uint32_t count; };  // at: 
 template <uint32_t TABLE>
 __device__ inline GradPiece grad_piece(const GradArgs<TABLE>& a, uint32_t adapter, uint32_t piece) {
   uint32_t lo = 0, hi = a.tensors;  // the last tensor whose first piece is not behind this one
-  while (hi - lo > 1u) {
-    const uint32_t mid = (lo + hi) / 2u;
-    if (a.tensor[mid].first_piece <= piece) lo = mid; else hi = mid;
+  if constexpr (TABLE == 0) {  // 64 places at a time
+    while (hi - lo > 1u) {
+      const uint32_t step = (hi - lo + 63u) / 64u, mid = lo + (threadIdx.x & 63u) * step;
+      const uint32_t in = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(mid < hi && a.first[mid < hi ? mid : lo] <= piece));
+      lo = __builtin_amdgcn_readfirstlane(lo + (in - 1u) * step);
+      hi = lo + step < hi ? lo + step : hi;
+    }
+  } else {
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) / 2u;
+      if (a.tensor[mid].first_piece <= piece) lo = mid; else hi = mid;
+    }
   }
   GradPiece p;
   p.t = &a.tensor[lo];
@@ -133,7 +158,7 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(GradArgs<TABLE> a) {
   const uint32_t adapter = blockIdx.y, piece = blockIdx.x;
   const GradPiece p = grad_piece(a, adapter, piece);
   const double s = grad_block_sum(p.t->f32 ? grad_squares<float>(p) : grad_squares<uint16_t>(p));
-  if (threadIdx.x == 0) a.parts[(uint64_t)adapter * a.parts_ld + a.part0 + piece] = s;
+  if (threadIdx.x == 0) a.parts[(uint64_t)adapter * a.pieces + piece] = s;
 }
 
 template <typename T>
@@ -171,9 +196,9 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(GradArgs<TABLE> a) {
   // from the last piece to the first: what the norm read last is in the caches yet
   const uint32_t adapter = gridDim.y - 1u - blockIdx.y, piece = gridDim.x - 1u - blockIdx.x;
   double s = 0.0;
-  for (uint32_t i = threadIdx.x; i < a.parts_used; i += 256u) s += a.parts[(uint64_t)adapter * a.parts_ld + i];
+  for (uint32_t i = threadIdx.x; i < a.pieces; i += 256u) s += a.parts[(uint64_t)adapter * a.pieces + i];
   const double norm = sqrt(grad_block_sum(s));
-  if (piece == 0 && a.part0 == 0 && threadIdx.x == 0) a.norms[adapter] = (float)norm;
+  if (piece == 0 && threadIdx.x == 0) a.norms[adapter] = (float)norm;
   if (!a.limits) return;
   const float given = a.limits[adapter];
   const double limit = given < 0.0f ? 0.0 : (double)given;

@@ -3,7 +3,7 @@
 // from one call for the next.  The steps take 14 to 16 us in Python beside the 7 us of the entry point's two launches, 4 to 6 here, and a decode
 // call's kernels 11 to 17: 2560 -> 6144, one row, 4 adapters of rank 64 23.3 -> 12.4 us a call; 12288 -> 4096, 16 rows, 4-bit codes 25.2 -> 18.1.
 //
-// Every function returns the output tensor (grouped_bwd: a tuple of two), an int (the entry point's status, not OK), or None for anything out of the ordinary -- a wrong
+// Every function returns the output tensor (grouped_bwd: a tuple of two; grad_table: the table's bytes and the adapters), an int (the entry point's status, not OK), or None for anything out of the ordinary -- a wrong
 // dtype, shape or device, a tensor subclass or mode, a tensor that is not contiguous, one that requires a gradient, a geometry that
 // the library refuses -- and the caller then goes the general way, which converts, differentiates or raises.
 #define PY_SSIZE_T_CLEAN
@@ -16,6 +16,9 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <vector>
 
 #include "bf16_api.h"
 
@@ -399,6 +402,62 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   END_HANDLE_TH_ERRORS
 }
 
+// A tensor of a gradient table: its values lie behind each other.
+bool whole_gradient(const at::Tensor& t, c10::Device device) {
+  return t.layout() == at::kStrided && !t.is_nested() && t.device() == device && t.is_contiguous() && t.unsafeGetTensorImpl()->has_storage() &&
+         !at::isTensorSubclassLike(t) && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat);
+}
+
+// grad_table(grads, outs, per_adapter), lists of tensors (outs: or None) -> (bytes of the C table, adapters), or None where something is not
+// ordinary: an output that overlaps anything but its own gradient, whose place it may have, is not.
+PyObject* grad_table(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  if (argc != 3) { PyErr_SetString(PyExc_TypeError, "grad_table takes 3 arguments"); return nullptr; }
+  HANDLE_TH_ERRORS
+  if (!PyList_CheckExact(argv[0]) || (argv[1] != Py_None && !PyList_CheckExact(argv[1])) || c10::impl::TorchDispatchModeTLS::any_modes_set()) Py_RETURN_NONE;
+  const Py_ssize_t n = PyList_GET_SIZE(argv[0]);
+  const bool written = argv[1] != Py_None, per_adapter = argv[2] == Py_True;
+  if (n < 1 || n > (Py_ssize_t)MI355_W8A8_GRAD_MAX_TENSORS || (written && PyList_GET_SIZE(argv[1]) != n)) Py_RETURN_NONE;
+  struct Span { uintptr_t from, to; Py_ssize_t of; };
+  std::vector<Span> outs;
+  std::vector<mi355_w8a8_grad_tensor> table((size_t)n);
+  int64_t adapters = 1;
+  c10::Device device(c10::DeviceType::CPU);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* const item = PyList_GET_ITEM(argv[0], i);
+    if (!THPVariable_Check(item)) Py_RETURN_NONE;
+    const at::Tensor& g = THPVariable_Unpack(item);
+    if (i == 0) {
+      device = g.device();
+      if (!device.is_cuda()) Py_RETURN_NONE;
+      if (per_adapter) adapters = g.dim() ? g.size(0) : 0;
+      if (adapters < 1 || adapters > 65535) Py_RETURN_NONE;
+    }
+    if (!whole_gradient(g, device) || (per_adapter && (g.dim() == 0 || g.size(0) != adapters))) Py_RETURN_NONE;
+    mi355_w8a8_grad_tensor& t = table[(size_t)i];
+    t = mi355_w8a8_grad_tensor{g.const_data_ptr(), nullptr, (uint64_t)(g.numel() / adapters),
+                               g.scalar_type() == at::kFloat ? MI355_W8A8_GRAD_F32 : MI355_W8A8_GRAD_BF16, 0u};
+    if (!written) continue;
+    PyObject* const target = PyList_GET_ITEM(argv[1], i);
+    if (!THPVariable_Check(target)) Py_RETURN_NONE;
+    const at::Tensor& o = THPVariable_Unpack(target);
+    if (!whole_gradient(o, device) || o.scalar_type() != g.scalar_type() || o.sizes() != g.sizes()) Py_RETURN_NONE;
+    t.out = const_cast<void*>(o.const_data_ptr());
+    const uintptr_t from = reinterpret_cast<uintptr_t>(t.out);
+    if (o.numel()) outs.push_back({from, from + (uintptr_t)o.nbytes(), i});
+  }
+  std::sort(outs.begin(), outs.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  for (size_t i = 1; i < outs.size(); ++i)
+    if (outs[i].from < outs[i - 1].to) Py_RETURN_NONE;
+  for (const Span& own : outs) {  // every gradient with values has an output of the same size
+    const uintptr_t from = reinterpret_cast<uintptr_t>(table[(size_t)own.of].grad), to = from + (own.to - own.from);
+    if (from == own.from) continue;
+    auto behind = std::lower_bound(outs.begin(), outs.end(), to, [](const Span& a, uintptr_t end) { return a.from < end; });
+    if (behind != outs.begin() && (behind - 1)->to > from) Py_RETURN_NONE;
+  }
+  return Py_BuildValue("(y#L)", reinterpret_cast<const char*>(table.data()), (Py_ssize_t)(table.size() * sizeof(mi355_w8a8_grad_tensor)), (long long)adapters);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"dense", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dense)), METH_FASTCALL, "One forward call of the per-channel linear."},
     {"group_scaled", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_scaled)), METH_FASTCALL,
@@ -407,6 +466,7 @@ PyMethodDef methods[] = {
     {"grouped_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grouped_bwd)), METH_FASTCALL, "Their two gradients."},
     {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding)), METH_FASTCALL, "One lookup of embedding rows."},
     {"embedding_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding_bwd)), METH_FASTCALL, "The table's gradient."},
+    {"grad_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_table)), METH_FASTCALL, "The C table of gradients and their outputs."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mi355_w8a8_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -168,3 +168,76 @@ def test_two_plans_at_once(gc):
     torch.cuda.synchronize()
     for plan, (out, norms) in zip(plans, want):
         assert torch.equal(plan.norms, norms) and all(torch.equal(a, b) for a, b in zip(plan.out, out))
+
+
+@pytest.mark.parametrize("n", [120, 121, 240, 1000, 4500])
+def test_many_tensors(gc, n):
+    """More tensors than a launch's arguments hold, empty ones among them, from plans that run again, in a captured graph too."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    sizes = [(7 * i) % 61 if i % 9 else 0 for i in range(n)]
+    sizes[n // 2] = 70001
+    grads = [torch.randn(2, s, generator=g, device=DEV).to(torch.bfloat16 if i % 3 else torch.float32) for i, s in enumerate(sizes)]
+    limits = torch.tensor([3.0, 1e6], device=DEV)
+
+    def check(out, norms):
+        want = torch.stack([t.double().square().sum(1) for t in grads]).sum(0).sqrt()
+        assert bool(((norms.double() - want).abs() <= 2.0 ** -23 * want).all())
+        for t, o in zip(grads, out):
+            scaled = t[0].double() * (3.0 / want[0])
+            step = 2.0 ** -8 if t.dtype == torch.bfloat16 else 2.0 ** -24
+            assert bool(((o[0].double() - scaled).abs() <= (step + 2.0 ** -22) * scaled.abs() + 1e-40).all()) and torch.equal(o[1], t[1])
+
+    check(*gc.clip_grad_norm(grads, limits, per_adapter=True))
+    captured, eager = (gc.GradClipPlan(grads, limits, per_adapter=True) for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # (a plan whose first run is captured)
+        captured.run()
+    for turn in range(3):
+        for t in grads:
+            t.copy_(torch.randn(t.shape, generator=g, device=DEV))
+        check(*eager.run())
+        graph.replay()
+        check(captured.out, captured.norms)
+        if turn == 1:
+            check(*captured.run())
+    again = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(again):  # (and one that has run before)
+        eager.run()
+    for t in grads:
+        t.mul_(0.5)
+    again.replay()
+    check(eager.out, eager.norms)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_tables_of_the_host_module_and_of_python(gc, monkeypatch, native):
+    """What both ways of making a table take and refuse, and that they give the same bits."""
+    want, norms = gc.clip_grad_norm([torch.arange(12, device=DEV).float().view(2, 6), torch.ones(2, 3, device=DEV).to(torch.bfloat16)], 2.0, per_adapter=True)
+    if not native:
+        monkeypatch.setattr(load_package()._native, "host", lambda: None)
+    grads = [torch.nn.Parameter(torch.arange(12, device=DEV).float().view(2, 6)), torch.ones(2, 3, device=DEV).to(torch.bfloat16), torch.empty(2, 0, device=DEV)]
+    bucket = torch.empty(12 * 4 + 6 * 2, dtype=torch.uint8, device=DEV)
+    outs = [bucket[:48].view(torch.float32).view(2, 6), bucket[48:].view(torch.bfloat16).view(2, 3), torch.empty(2, 0, device=DEV)]
+    out, got = gc.GradClipPlan(grads, 2.0, per_adapter=True, out=outs).run()
+    assert torch.equal(got, norms) and all(torch.equal(a, b) for a, b in zip(out, want))
+    f = torch.zeros(40, device=DEV)
+    plan = lambda g, o, per=False: gc.GradClipPlan(g, 1.0, per_adapter=per, out=o)
+    plan([f[:10], f[10:20]], [f[:10], f[10:20]])        # in place
+    plan([f[:10], f[:10]], [f[20:30], f[30:]])          # one gradient read twice
+    plan([f[:10], f[5:15]], [f[20:30], f[30:]])
+    for g, o in (([f[:10], f[5:15]], [f[:10], f[20:30]]), ([f[:10], f[10:20]], [f[10:20], f[20:30]]), ([f[:10], f[20:30]], [f[30:], f[25:35]]),
+                 ([f[:20]], [f[10:30]]), ([f[10:30]], [f[:20]]), ([f[5:6], f[:10]], [f[20:21], f[:10]]), ([f[:10], f[5:6]], [f[:10], f[20:21]])):
+        with pytest.raises(ValueError, match="overlap"):
+            plan(g, o)
+    for g, o, message in (([f[:10]], [f[20:31]], "out must be"), ([f[:10]], [f[20:30].to(torch.bfloat16)], "out must be"), ([f[:10]], [], "names 0"),
+                          ([f[::2]], None, "contiguous"), ([f[:10]], [f[20:40:2]], "out must be")):
+        with pytest.raises(ValueError, match=message):
+            plan(g, o)
+    with pytest.raises(ValueError, match="leading axis"):
+        plan([torch.zeros(2, 3, device=DEV), torch.zeros(3, 2, device=DEV)], None, True)
+    with pytest.raises(ValueError, match="1 to 65535"):
+        plan([torch.zeros(0, 3, device=DEV)], None, True)
+    with pytest.raises(TypeError, match="BF16"):
+        plan([f, f.double()], None)
+    with pytest.raises(RuntimeError, match="GPU"):
+        plan([f, f.cpu()], None)

@@ -94,13 +94,14 @@ def test_embedding_calls(native, change, status):
 def test_gradient_calls(native):
     lib = native.load()
 
-    def clip(tensors, adapters=2, limits=A, norms=A + 64, ws=A + 5 * STEP, ws_bytes=1 << 20, n=None):
+    def clip(tensors, adapters=2, limits=A, norms=A + 64, ws=A + 5 * STEP, ws_bytes=1 << 20, n=None, flags=0):
         table = (native.GradTensor * max(1, len(tensors)))(*[native.GradTensor(*t) for t in tensors])
-        return lib.mi355_w8a8_grad_clip_v1(table, len(tensors) if n is None else n, adapters, limits, norms, ws, ws_bytes, None)
+        return lib.mi355_w8a8_grad_clip_v1(table, len(tensors) if n is None else n, adapters, limits, norms, ws, ws_bytes, flags, None)
 
     good = (A + STEP, A + 2 * STEP, 100, 0, 0)
-    assert lib.mi355_w8a8_grad_clip_v1(None, 1, 1, A, A, A, 1, None) == -1
+    assert lib.mi355_w8a8_grad_clip_v1(None, 1, 1, A, A, A, 1, 0, None) == -1
     assert clip([]) == -2 and clip([good], adapters=0) == -2 and clip([good], adapters=65536) == -7
+    assert clip([good], flags=2) == -2
     assert clip([good], limits=None) == -1 and clip([good], norms=None) == -1
     assert clip([(None, A, 100, 0, 0)]) == -1 and clip([(A + STEP, None, 100, 0, 0)]) == -1
     assert clip([(A + STEP, A + 2 * STEP, 100, 2, 0)]) == -2 and clip([(A + STEP, A + 2 * STEP, 100, 0, 1)]) == -2
@@ -108,7 +109,7 @@ def test_gradient_calls(native):
     assert clip([(A + STEP, A + STEP + 16, 100, 0, 0)]) == -4 and clip([good], norms=A + STEP) == -4 and clip([good], limits=A + 2 * STEP) == -4
     assert clip([good], ws=None) == -5 and clip([good], ws_bytes=4) == -5 and clip([good], ws=A + 5 * STEP + 8) == -3
     assert clip([good], ws=A + STEP) == -4 and clip([(A + STEP, A + 2 * STEP, 1 << 40, 0, 0)]) == -7
-    assert lib.mi355_w8a8_grad_norm_v1((native.GradTensor * 1)(native.GradTensor(*good)), 1, 1, None, A, 1 << 20, None) == -1
+    assert lib.mi355_w8a8_grad_norm_v1((native.GradTensor * 1)(native.GradTensor(*good)), 1, 1, None, A, 1 << 20, 0, None) == -1
 
 
 def test_python_grouped(native):
