@@ -341,8 +341,8 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
   a.bits = L.bits; a.passes = L.passes; a.chunks = L.chunks;
   a.notes = words(L.notes);
   // the launches that count clear a share of the gradient each (in those that place the reads would wait behind so many stores: 20 MB beside
-  // 32768 tokens 12 us instead of 9), by 256 workgroups (they write 6.0 TB/s, 2048 of them 5.5), and past the caches where
-  // the last one, 256 MiB, does not hold it (the rows of dy stay there then: 778 MB 193 us in all, 199 through the caches; 102 MB 26 and 23)
+  // 32768 tokens 12 us instead of 9), and past the caches where the
+  // last one, 256 MiB, does not hold it (the rows of dy stay there then: 778 MB 193 us in all, 199 through the caches; 102 MB 26 and 23)
   const uint64_t pieces = out_bytes / 16u;
   const bool small = L.chunks == 1u;
   const uint32_t launches = small ? 1u : L.passes;
@@ -354,8 +354,8 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
     a.clear = static_cast<uint4*>(p->out) + launched * each;
     a.clear_pieces = last ? pieces - launched * each : each;
     a.clear_rest = last ? (uint32_t)(out_bytes % 16u) : 0u;
-    const uint64_t wanted = (a.clear_pieces + 4095u) / 4096u + (a.clear_rest ? 1u : 0u);
-    clearing = (uint32_t)(wanted < 256u ? wanted : 256u);
+    const uint64_t wanted = (a.clear_pieces + 1023u) / 1024u + (a.clear_rest ? 1u : 0u);
+    clearing = (uint32_t)(wanted < kEmbedClearing ? wanted : kEmbedClearing);
     ++launched;
   };
   const uint32_t place_lds = (kEmbedDigits + 16u) * 4u + (32u << L.bits), small_lds = place_lds + 8192u;

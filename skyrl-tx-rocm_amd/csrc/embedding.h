@@ -131,14 +131,18 @@ struct EmbedSortArgs {
 
 __device__ inline uint32_t embed_key(const EmbedSortArgs& a, uint32_t p) { return a.keys ? a.keys[p] : embed_row(a.e, p); }
 
+// The first 256 threads of each of at most 256 workgroups, 16 bytes after 16 bytes all over the share: so few write 6.9 TB/s (past the
+// caches 6.4), four times the threads 6.2 (5.6).
+constexpr uint32_t kEmbedClearing = 256;
 __device__ inline void embed_clear(const EmbedSortArgs& a, uint32_t block, uint32_t blocks) {
-  const uint64_t step = (uint64_t)blocks * 1024u;
+  if (threadIdx.x >= 256u) return;
+  const uint64_t step = (uint64_t)blocks * 256u;
   const v4u_at_2 zeros = {0u, 0u, 0u, 0u};
   v4u_at_2* const clear = reinterpret_cast<v4u_at_2*>(a.clear);
   if (a.stream) {
-    for (uint64_t i = (uint64_t)block * 1024u + threadIdx.x; i < a.clear_pieces; i += step) __builtin_nontemporal_store(zeros, clear + i);
+    for (uint64_t i = (uint64_t)block * 256u + threadIdx.x; i < a.clear_pieces; i += step) __builtin_nontemporal_store(zeros, clear + i);
   } else {
-    for (uint64_t i = (uint64_t)block * 1024u + threadIdx.x; i < a.clear_pieces; i += step) clear[i] = zeros;
+    for (uint64_t i = (uint64_t)block * 256u + threadIdx.x; i < a.clear_pieces; i += step) clear[i] = zeros;
   }
   if (block == 0 && threadIdx.x < a.clear_rest) reinterpret_cast<unsigned char*>(a.clear + a.clear_pieces)[threadIdx.x] = 0;
 }
