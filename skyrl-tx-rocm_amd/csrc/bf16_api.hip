@@ -50,21 +50,47 @@ inline uint64_t most_row_tiles(uint32_t m, uint32_t groups, uint32_t tile) {
   return (m + (uint64_t)(tile - 1u) * held) / tile;
 }
 
+template <int TM, int TN, int STAGES>
+uint32_t grouped_lds(uint32_t groups) { return (TM + TN) * kBgDepth * 2u * STAGES + (kBgScratch + 2u * (groups + 2u)) * 4u; }
+// one workgroup a CU: its stages fill the LDS
+template <int TM, int TN>
+uint32_t grouped_blocks(GroupedKind kind, const BgArgs& g) {
+  const uint64_t n_tiles = (g.cols + TN - 1u) / TN * g.splits;
+  const uint64_t tiles = n_tiles * (kind == kGroupedDw ? (uint64_t)g.groups * ((g.rows + TM - 1u) / TM) : most_row_tiles(g.m, g.groups + 1u, TM));
+  return (uint32_t)(tiles < 256u ? (tiles + 7u) / 8u * 8u : 256u);
+}
 template <int KIND, int TM, int TN, int WM, int WN, int STAGES, int LOADERS, bool F32>
 int launch_grouped_tiles(const BgArgs& g, hipStream_t s) {
   auto kernel = &bf16_grouped_kernel<KIND, TM, TN, WM, WN, STAGES, LOADERS, F32>;
-  const uint32_t lds = (TM + TN) * kBgDepth * 2u * STAGES + (kBgScratch + 2u * (g.groups + 2u)) * 4u;
+  const uint32_t lds = grouped_lds<TM, TN, STAGES>(g.groups);
   if (!allow_lds(kernel, lds)) return MI355_W8A8_ERR_LAUNCH;
-  const uint64_t n_tiles = (g.cols + TN - 1u) / TN * g.splits;
-  const uint64_t tiles = n_tiles * (KIND == kGroupedDw ? (uint64_t)g.groups * ((g.rows + TM - 1u) / TM) : most_row_tiles(g.m, g.groups + 1u, TM));
-  const uint32_t grid = (uint32_t)(tiles < 256u ? (tiles + 7u) / 8u * 8u : 256u);  // (one workgroup a CU: its stages fill the LDS)
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * (WM * WN + LOADERS)), lds, s, g);
+  hipLaunchKernelGGL(kernel, dim3(grouped_blocks<TM, TN>((GroupedKind)KIND, g)), dim3(64 * (WM * WN + LOADERS)), lds, s, g);
+  return launch_status();
+}
+template <int TM, int TN, int WM, int WN, int STAGES, int LOADERS, bool F32>
+int launch_grouped_both(const BgArgs& dx, const BgArgs& dw, hipStream_t s) {
+  auto kernel = &bf16_grouped_both_kernel<TM, TN, WM, WN, STAGES, LOADERS, F32>;
+  const uint32_t lds = grouped_lds<TM, TN, STAGES>(dx.groups);
+  if (!allow_lds(kernel, lds)) return MI355_W8A8_ERR_LAUNCH;
+  const BgBothArgs both{dx, dw, grouped_blocks<TM, TN>(kGroupedDx, dx)};
+  hipLaunchKernelGGL(kernel, dim3(both.dx_blocks + grouped_blocks<TM, TN>(kGroupedDw, dw)), dim3(64 * (WM * WN + LOADERS)), lds, s, both);
   return launch_status();
 }
 
 struct GroupedPlan {
   uint32_t tile;    // one of kGroupedTiles
   uint32_t splits;  // of the contraction
+  float us;         // about what it takes
+};
+struct GroupedSize {  // of C in tiles, and their depth in stages
+  GroupedKind kind;
+  uint32_t m, groups, rows, cols, depth;
+  float held() const { return (float)(groups < m ? groups : m); }
+  float tiles(uint32_t tm, uint32_t tn) const {
+    const float row_tiles = kind == kGroupedDw ? (float)((uint64_t)groups * ((rows + tm - 1u) / tm)) : fmaxf((float)m / tm + 0.5f * held(), held());
+    return row_tiles * ((cols + tn - 1u) / tn);
+  }
+  uint32_t stages() const { return bg_stages(kind == kGroupedDw ? (uint32_t)((float)m / held()) : depth); }
 };
 
 // Which tiles.  A call costs the rounds of its tiles on the 256 CUs times what a round takes: 4 units for 256 x 256, 2.2 for 128 x 256 and
@@ -75,30 +101,30 @@ struct GroupedPlan {
 // 2048 rows 96 / 70 / 126; 1024 -> 1024, 8 groups, 4096 rows 27 / 19 / 19; 512 -> 512, 16 groups, 16384 rows 21 / 17 / 21.5.
 // rows: of C a group (dW); depth: contraction of forward and dx.
 GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols, uint32_t depth, uint32_t forced) {
-  if (forced) return {forced, 1u};
-  const float held = (float)(groups < m ? groups : m);
-  auto tiles = [&](uint32_t tm, uint32_t tn) {
-    const float row_tiles = kind == kGroupedDw ? (float)((uint64_t)groups * ((rows + tm - 1u) / tm)) : fmaxf((float)m / tm + 0.5f * held, held);
-    return row_tiles * ((cols + tn - 1u) / tn);
-  };
+  if (forced) return {forced, 1u, 0.0f};
+  const GroupedSize size{kind, m, groups, rows, cols, depth};
+  const float held = size.held();
+  auto tiles = [&](uint32_t tm, uint32_t tn) { return size.tiles(tm, tn); };
   auto rounds = [](float n) { return n <= 256.0f ? 1.0f : n / 256.0f + 0.5f; };  // (how many tiles the groups make is not known, nor whether they fill the last round)
   const float small_tiles = tiles(64u, 128u), middle_tiles = tiles(128u, 256u);
   const float large = rounds(tiles(256u, 256u)) * 4.0f, middle = rounds(middle_tiles) * 2.2f, small = rounds(small_tiles) * 1.15f;
   uint32_t tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128;
   float round_us = 0.47f;  // a round's time for each stage
-  // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 22 / 18)
+  // (a dW of one round that is not eight stages deep is all latency and stores: 712 -> 1096, 13 groups, 1003 rows, float32 22 / 18 in the
+  // smaller tiles)
   const bool shallow = kind == kGroupedDw && large == 4.0f && m / groups < 8u * kBgDepth;
   if (!shallow && large <= middle && large <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256, round_us = large / 4.0f * 1.7f;
-  else if (shallow || middle <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256, round_us = middle / 2.2f * 0.95f;
+  else if (middle <= small) tile = MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256, round_us = middle / 2.2f * 0.95f;
   else round_us *= small / 1.15f;
   // Few tiles of a long contraction leave most CUs idle: then parts of it are products of their own, with float32 results
   // that a second launch adds up (4 us, and the parts written and read).  Neither is faster than the operands come from memory.  us, whole / in
   // parts: 1 row of 4096 -> 4096 27 / 14.4, 8 rows of 8952 -> 704 in 6 groups 52 / 22, 64 rows of 4096 -> 64 in 16 groups 27 / 13, dW of 272 -> 1696
   // in 4 groups of 28533 rows 78 / 57.
-  const uint32_t stages = bg_stages(kind == kGroupedDw ? (uint32_t)((float)m / held) : depth);
+  const uint32_t stages = size.stages();
   const float bytes = kind == kGroupedDw ? (float)m * (rows + cols) * 2.0f : (held * cols + (float)m) * depth * 2.0f;
   const float values = kind == kGroupedDw ? (float)groups * rows * cols : (float)m * cols, memory_us = bytes / 5.0e6f;
-  float best = 0.9f * fmaxf(round_us * (stages + 3.0f), memory_us);
+  const float whole = fmaxf(round_us * (stages + 3.0f), memory_us);
+  float best = 0.9f * whole;
   uint32_t splits = 1;
   for (uint32_t n = 2; n <= 64u && n * 2u <= stages && middle_tiles * n <= 1024.0f; ++n) {
     const float each = (float)((stages + n - 1u) / n) + 3.0f;
@@ -109,7 +135,7 @@ GroupedPlan plan_grouped(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t
     splits = n;
     tile = s < m2 ? MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128 : MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256;
   }
-  return {tile, splits};
+  return {tile, splits, splits > 1u ? best : whole};
 }
 
 inline uint64_t grouped_plane(GroupedKind kind, uint32_t m, uint32_t groups, uint32_t rows, uint32_t cols) {
@@ -138,6 +164,38 @@ int launch_grouped(BgArgs g, uint32_t forced, void* workspace, hipStream_t s) {
   if (plan.tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256) return launch_grouped_tiles<KIND, 256, 256, 2, 4, 2, 0, F32>(g, s);
   if (plan.tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256) return launch_grouped_tiles<KIND, 128, 256, 2, 4, 3, 4, F32>(g, s);
   return launch_grouped_tiles<KIND, 64, 128, 2, 2, 6, 4, F32>(g, s);
+}
+
+// Tiles for both gradients in one launch, or 0: with tiles of one size for both their work fills the CUs together, and it is a launch (4 us) less; a
+// tile's time is that of its stages.  Not where bytes come near to bound them: reading weights and writing their gradients at once is the slower.  us, two launches /
+// one: 712 -> 1096, 13 groups, 1003 rows, float32 32.3 / 23.5; 128 -> 120, 22 groups, 4051 rows 16 / 7.8; 1024 -> 1024, 8 groups, 4096 rows 41 / 31.5;
+// 1576 -> 1744, 25 groups, 8260 rows 173 / 165; but 1944 -> 2072, 115 groups, 560 rows, float32 675 / 770.
+uint32_t plan_grouped_both(const BgArgs& dx, const BgArgs& dw, uint32_t dw_bytes, uint32_t forced) {
+  const GroupedPlan a = plan_grouped(kGroupedDx, dx.m, dx.groups, dx.rows, dx.cols, dx.depth, forced);
+  const GroupedPlan b = plan_grouped(kGroupedDw, dw.m, dw.groups, dw.rows, dw.cols, dw.depth, forced);
+  if (forced) return forced;
+  if (a.splits > 1u || b.splits > 1u) return 0;
+  const GroupedSize x{kGroupedDx, dx.m, dx.groups, dx.rows, dx.cols, dx.depth}, w{kGroupedDw, dw.m, dw.groups, dw.rows, dw.cols, dw.depth};
+  const float rows = (float)dx.m * (dx.cols + dw.cols) * 2.0f, weights = (float)dx.cols * dw.cols;
+  const float dx_us = (rows + x.held() * weights * 2.0f) / 5.0e6f, dw_us = (rows + w.groups * weights * dw_bytes) / 5.0e6f;
+  float best = 0.97f * (fmaxf(a.us, dx_us) + fmaxf(b.us, dw_us) + 4.0f);
+  uint32_t tile = 0;
+  auto consider = [&](uint32_t flag, uint32_t tm, uint32_t tn, float stage_us) {
+    const float each_x = (x.stages() + 3.0f) * stage_us, each_w = (w.stages() + 3.0f) * stage_us, longest = fmaxf(each_x, each_w);
+    const float us = fmaxf((x.tiles(tm, tn) * each_x + w.tiles(tm, tn) * each_w) / 256.0f + 0.5f * longest, longest);
+    if (us < best && dx_us + dw_us < 0.75f * us) best = us, tile = flag;
+  };
+  consider(MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256, 256u, 256u, 1.7f);
+  consider(MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256, 128u, 256u, 0.95f);
+  consider(MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128, 64u, 128u, 0.47f);
+  return tile;
+}
+template <bool F32>
+int launch_both(BgArgs dx, BgArgs dw, uint32_t tile, hipStream_t s) {
+  dx.splits = dw.splits = 1;
+  if (tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256) return launch_grouped_both<256, 256, 2, 4, 2, 0, F32>(dx, dw, s);
+  if (tile == MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256) return launch_grouped_both<128, 256, 2, 4, 3, 4, F32>(dx, dw, s);
+  return launch_grouped_both<64, 128, 2, 2, 6, 4, F32>(dx, dw, s);
 }
 
 int check_grouped_workspace(const void* workspace, uint64_t given, uint64_t needed) {
@@ -201,20 +259,22 @@ int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s)
   }
   if (overlaps(p->dx, x_bytes, p->dw, dw_bytes) || overlaps(p->workspace, needed, p->dx, x_bytes) || overlaps(p->workspace, needed, p->dw, dw_bytes)) return MI355_W8A8_ERR_ALIAS;
   (void)hipGetLastError();
-  BgArgs g{};
-  g.sizes = p->group_sizes; g.m = p->m; g.groups = p->n_groups;
-  if (p->dx) {
-    g.a = static_cast<const uint16_t*>(p->dy); g.b = static_cast<const uint16_t*>(p->weight); g.out = p->dx;
-    g.rows_ld = p->n; g.cols_ld = p->n; g.depth = p->n; g.cols = p->k;
-    g.b_group = (uint64_t)p->k * p->n;
-    if ((st = launch_grouped<kGroupedDx>(g, forced, p->workspace, s))) return st;
+  BgArgs dx{}, dw{};
+  dx.sizes = dw.sizes = p->group_sizes;
+  dx.m = dw.m = p->m;
+  dx.groups = dw.groups = p->n_groups;
+  dx.a = static_cast<const uint16_t*>(p->dy); dx.b = static_cast<const uint16_t*>(p->weight); dx.out = p->dx;
+  dx.rows_ld = p->n; dx.cols_ld = p->n; dx.depth = p->n; dx.cols = p->k;
+  dx.b_group = (uint64_t)p->k * p->n;
+  dw.a = static_cast<const uint16_t*>(p->x); dw.b = static_cast<const uint16_t*>(p->dy); dw.out = p->dw;
+  dw.rows_ld = p->k; dw.cols_ld = p->n; dw.depth = 0; dw.cols = p->n; dw.rows = p->k;
+  dw.out_group = (uint64_t)p->k * p->n;
+  if (p->dx && p->dw) {
+    const uint32_t tile = plan_grouped_both(dx, dw, f32 ? 4u : 2u, forced);
+    if (tile) return f32 ? launch_both<true>(dx, dw, tile, s) : launch_both<false>(dx, dw, tile, s);
   }
-  if (p->dw) {
-    g.a = static_cast<const uint16_t*>(p->x); g.b = static_cast<const uint16_t*>(p->dy); g.out = p->dw;
-    g.rows_ld = p->k; g.cols_ld = p->n; g.depth = 0; g.cols = p->n; g.rows = p->k;
-    g.out_group = (uint64_t)p->k * p->n;
-    st = f32 ? launch_grouped<kGroupedDw, true>(g, forced, p->workspace, s) : launch_grouped<kGroupedDw>(g, forced, p->workspace, s);
-  }
+  if (p->dx && (st = launch_grouped<kGroupedDx>(dx, forced, p->workspace, s))) return st;
+  if (p->dw) st = f32 ? launch_grouped<kGroupedDw, true>(dw, forced, p->workspace, s) : launch_grouped<kGroupedDw>(dw, forced, p->workspace, s);
   return st;
 }
 

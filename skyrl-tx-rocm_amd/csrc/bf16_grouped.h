@@ -97,7 +97,7 @@ constexpr uint32_t kBgScratch = 64;
 // Sizes are clamped to [0, m] one by one, starts to [0, m]: whatever the array holds, no row beyond m is touched.
 // tiles_of, cost_of: tiles of a group with `rows` rows (nothing behind the last of `held` groups), what each costs.  scratch: kBgScratch words.
 template <int THREADS, class TilesOf, class CostOf>
-__device__ inline BgShare bg_tables(const BgArgs& g, uint32_t held, const BgTables& tab, uint32_t* scratch, TilesOf tiles_of, CostOf cost_of) {
+__device__ inline BgShare bg_tables(const BgArgs& g, uint32_t block, uint32_t held, const BgTables& tab, uint32_t* scratch, TilesOf tiles_of, CostOf cost_of) {
   constexpr uint32_t kPer = (kBgMaxGroups + THREADS) / THREADS, kWaves = THREADS / 64;  // groups a thread looks at, one more for the rows behind them
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   uint32_t size[kPer], rows = 0, first = tid * kPer;
@@ -150,7 +150,7 @@ __device__ inline BgShare bg_tables(const BgArgs& g, uint32_t held, const BgTabl
     all += costs[w];
   }
   // tiles in front of the share that starts at x eighths of the cost: found by the thread whose groups hold that place
-  const uint32_t die = blockIdx.x & 7u;
+  const uint32_t die = block & 7u;
   const uint64_t from = all * die / 8u, to = all * (die + 1u) / 8u;
   if (tid == 0) {
     tab.start[g.groups + 1u] = g.m;
@@ -270,9 +270,9 @@ struct BgTile {
 // share).  A wave's loads and stores return in one order, so one that waits for a stage waits for the results it stored before: with
 // loaders nobody does, which is what a dW of few stages a tile is made of.  A workgroup takes tile after tile, and the stages of one follow those of
 // the tile before in one stream: while a tile's results are stored the first stages of the next are on their way.
-// A die's workgroups take the tiles of its share in turn.
-template <int KIND, int TM, int TN, int WM, int WN, int STAGES, int LOADERS = 0, bool F32 = false>
-__global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(BgArgs g) {
+// A die's workgroups take the tiles of its share in turn.  block, blocks: of this product's workgroups (a multiple of eight).
+template <int KIND, int TM, int TN, int WM, int WN, int STAGES, int LOADERS, bool F32>
+__device__ __forceinline__ void bg_run(const BgArgs& g, uint32_t block, uint32_t blocks) {
   constexpr int BK = kBgDepth;
   constexpr int kWaves = WM * WN, kLoading = LOADERS ? LOADERS : kWaves, FM = TM / WM / 16, FN = TN / WN / 16;
   static_assert(FN % (F32 ? 2 : 4) == 0, "a wave stores whole lines");
@@ -289,15 +289,15 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
   tab.tile = tab.start + g.groups + 2u;
   const uint32_t held = KIND == kGroupedDw ? g.groups : g.groups + 1u;
   const BgShare share = bg_tables<64 * (kWaves + LOADERS)>(
-      g, held, tab, scratch,
+      g, block, held, tab, scratch,
       [&](uint32_t rows) { return ((KIND == kGroupedDw ? g.rows : rows) + TM - 1u) / TM * n_tiles * (F32 ? g.splits : 1u); },
       // (a tile's results take about as long to store as three of its stages to compute)
       [&](uint32_t group, uint32_t rows) {
         const uint32_t stages = bg_stages(KIND == kGroupedDw ? rows : (group < g.groups ? g.depth : 0u));
         return 3u + (F32 ? (stages + g.splits - 1u) / g.splits : stages);
       });
-  const uint32_t stride = gridDim.x >> 3, end = share.end;
-  uint32_t tile = share.first + (blockIdx.x >> 3);
+  const uint32_t stride = blocks >> 3, end = share.end;
+  uint32_t tile = share.first + (block >> 3);
   if (tile >= end) return;
 
   auto describe = [&](uint32_t t) {
@@ -533,6 +533,19 @@ __global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(
     stored = true;
   }
   if constexpr (!LOADERS) wait_vmcnt0();
+}
+
+template <int KIND, int TM, int TN, int WM, int WN, int STAGES, int LOADERS = 0, bool F32 = false>
+__global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_kernel(BgArgs g) {
+  bg_run<KIND, TM, TN, WM, WN, STAGES, LOADERS, F32>(g, blockIdx.x, gridDim.x);
+}
+
+// Both gradients in one launch: dx by the first dx_blocks workgroups, dW by the others, which begin where dx leaves CUs or is done.
+struct BgBothArgs { BgArgs dx, dw; uint32_t dx_blocks; };
+template <int TM, int TN, int WM, int WN, int STAGES, int LOADERS, bool F32>
+__global__ __launch_bounds__(64 * (WM * WN + LOADERS)) void bf16_grouped_both_kernel(BgBothArgs g) {
+  if (blockIdx.x < g.dx_blocks) bg_run<kGroupedDx, TM, TN, WM, WN, STAGES, LOADERS, false>(g.dx, blockIdx.x, g.dx_blocks);
+  else bg_run<kGroupedDw, TM, TN, WM, WN, STAGES, LOADERS, F32>(g.dw, blockIdx.x - g.dx_blocks, gridDim.x - g.dx_blocks);
 }
 
 // The parts of a split contraction: C = their sum in order, with the one rounding.  A thread four values of C.
