@@ -93,6 +93,32 @@ def test_each_tile(gl, rows, k, n, sizes, tile):
     x, w, dy, st = make(rows, k, n, sizes, seed=1)
     check(gl, x, w, dy, st, sizes, flags=flags)
     check(gl, x, w, dy, st, sizes, torch.float32, flags=flags)
+    for dtype in (torch.bfloat16, torch.float32):  # in one launch and by themselves: the same bits
+        dx, dw = gl.grouped_matmul_backward(x, dy, w, st, dw_dtype=dtype, flags=flags)
+        assert torch.equal(dx, gl.grouped_matmul_backward(None, dy, w, st, need_dw=False, flags=flags)[0])
+        assert torch.equal(dw, gl.grouped_matmul_backward(x, dy, None, st, need_dx=False, dw_dtype=dtype, flags=flags)[1])
+
+
+@pytest.mark.parametrize("rows,k,n,groups", [
+    (4051, 128, 120, 22), (886, 168, 736, 13), (1003, 712, 1096, 13), (4096, 1024, 1024, 8), (300, 64, 280, 28), (8000, 1576, 1744, 25), (1, 8, 8, 1), (70, 40, 136, 1024)])
+def test_both_gradients_and_each(gl, rows, k, n, groups):
+    """The sizes at which both come from one launch, with empty and uneven groups and spare rows, against float64 and in a captured graph."""
+    g = torch.Generator().manual_seed(rows)
+    share = torch.rand(groups, generator=g) ** 2 * (torch.rand(groups, generator=g) > 0.25)
+    share[0] += 0.01
+    sizes = (share / share.sum() * rows * 0.97).long().tolist()
+    x, w, dy, st = make(rows, k, n, sizes, seed=6)
+    check(gl, x, w, dy, st, sizes)
+    check(gl, x, w, dy, st, sizes, torch.float32)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, dw = gl.grouped_matmul_backward(x, dy, w, st)
+    for turn in range(3):
+        dy.copy_(torch.randn(dy.shape, device=DEV))
+        st.copy_(st.roll(1))
+        graph.replay()
+        got = dx.clone(), dw.clone()
+        assert all(torch.equal(a, b) for a, b in zip(got, gl.grouped_matmul_backward(x, dy, w, st))), turn
 
 
 @pytest.mark.parametrize("sizes", [[0, 0, 0], [40, 200, 7], [-5, 40, -1], [1 << 30, 5, 1 << 30], [100, 0, 0]])
