@@ -66,7 +66,8 @@ class GradClipPlan:
     ``grads`` are contiguous bf16 or float32 tensors, read at every run where they lie: a loop whose backward writes the same
     buffers each step (``BackwardPlan``) builds the plan once.  ``max_norm`` is a number or a tensor (one value, or [adapters]
     with ``per_adapter``); None: only norms.  A contiguous float32 [adapters] tensor on the gradients' device is read at every
-    run where it lies, any other form is copied when the plan is made.  Runs of a plan share its workspace: on one stream, or one behind the other.  ``out`` names the tensors that the scaled gradients go
+    run where it lies, any other form is copied when the plan is made.  Runs of a plan share its workspace: on one stream, or one behind the
+    other; a graph that captured one needs the plan as long as it is replayed.  ``out`` names the tensors that the scaled gradients go
     to, of the same shapes and types; the gradients themselves scale in place."""
 
     def __init__(self, grads, max_norm=None, *, per_adapter: bool = False, out=None):
@@ -121,8 +122,9 @@ class GradClipPlan:
             else:
                 status = self._lib.mi355_w8a8_grad_clip_v1(table, len(table), self._adapters, self.limits.data_ptr(), self.norms.data_ptr(),
                                                            ws.data_ptr(), ws.numel(), flags, stream)
+            written = not flags and not torch.cuda.is_current_stream_capturing()  # (a captured run has written nothing yet)
         _native.check("mi355_w8a8_grad_norm_v1" if self.limits is None else "mi355_w8a8_grad_clip_v1", status)
-        if not flags and not torch.cuda.is_current_stream_capturing():  # (a captured run has written nothing yet)
+        if written:
             self._table_kept = _native.FLAG_GRAD_TABLE_KEPT
         return self.out, (self.norms if self._per_adapter else self.norms.reshape(()))
 
