@@ -218,6 +218,11 @@ bool here(const at::Tensor* t) {
   return t && t->is_cuda() && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
          c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice() == t->device();
 }
+// no flags but those of the tiles: the type of dw is that of the tensor made here
+bool grouped_flags(int64_t flags) {
+  return (flags & ~(int64_t)(MI355_W8A8_FLAG_BF16_GROUPED_TILE_256X256 | MI355_W8A8_FLAG_BF16_GROUPED_TILE_128X256 |
+                             MI355_W8A8_FLAG_BF16_GROUPED_TILE_64X128)) == 0;
+}
 bool grouped_dims(int64_t m, int64_t k, int64_t n, int64_t g) {
   return m > 0 && m <= (1 << 20) && k > 0 && n > 0 && k % 8 == 0 && n % 8 == 0 && k <= MI355_W8A8_BF16_GROUPED_MAX_FEATURES &&
          n <= MI355_W8A8_BF16_GROUPED_MAX_FEATURES && g > 0 && g <= 1024;
@@ -233,7 +238,7 @@ PyObject* grouped(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_bf16_grouped_problem*, void*)>(arg.address(4));
   const auto bytes_of = reinterpret_cast<uint64_t (*)(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t)>(arg.address(5));
   void* const stream = arg.address(6);
-  if (!arg.ok || !entry || !bytes_of || !here(x)) Py_RETURN_NONE;
+  if (!arg.ok || !entry || !bytes_of || !grouped_flags(flags) || !here(x)) Py_RETURN_NONE;
   const c10::Device device = x->device();
   if (!whole(x, at::kBFloat16, device, 2) || !whole(w, at::kBFloat16, device, 3) || !sizes || !plain(*sizes, at::kInt, device) || sizes->dim() != 1) Py_RETURN_NONE;
   const int64_t m = x->size(0), k = x->size(1), n = w->size(2), g = w->size(0);
@@ -271,7 +276,7 @@ PyObject* grouped_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   const auto entry = reinterpret_cast<int (*)(const mi355_w8a8_bf16_grouped_bwd_problem*, void*)>(arg.address(8));
   const auto bytes_of = reinterpret_cast<uint64_t (*)(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t)>(arg.address(9));
   void* const stream = arg.address(10);
-  if (!arg.ok || !entry || !bytes_of || !here(dy) || !x || !w) Py_RETURN_NONE;
+  if (!arg.ok || !entry || !bytes_of || !grouped_flags(flags) || !here(dy) || !x || !w) Py_RETURN_NONE;
   const c10::Device device = dy->device();
   if (!whole(dy, at::kBFloat16, device, 2) || !whole(x, at::kBFloat16, device, 2) || !whole(w, at::kBFloat16, device, 3) || !sizes ||
       !plain(*sizes, at::kInt, device) || sizes->dim() != 1)

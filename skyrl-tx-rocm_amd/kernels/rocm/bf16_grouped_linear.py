@@ -57,6 +57,15 @@ def _geometry(rows: torch.Tensor, name: str, width: int, weight_shape, group_siz
     return m, k, n, g, sizes.to(device=dev, dtype=torch.int32).contiguous()
 
 
+_TILES = (0, _native.FLAG_BF16_GROUPED_TILE_256X256, _native.FLAG_BF16_GROUPED_TILE_128X256, _native.FLAG_BF16_GROUPED_TILE_64X128)
+
+
+def _check_flags(flags: int) -> None:
+    """The tiles are all that a caller may force: the C calls know a flag for the type of dw too, which has to be that of the tensor."""
+    if flags not in _TILES:
+        raise ValueError(f"flags must be 0 or one of FLAG_BF16_GROUPED_TILE_*, got {flags!r}")
+
+
 def _same_device(first: torch.Tensor, *others) -> None:
     for t in others:
         if t.device != first.device:
@@ -67,6 +76,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Ten
     """``out[rows of g] = bf16(x[rows of g] @ weight[g])`` with float32 sums: x bf16 [rows, K], weight bf16
     [groups, K, N], group_sizes integers [groups].  Rows behind the last group are zero.  ``flags`` may force the tiles
     (``_native.FLAG_BF16_GROUPED_TILE_*``); by default they follow the sizes."""
+    _check_flags(flags)
     host = _native.host() if isinstance(x, torch.Tensor) and x.is_cuda else None
     if host is not None:
         # an ordinary call goes through the host module; for any other it returns None
@@ -101,6 +111,7 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
         raise ValueError("dw needs x and dx needs weight")
     if dw_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"dw_dtype must be BF16 or FP32, got {dw_dtype}")
+    _check_flags(flags)
     host = _native.host() if isinstance(dy, torch.Tensor) and dy.is_cuda else None
     if host is not None:
         result = host.grouped_bwd(x, dy, weight, group_sizes, need_dx, need_dw, dw_dtype == torch.float32, flags,

@@ -188,3 +188,20 @@ def test_capture_beside_a_living_graph(native, monkeypatch):
     gl.check_capture(mine)
     capturing[0] = False
     gl.check_capture(mine)
+
+
+@pytest.mark.parametrize("flags", [1, 2, 5, 12, 32, -1, 1 << 32, 1 << 40])
+def test_flags_that_are_no_tiles(native, flags):
+    """Above all the C call's flag of a float32 dw (1): beside a bf16 dw its stores would go past the tensor's end."""
+    gl = load_package().bf16_grouped_linear
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    sizes = torch.zeros(2, dtype=torch.int32)
+    assert native.FLAG_BF16_GROUPED_DW_F32 == 1
+    with pytest.raises(ValueError, match="flags"):
+        gl.grouped_matmul(bf(4, 8), bf(2, 8, 8), sizes, flags=flags)
+    for dtype in (torch.bfloat16, torch.float32):
+        with pytest.raises(ValueError, match="flags"):
+            gl.grouped_matmul_backward(bf(4, 8), bf(4, 8), bf(2, 8, 8), sizes, dw_dtype=dtype, flags=flags)
+    for tile in (0, 4, 8, 16):  # (these go on, to the next check)
+        with pytest.raises(RuntimeError, match="GPU"):
+            gl.grouped_matmul(bf(4, 8), bf(2, 8, 8), sizes, flags=tile)
