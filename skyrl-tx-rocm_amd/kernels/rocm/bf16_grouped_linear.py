@@ -34,6 +34,16 @@ def _bf16(t: torch.Tensor, name: str) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()  # (a view into the middle of a buffer: the kernels load 16 bytes)
 
 
+def whole_numbers(t: torch.Tensor, name: str, low: int, high: int) -> torch.Tensor:
+    """``t`` as int32, with what that cannot hold at ``low`` or ``high``.  (Clamped as int64: a narrower type may not hold the bounds, and
+    those of an unsigned one turn over.)"""
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype in (torch.bool, torch.uint64):
+        raise TypeError(f"{name} must be integers that int64 holds, got {t.dtype}")
+    if t.dtype in (torch.int64, torch.uint32):
+        t = t.to(torch.int64).clamp(low, high)
+    return t.to(torch.int32)
+
+
 def _geometry(rows: torch.Tensor, name: str, width: int, weight_shape, group_sizes: torch.Tensor):
     """``(m, k, n, groups, sizes)`` of a call, or what is wrong with it."""
     if len(weight_shape) != 3:
@@ -43,18 +53,13 @@ def _geometry(rows: torch.Tensor, name: str, width: int, weight_shape, group_siz
         raise ValueError(f"{name} must be [rows, {weight_shape[width]}] with at least one row, got {tuple(rows.shape)}")
     if group_sizes.ndim != 1 or group_sizes.shape[0] != g:
         raise ValueError(f"group_sizes must have shape ({g},), got {tuple(group_sizes.shape)}")
-    if group_sizes.dtype.is_floating_point or group_sizes.dtype == torch.bool:
-        raise TypeError(f"group_sizes must be integers, got {group_sizes.dtype}")
     m = rows.shape[0]
+    sizes = whole_numbers(group_sizes.detach(), "group_sizes", 0, m)  # (what an int32 could not hold is more than there are rows)
     if k % 8 or n % 8 or not 0 < k <= MAX_FEATURES or not 0 < n <= MAX_FEATURES:
         raise ValueError(f"K and N must be positive multiples of 8 not exceeding {MAX_FEATURES}, got {k} and {n}")
     if not 0 < g <= MAX_GROUPS or m > MAX_ROWS:
         raise ValueError(f"at most {MAX_GROUPS} groups and {MAX_ROWS} rows are supported, got {g} and {m}")
-    dev = rows.device
-    sizes = group_sizes.detach()
-    if sizes.dtype != torch.int32:
-        sizes = sizes.clamp(0, m)  # (what an int32 could not hold is more than there are rows)
-    return m, k, n, g, sizes.to(device=dev, dtype=torch.int32).contiguous()
+    return m, k, n, g, sizes.to(rows.device).contiguous()
 
 
 _TILES = (0, _native.FLAG_BF16_GROUPED_TILE_256X256, _native.FLAG_BF16_GROUPED_TILE_128X256, _native.FLAG_BF16_GROUPED_TILE_64X128)

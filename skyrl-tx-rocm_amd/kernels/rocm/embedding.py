@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ... import _native
-from .bf16_grouped_linear import check_capture, note_leaves
+from .bf16_grouped_linear import check_capture, note_leaves, whole_numbers
 from .w8a8_lora import _on, _require_cuda, _stream_ptr
 
 MAX_TOKENS = 1 << 20
@@ -47,16 +47,12 @@ def _problem(ids, shape, scale, adapter_indices, dtype, dev):
     if adapter_indices is not None:
         if not adapters:
             raise ValueError("adapter_indices given without a table of adapters")
-        index = adapter_indices.detach().reshape(-1)
-        if index.dtype.is_floating_point or index.dtype == torch.bool:
-            raise TypeError(f"adapter_indices must be integers, got {index.dtype}")
+        index = whole_numbers(adapter_indices.detach().reshape(-1), "adapter_indices", -1, adapters)
         if index.shape[0] != n:
             if index.shape[0] == 0 or n % index.shape[0]:
                 raise ValueError(f"adapter_indices of length {index.shape[0]} do not divide {n} ids")
             index = index.repeat_interleave(n // index.shape[0])  # one entry per example
-        if index.dtype != torch.int32:
-            index = index.clamp(-1, adapters)
-        index = index.to(device=dev, dtype=torch.int32).contiguous()
+        index = index.to(dev).contiguous()
     elif adapters > 1:
         raise ValueError("a table of several adapters needs adapter_indices")
     scales, factor = None, 1.0

@@ -22,7 +22,7 @@ from ..kernels import quantized_lora as ql
 from ..kernels.rocm import embedding as emb
 from ..kernels.rocm import grad_clip
 from ..kernels.rocm import w8a8_lora as w8
-from ..kernels.rocm.bf16_grouped_linear import bf16_grouped_linear
+from ..kernels.rocm.bf16_grouped_linear import bf16_grouped_linear, whole_numbers
 
 
 class LoRAMixin:
@@ -227,11 +227,10 @@ class LoRAEmbed(LoRAMixin):
             return out
         if ids.ndim == 0 or adapter_indices.ndim != 1 or adapter_indices.shape[0] != ids.shape[0]:
             raise ValueError("adapter_indices must hold one entry per example (leading axis of ids)")
-        if adapter_indices.dtype.is_floating_point or adapter_indices.dtype == torch.bool:
-            raise TypeError(f"adapter_indices must be integers, got {adapter_indices.dtype}")
         n_ad = self.max_lora_adapters
         flat = ids.reshape(-1)
-        adapters = adapter_indices.clamp(-1, n_ad).to(device=flat.device, dtype=torch.int32).repeat_interleave(flat.numel() // adapter_indices.shape[0])
+        adapters = whole_numbers(adapter_indices, "adapter_indices", -1, n_ad).clamp(-1, n_ad)
+        adapters = adapters.to(flat.device).repeat_interleave(flat.numel() // adapter_indices.shape[0])
         order = back = None
         sizes = torch.full((1,), flat.numel(), dtype=torch.int32, device=flat.device)
         if n_ad > 1:

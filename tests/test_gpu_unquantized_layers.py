@@ -323,3 +323,33 @@ def test_second_derivatives_are_refused():
     dx, = torch.autograd.grad(pkg.bf16_grouped_linear.bf16_grouped_linear(x, w, torch.tensor([4], device=DEV)).float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32])
+def test_whole_numbers_of_any_width(lora, dtype):
+    """Adapters and sizes of narrow types give what int64 ones give, forward and backward."""
+    pkg = load_package()
+    g = torch.Generator(device=DEV).manual_seed(11)
+    layer = lora.LoRAEmbed(50, 24, embedding=torch.randn(50, 24, generator=g, device=DEV), max_lora_adapters=3)
+    fill(layer, g)
+    ids, index = torch.randint(0, 50, (6, 5), generator=g, device=DEV), torch.tensor([0, 2, 1, 1, 0, 2], device=DEV)
+    dy = torch.randn(6, 5, 24, generator=g, device=DEV).to(BF16)
+
+    def of(index):
+        out = layer(ids, index)
+        return out.detach(), *torch.autograd.grad(out, (layer.lora_A, layer.lora_B), dy)
+
+    want = of(index)
+    assert all(torch.equal(a, b) for a, b in zip(want, of(index.to(dtype)))) and not torch.equal(want[0], layer(ids).detach()) and want[1].any()
+    if dtype.is_signed:
+        assert torch.equal(layer(ids, torch.full((6,), -1, dtype=dtype, device=DEV)), layer(ids))
+    em, gl = pkg.embedding, pkg.bf16_grouped_linear
+    assert torch.equal(em.lookup(layer.lora_A, ids, 2.0, adapter_indices=index.to(dtype)), em.lookup(layer.lora_A, ids, 2.0, adapter_indices=index))
+    sizes = torch.tensor([100, 0, 127], device=DEV)
+    x, w = torch.randn(40000, 16, generator=g, device=DEV).to(BF16), torch.randn(3, 16, 24, generator=g, device=DEV).to(BF16)
+    assert torch.equal(gl.grouped_matmul(x, w, sizes.to(dtype)), gl.grouped_matmul(x, w, sizes))
+    experts = lora.LoRAExpert(3, 16, 24, max_lora_adapters=3)
+    experts.load_unquantized(w)
+    fill(experts, g)
+    adapters = torch.randint(0, 3, (40000,), generator=g, device=DEV)
+    assert torch.equal(experts(x, sizes.to(dtype), adapters.to(dtype)), experts(x, sizes, adapters))

@@ -205,3 +205,33 @@ def test_flags_that_are_no_tiles(native, flags):
     for tile in (0, 4, 8, 16):  # (these go on, to the next check)
         with pytest.raises(RuntimeError, match="GPU"):
             gl.grouped_matmul(bf(4, 8), bf(2, 8, 8), sizes, flags=tile)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64])
+def test_whole_numbers_of_any_width(native, monkeypatch, dtype):
+    """Sizes and adapter indices keep their values where there are more rows or adapters than their type can hold."""
+    from skyrl_tx_rocm_amd.kernels.rocm import bf16_grouped_linear as gl, embedding as em
+    sizes = gl._geometry(torch.zeros(40000, 8, dtype=torch.bfloat16), "x", 1, (3, 8, 8), torch.tensor([100, 0, 27], dtype=dtype))[-1]
+    assert sizes.dtype == torch.int32 and sizes.tolist() == [100, 0, 27]
+    monkeypatch.setattr(em, "_require_cuda", lambda t, name: None)
+    ids = torch.zeros(3, dtype=torch.int64)
+    for adapters, given in ((2, [0, 1, 1]), (40000, [0, 127, 3])):
+        _, (_, index, _) = em._problem(ids, (adapters, 4, 8), None, torch.tensor(given, dtype=dtype), torch.bfloat16, ids.device)
+        assert index.dtype == torch.int32 and index.tolist() == given
+    if dtype.is_signed:
+        assert gl._geometry(torch.zeros(40000, 8, dtype=torch.bfloat16), "x", 1, (2, 8, 8), torch.tensor([-7, 3], dtype=dtype))[-1].tolist()[0] <= 0
+        assert int(em._problem(ids, (2, 4, 8), None, torch.tensor([-1, -128, 1], dtype=dtype), torch.bfloat16, ids.device)[1][1][:2].max()) < 0
+    if dtype in (torch.int64, torch.uint32):  # what int32 cannot hold is out of range, not another number
+        assert gl._geometry(torch.zeros(40000, 8, dtype=torch.bfloat16), "x", 1, (2, 8, 8), torch.tensor([2 ** 32 - 1, 3], dtype=dtype))[-1].tolist() == [40000, 3]
+        assert em._problem(ids, (2, 4, 8), None, torch.tensor([2 ** 32 - 1, 2 ** 31, 1], dtype=dtype), torch.bfloat16, ids.device)[1][1].tolist() == [2, 2, 1]
+
+
+def test_what_are_no_whole_numbers(native, monkeypatch):
+    from skyrl_tx_rocm_amd.kernels.rocm import bf16_grouped_linear as gl, embedding as em
+    monkeypatch.setattr(em, "_require_cuda", lambda t, name: None)
+    ids = torch.zeros(2, dtype=torch.int64)
+    for dtype in (torch.float32, torch.bool, torch.complex64, torch.uint64):
+        with pytest.raises(TypeError, match="integers"):
+            gl._geometry(torch.zeros(4, 8, dtype=torch.bfloat16), "x", 1, (2, 8, 8), torch.zeros(2, dtype=dtype))
+        with pytest.raises(TypeError, match="integers"):
+            em._problem(ids, (2, 4, 8), None, torch.zeros(2, dtype=dtype), torch.bfloat16, ids.device)
