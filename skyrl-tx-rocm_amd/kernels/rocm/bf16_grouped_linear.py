@@ -110,6 +110,7 @@ def grouped_matmul_backward(x: torch.Tensor | None, dy: torch.Tensor, weight: to
     """Cotangents ``(dx, dw)`` of ``grouped_matmul``: ``dx[rows of g] = bf16(dy[rows of g] @ weight[g].T)`` and
     ``dw[g] = x[rows of g].T @ dy[rows of g]`` in ``dw_dtype`` (bf16 or float32), both from float32 sums; None for the one
     that is not wanted.  ``x`` may be None without ``need_dw``, ``weight`` without ``need_dx``."""
+    need_dx, need_dw = bool(need_dx), bool(need_dw)  # (the host module takes True alone for yes)
     if not need_dx and not need_dw:
         return None, None
     if (need_dw and x is None) or (need_dx and weight is None):

@@ -4,6 +4,7 @@ Tolerance: products of bf16 values are exact in float32, so a sum of d of them i
 products' magnitudes; one unit of the last place an addition, whichever way the matrix instruction rounds), and the one
 rounding to bf16 by half a step, 2^-8 of the value."""
 
+import numpy
 import pytest
 import torch
 
@@ -301,3 +302,17 @@ def test_the_most_groups_and_rows(gl):
     assert torch.equal(dw, outer)
     with pytest.raises(ValueError, match="at most"):
         gl.grouped_matmul(torch.zeros(rows + 1, 8, dtype=torch.bfloat16, device=DEV), w, sizes)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_wanted_gradients_go_by_truth(gl, monkeypatch, native):
+    """Whole numbers and NumPy's truth values say what True and False say, through the host module and without it."""
+    if not native:
+        monkeypatch.setattr(load_package()._native, "host", lambda: None)
+    x, w, dy, st = make(50, 64, 40, [20, 0, 25])
+    dx, dw = gl.grouped_matmul_backward(x, dy, w, st)
+    for want_dx, want_dw in ((1, 1), (1, 0), (0, 1), (True, 1), (2, False), (numpy.True_, numpy.True_), (numpy.True_, numpy.False_), (numpy.bool_(0), numpy.bool_(1))):
+        got = gl.grouped_matmul_backward(x, dy, w, st, need_dx=want_dx, need_dw=want_dw)
+        for value, ref, wanted in zip(got, (dx, dw), (want_dx, want_dw)):
+            assert torch.equal(value, ref) if wanted else value is None, (want_dx, want_dw)
+    assert gl.grouped_matmul_backward(x, dy, w, st, need_dx=0, need_dw=numpy.False_) == (None, None)
