@@ -22,7 +22,7 @@ from ..kernels import quantized_lora as ql
 from ..kernels.rocm import embedding as emb
 from ..kernels.rocm import grad_clip
 from ..kernels.rocm import w8a8_lora as w8
-from ..kernels.rocm.bf16_grouped_linear import bf16_grouped_linear, whole_numbers
+from ..kernels.rocm.bf16_grouped_linear import MAX_GROUPS, bf16_grouped_linear, whole_numbers
 
 
 class LoRAMixin:
@@ -229,17 +229,19 @@ class LoRAEmbed(LoRAMixin):
             raise ValueError("adapter_indices must hold one entry per example (leading axis of ids)")
         n_ad = self.max_lora_adapters
         flat = ids.reshape(-1)
-        adapters = whole_numbers(adapter_indices, "adapter_indices", -1, n_ad).clamp(-1, n_ad)
-        adapters = adapters.to(flat.device).repeat_interleave(flat.numel() // adapter_indices.shape[0])
-        order = back = None
-        sizes = torch.full((1,), flat.numel(), dtype=torch.int32, device=flat.device)
-        if n_ad > 1:
-            _, sizes, order, back, _ = w8.moe_dispatch(None, adapters, n_ad)
-            flat, adapters = flat.index_select(0, order), adapters.index_select(0, order)
-        z = emb.embed(self.lora_A, flat, self.lora_scaling, adapter_indices=adapters)
-        delta = bf16_grouped_linear(_whole_units(z, 1), _whole_units(self.lora_B, 1), sizes)
-        if order is not None:
-            delta = _Reorder.apply(delta, back, order)
+        adapters = whole_numbers(adapter_indices, "adapter_indices", -1, n_ad).to(flat.device)
+        adapters = adapters.repeat_interleave(flat.numel() // adapter_indices.shape[0])
+        # A token without an adapter or a row goes behind the last adapter's: there it has no part in the product and its gradients, which would
+        # carry infinities of B into its row and those of the row's gradient into B's.
+        held = (flat >= 0) & (flat < self.num_embeddings) & (adapters >= 0) & (adapters < n_ad)
+        adapters = torch.where(held, adapters, n_ad)
+        groups = min(n_ad + 1, MAX_GROUPS)
+        _, sizes, order, back, _ = w8.moe_dispatch(None, adapters, groups)
+        z = emb.embed(self.lora_A, flat.index_select(0, order), self.lora_scaling, adapter_indices=adapters.index_select(0, order))
+        delta = bf16_grouped_linear(_whole_units(z, 1), _whole_units(self.lora_B, 1), sizes[:n_ad])
+        delta = _Reorder.apply(delta, back, order)
+        if groups == n_ad:  # (no group is left for them: they are among the last adapter's)
+            delta = torch.where(held[:, None], delta, 0)
         return out + delta.reshape(out.shape)
 
 

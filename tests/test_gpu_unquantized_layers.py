@@ -353,3 +353,24 @@ def test_whole_numbers_of_any_width(lora, dtype):
     fill(experts, g)
     adapters = torch.randint(0, 3, (40000,), generator=g, device=DEV)
     assert torch.equal(experts(x, sizes.to(dtype), adapters.to(dtype)), experts(x, sizes, adapters))
+
+
+@pytest.mark.parametrize("n_ad", [1, 3, 1024])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_infinities_beside_adapters_and_ids_out_of_range(lora, n_ad, bad):
+    """A token without an adapter or a row has no part in the adapters' term: infinities of B do not reach its row, those of its gradient neither A nor B."""
+    g = torch.Generator(device=DEV).manual_seed(12)
+    layer = lora.LoRAEmbed(40, 16, embedding=torch.randn(40, 16, generator=g, device=DEV), max_lora_adapters=n_ad)
+    fill(layer, g)
+    ids = torch.tensor([[3, 4], [5, 6], [7, 40], [-1, 8]], device=DEV)
+    index = torch.tensor([-1, 2 ** 32, n_ad, n_ad - 1], device=DEV)
+    dy = torch.randn(4, 2, 16, generator=g, device=DEV).to(BF16)
+    held = torch.zeros(4, 2, dtype=torch.bool, device=DEV)
+    held[3, 1] = True
+    out = layer(ids, index)
+    want = torch.autograd.grad(out, (layer.lora_A, layer.lora_B), dy)
+    got = torch.autograd.grad(layer(ids, index), (layer.lora_A, layer.lora_B), torch.where(held[..., None], dy, bad))
+    assert all(torch.equal(a, b) and torch.isfinite(a).all() and a.any() for a, b in zip(got, want))
+    layer.lora_B.data[...] = bad
+    other = layer(ids, index)
+    assert torch.equal(other[~held], out[~held]) and torch.equal(other[~held], layer(ids)[~held]) and not torch.isfinite(other[held]).any()
