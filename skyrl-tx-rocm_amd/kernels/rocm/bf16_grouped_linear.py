@@ -16,6 +16,7 @@ import ctypes
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ... import _native
@@ -182,6 +183,13 @@ def check_capture(uses: list) -> None:
                                "let go of its outputs (the last loss, say) first, or run it on the capture's stream")
 
 
+def refuse_tangents(name: str, *tensors) -> None:
+    """Forward-mode derivatives do not exist here; a dual tensor's would be lost without a word."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 class _GroupedMatmulFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group_sizes):
@@ -201,6 +209,7 @@ class _GroupedMatmulFunction(torch.autograd.Function):
 
 def bf16_grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_sizes: torch.Tensor) -> torch.Tensor:
     """``grouped_matmul`` that autograd can differentiate in ``x`` and ``weight``."""
+    refuse_tangents("bf16_grouped_linear", x, weight)
     if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
         return grouped_matmul(x, weight, group_sizes)
     return _GroupedMatmulFunction.apply(x, weight, group_sizes)

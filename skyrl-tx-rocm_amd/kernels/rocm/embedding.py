@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ... import _native
-from .bf16_grouped_linear import check_capture, note_leaves, whole_numbers
+from .bf16_grouped_linear import check_capture, note_leaves, refuse_tangents, whole_numbers
 from .w8a8_lora import _on, _require_cuda, _stream_ptr
 
 MAX_TOKENS = 1 << 20
@@ -149,6 +149,7 @@ class _LookupFunction(torch.autograd.Function):
 
 def embed(table: torch.Tensor, ids: torch.Tensor, scale=None, *, adapter_indices: torch.Tensor | None = None) -> torch.Tensor:
     """``lookup`` that autograd can differentiate in the table (the scale is a constant)."""
+    refuse_tangents("embed", table, scale)
     if isinstance(scale, torch.Tensor) and scale.requires_grad:
         raise ValueError("the scale of an embedding is a constant: detach it")
     if not (torch.is_grad_enabled() and table.requires_grad):

@@ -235,3 +235,25 @@ def test_what_are_no_whole_numbers(native, monkeypatch):
             gl._geometry(torch.zeros(4, 8, dtype=torch.bfloat16), "x", 1, (2, 8, 8), torch.zeros(2, dtype=dtype))
         with pytest.raises(TypeError, match="integers"):
             em._problem(ids, (2, 4, 8), None, torch.zeros(2, dtype=dtype), torch.bfloat16, ids.device)
+
+
+def test_forward_mode_tangents(native):
+    """No tangent is dropped: the calls that autograd may differentiate say that they have none to give, whether a gradient is required or not."""
+    from torch.autograd import forward_ad
+    pkg = load_package()
+    gl, em = pkg.bf16_grouped_linear, pkg.embedding
+    x, w, sizes = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(2, 8, 8, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    ids = torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        for required in (False, True):
+            dual = lambda t: forward_ad.make_dual(t.clone().requires_grad_(required), torch.ones_like(t))
+            for call in (lambda: gl.bf16_grouped_linear(dual(x), w, sizes), lambda: gl.bf16_grouped_linear(x, dual(w), sizes), lambda: em.embed(dual(x), ids),
+                         lambda: em.embed(dual(w), ids, adapter_indices=ids)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            em.embed(w, ids, forward_ad.make_dual(torch.ones(2), torch.ones(2)), adapter_indices=ids)
+        with pytest.raises(RuntimeError, match="GPU"):  # a level alone is no tangent
+            gl.bf16_grouped_linear(x, w, sizes)
+    with pytest.raises(RuntimeError, match="GPU"):
+        gl.bf16_grouped_linear(x, w, sizes)
