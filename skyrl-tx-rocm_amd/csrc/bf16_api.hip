@@ -321,8 +321,9 @@ int run_embedding(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
   if (overlaps(p->out, out_bytes, p->table, embedding_rows(p) * p->width * size) || overlaps_indices(p, p->out, out_bytes)) return MI355_W8A8_ERR_ALIAS;
   const EmbedArgs e = embed_args(p);
   const bool wide = p->width >= 16u / size;
-  const uint64_t threads = (uint64_t)p->n_tokens * embed_units(p->width, wide ? 16u / size : 1u);
-  const dim3 grid(blocks_of(threads)), block(256);
+  // (an axis of a launch has fewer than 2^32 threads, the widest rows of the most tokens 2^34 units)
+  const uint32_t blocks = blocks_of((uint64_t)p->n_tokens * embed_units(p->width, wide ? 16u / size : 1u)), planes = (blocks + kEmbedRowBlocks - 1u) / kEmbedRowBlocks;
+  const dim3 grid(planes > 1u ? kEmbedRowBlocks : blocks, planes), block(256);
   (void)hipGetLastError();
   if (size == 4u) {
     if (wide) hipLaunchKernelGGL((embed_rows_kernel<float, 4>), grid, block, 0, s, e);

@@ -87,10 +87,11 @@ template <> struct EmbedUnit<float, 1> {
   static __device__ inline void store(void* p, const float (&f)[1]) { *static_cast<float*>(p) = f[0]; }
 };
 
+constexpr uint32_t kEmbedRowBlocks = 1u << 20;  // workgroups along the first axis
 template <typename T, int V>
 __global__ __launch_bounds__(256) void embed_rows_kernel(EmbedArgs e) {
   const uint32_t units = embed_units(e.width, V);
-  const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+  const uint64_t i = ((uint64_t)blockIdx.y * kEmbedRowBlocks + blockIdx.x) * 256u + threadIdx.x;
   const uint32_t t = (uint32_t)(i / units), at = embed_start((uint32_t)(i - (uint64_t)t * units), e.width, V);
   if (t >= e.n) return;
   const uint32_t row = embed_row(e, t);

@@ -232,3 +232,16 @@ def test_the_widest_rows(em):
         want = torch.zeros(5, width, device=DEV).index_add_(0, ids, dy.float())
         grad = em.lookup_backward(dy, ids, (5, width))
         assert torch.equal(grad.float(), want) and torch.equal(em.lookup(grad, ids).float(), want[ids])
+
+
+@pytest.mark.parametrize("width,n", [(65536, (1 << 18) + 5), (16384, (1 << 16) + 3), (16384, 1 << 16), (65535, 20000)])
+def test_more_units_than_an_axis_of_a_launch(em, width, n):
+    """2^28 units (a plane of workgroups) and 2^32 (the threads of an axis) and more: 69 GB of float32 rows, compared 1 GB at a time."""
+    print(f"[case] {n} x {width}", flush=True)
+    g = gen(11)
+    table = torch.randn(3, width, generator=g, device=DEV)
+    ids = torch.randint(0, 3, (n,), generator=g, device=DEV)
+    out = em.lookup(table, ids)
+    step = (1 << 28) // width
+    for r in range(0, n, step):
+        assert torch.equal(out[r:r + step], table[ids[r:r + step]]), r
