@@ -13,6 +13,7 @@ or eager fallback.
 from __future__ import annotations
 
 import ctypes
+import threading
 import weakref
 
 import torch
@@ -161,12 +162,14 @@ class _LeafUse:
 
 
 _leaf_uses: weakref.WeakSet = weakref.WeakSet()
+_leaf_uses_lock = threading.RLock()  # (a set that grows in another thread cannot be walked)
 
 
 def note_leaves(*tensors: torch.Tensor) -> list:
     """Uses of those ``tensors`` that are leaves, for the graph to keep and ``check_capture`` to look at."""
     uses = [_LeafUse(t, _stream_ptr(t.device)) for t in tensors if t.requires_grad and t.is_leaf]
-    _leaf_uses.update(uses)
+    with _leaf_uses_lock:
+        _leaf_uses.update(uses)
     return uses
 
 
@@ -176,7 +179,9 @@ def check_capture(uses: list) -> None:
     capture, which ends the process when it is the default one."""
     if not uses or not torch.cuda.is_current_stream_capturing():
         return
-    for other in list(_leaf_uses):
+    with _leaf_uses_lock:
+        others = list(_leaf_uses)
+    for other in others:
         leaf = other.leaf()
         if leaf is not None and any(use.leaf() is leaf and use.stream != other.stream for use in uses):
             raise RuntimeError("a backward pass is captured while a graph of the same parameters, made on another stream, lives: "

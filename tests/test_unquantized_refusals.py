@@ -2,6 +2,9 @@
 never read, the Python entry points with CPU tensors."""
 
 import ctypes
+import sys
+import threading
+import time
 
 import pytest
 import torch
@@ -257,3 +260,35 @@ def test_forward_mode_tangents(native):
             gl.bf16_grouped_linear(x, w, sizes)
     with pytest.raises(RuntimeError, match="GPU"):
         gl.bf16_grouped_linear(x, w, sizes)
+
+
+def test_captures_beside_forwards_of_other_threads(native, monkeypatch):
+    """The rule is looked at while other threads record uses of their own leaves: neither waits for nor disturbs the other."""
+    from skyrl_tx_rocm_amd.kernels.rocm import bf16_grouped_linear as gl
+    monkeypatch.setattr(gl, "_stream_ptr", lambda device: 1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    kept, stop, failed = [], threading.Event(), []
+    mine = gl.note_leaves(torch.zeros(2, requires_grad=True))
+
+    def forwards():
+        while not stop.is_set():
+            kept.append(gl.note_leaves(*[torch.zeros(1, requires_grad=True) for _ in range(8)]))
+
+    workers = [threading.Thread(target=forwards) for _ in range(4)]
+    try:
+        for w in workers:
+            w.start()
+        end = time.monotonic() + 3.0
+        while time.monotonic() < end and not failed:
+            try:
+                gl.check_capture(mine)
+            except RuntimeError as e:
+                failed.append(e)
+    finally:
+        stop.set()
+        for w in workers:
+            w.join()
+        sys.setswitchinterval(interval)
+    assert not failed
