@@ -3,7 +3,7 @@
 // from one call for the next.  The steps take 14 to 16 us in Python beside the 7 us of the entry point's two launches, 4 to 6 here, and a decode
 // call's kernels 11 to 17: 2560 -> 6144, one row, 4 adapters of rank 64 23.3 -> 12.4 us a call; 12288 -> 4096, 16 rows, 4-bit codes 25.2 -> 18.1.
 //
-// Every function returns the output tensor (grouped_bwd: a tuple of two; grad_table: the table's bytes and the adapters), an int (the entry point's status, not OK), or None for anything out of the ordinary -- a wrong
+// Every function returns the output tensor (grouped_bwd: a tuple of two; grad_table: the table's bytes and the adapters; accumulation_stream: a number), an int (the entry point's status, not OK), or None for anything out of the ordinary -- a wrong
 // dtype, shape or device, a tensor subclass or mode, a tensor that is not contiguous, one that requires a gradient, a geometry that
 // the library refuses -- and the caller then goes the general way, which converts, differentiates or raises.
 #define PY_SSIZE_T_CLEAN
@@ -15,7 +15,9 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <vector>
@@ -407,6 +409,18 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   END_HANDLE_TH_ERRORS
 }
 
+// accumulation_stream(leaf) -> number of the stream (0: the default one) on which autograd adds to the leaf's gradient as long as one of its graphs
+// lives, or None where none does.
+PyObject* accumulation_stream(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  if (argc != 1 || !THPVariable_Check(argv[0])) { PyErr_SetString(PyExc_TypeError, "accumulation_stream takes a tensor"); return nullptr; }
+  HANDLE_TH_ERRORS
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(THPVariable_Unpack(argv[0]));
+  const auto stream = node ? node->stream() : std::nullopt;
+  if (!stream) Py_RETURN_NONE;
+  return PyLong_FromLongLong(stream->id());
+  END_HANDLE_TH_ERRORS
+}
+
 // A tensor of a gradient table: its values lie behind each other.
 bool whole_gradient(const at::Tensor& t, c10::Device device) {
   return t.layout() == at::kStrided && !t.is_nested() && t.device() == device && t.is_contiguous() && t.unsafeGetTensorImpl()->has_storage() &&
@@ -471,6 +485,8 @@ PyMethodDef methods[] = {
     {"grouped_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grouped_bwd)), METH_FASTCALL, "Their two gradients."},
     {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding)), METH_FASTCALL, "One lookup of embedding rows."},
     {"embedding_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embedding_bwd)), METH_FASTCALL, "The table's gradient."},
+    {"accumulation_stream", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(accumulation_stream)), METH_FASTCALL,
+     "The stream on which autograd adds to a leaf's gradient."},
     {"grad_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_table)), METH_FASTCALL, "The C table of gradients and their outputs."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mi355_w8a8_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -165,6 +165,10 @@ _leaf_uses: weakref.WeakSet = weakref.WeakSet()
 _leaf_uses_lock = threading.RLock()  # (a set that grows in another thread cannot be walked)
 
 
+_LIVING = ("a backward pass is captured while a graph of the same parameters, made on another stream, lives: "
+           "let go of its outputs (the last loss, say) first, or run it on a stream of its own, the capture's for one")
+
+
 def note_leaves(*tensors: torch.Tensor) -> list:
     """Uses of those ``tensors`` that are leaves, for the graph to keep and ``check_capture`` to look at."""
     uses = [_LeafUse(t, _stream_ptr(t.device)) for t in tensors if t.requires_grad and t.is_leaf]
@@ -174,18 +178,28 @@ def note_leaves(*tensors: torch.Tensor) -> list:
 
 
 def check_capture(uses: list) -> None:
-    """Refuse a backward pass under stream capture while another graph of the same leaves, made on another stream, lives.  Autograd
-    adds to a leaf's gradient on the stream of the leaf's first use among the living graphs: that stream would be drawn into the
-    capture, which ends the process when it is the default one."""
+    """Refuse a backward pass under stream capture that would draw the default stream into the capture, which ends the process.  Autograd adds to
+    a leaf's gradient on the stream on which the leaf was first used, by any operation, since a graph of it last lived throughout: the
+    host module knows that stream.  (Any other stream joins the capture and leaves it again: a warm-up on a side stream may live on.)
+    Without the module: refuse it beside a graph of the same leaves made here on another stream."""
     if not uses or not torch.cuda.is_current_stream_capturing():
+        return
+    unknown = []
+    for use in uses:
+        leaf = use.leaf()
+        host = _native.host() if leaf is not None and leaf.is_cuda else None
+        if host is None:
+            unknown.append(use)
+        elif host.accumulation_stream(leaf) == 0:
+            raise RuntimeError(_LIVING)
+    if not unknown:
         return
     with _leaf_uses_lock:
         others = list(_leaf_uses)
     for other in others:
         leaf = other.leaf()
-        if leaf is not None and any(use.leaf() is leaf and use.stream != other.stream for use in uses):
-            raise RuntimeError("a backward pass is captured while a graph of the same parameters, made on another stream, lives: "
-                               "let go of its outputs (the last loss, say) first, or run it on the capture's stream")
+        if leaf is not None and any(use.leaf() is leaf and use.stream != other.stream for use in unknown):
+            raise RuntimeError(_LIVING)
 
 
 def refuse_tangents(name: str, *tensors) -> None:

@@ -374,3 +374,92 @@ def test_infinities_beside_adapters_and_ids_out_of_range(lora, n_ad, bad):
     layer.lora_B.data[...] = bad
     other = layer(ids, index)
     assert torch.equal(other[~held], out[~held]) and torch.equal(other[~held], layer(ids)[~held]) and not torch.isfinite(other[held]).any()
+
+
+def test_streams_of_living_graphs(monkeypatch):
+    """The rule for captured backward passes with streams as they are and captures that are only claimed: no graph that lives, ours or another
+    operation's, may have brought the default stream to a leaf; any other stream may be there."""
+    gl = load_package().bf16_grouped_linear
+    x, w = torch.ones(8, 8, dtype=BF16, device=DEV), torch.ones(1, 8, 8, dtype=BF16, device=DEV).requires_grad_()
+    sizes = torch.tensor([8], dtype=torch.int32, device=DEV)
+    ours, theirs, side = lambda: gl.bf16_grouped_linear(x, w, sizes), lambda: (w * 2).sum(), torch.cuda.Stream()
+
+    def on_side(call):
+        with torch.cuda.stream(side):
+            return call()
+
+    def captured():
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                return torch.autograd.grad(gl.bf16_grouped_linear(x, w, sizes).sum(), w)
+
+    captured()
+    for call in (ours, theirs):
+        graph = call()
+        with pytest.raises(RuntimeError, match="lives"):
+            captured()
+        later = on_side(ours)
+        del graph
+        with pytest.raises(RuntimeError, match="lives"):  # (a graph of the side stream keeps what the default one's made)
+            captured()
+        del later
+        captured()
+        graph = on_side(call)
+        captured()
+        later = call()
+        captured()
+        del graph
+        captured()
+        del later
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kept", [False, True])
+def test_a_capture_beside_the_last_warm_up(lora, kept):
+    """A training step warmed up on a side stream and captured while its last output still lives, its gradients new or (kept) added to the ones that
+    are there; replays with other inputs give what an eager step of the same weights gives."""
+    g = torch.Generator(device=DEV).manual_seed(13)
+    embed = lora.LoRAEmbed(300, 64, embedding=torch.randn(300, 64, generator=g, device=DEV), max_lora_adapters=3, max_lora_rank=8)
+    fill(embed, g)
+    head = torch.randn(1, 64, 96, generator=g, device=DEV).to(BF16).requires_grad_()
+    ids = torch.randint(0, 300, (6, 20), generator=g, device=DEV)
+    index = torch.randint(0, 3, (6,), generator=g, device=DEV)
+    target = torch.randn(120, 96, generator=g, device=DEV).to(BF16)
+    sizes = torch.tensor([120], dtype=torch.int32, device=DEV)
+    gl = load_package().bf16_grouped_linear
+    leaves = [embed.lora_A, embed.lora_B, head]
+    twins = [t.detach().clone().requires_grad_() for t in leaves]
+
+    def step(a, b, w):
+        embed.lora_A, embed.lora_B = a, b
+        for p in (a, b, w):
+            if kept and p.grad is not None:
+                p.grad.zero_()
+            else:
+                p.grad = None
+        out = gl.bf16_grouped_linear(embed(ids, index).reshape(-1, 64), w, sizes)
+        out.backward(target)
+        return out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            last = step(*leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(*leaves)
+    grads = [p.grad for p in leaves]
+    assert last.grad_fn is not None
+    for turn in range(4):
+        ids.copy_(torch.randint(0, 300, ids.shape, generator=g, device=DEV))
+        index.copy_(torch.randint(0, 3, index.shape, generator=g, device=DEV))
+        target.copy_(torch.randn(target.shape, generator=g, device=DEV))
+        graph.replay()
+        got = [t.detach().clone() for t in (captured, *grads)]
+        want = step(*twins)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (want.detach(), *(p.grad for p in twins)))), turn
