@@ -73,7 +73,7 @@ EXPORTS = (
 PRIVATE_EXPORTS = (
     "mi355_w8a8_gq_bwd_workspace_bytes", "mi355_w8a8_gq_linear_bwd_v1",
     "mi355_w8a8_bf16_grouped_workspace_bytes", "mi355_w8a8_bf16_grouped_bwd_workspace_bytes", "mi355_w8a8_bf16_grouped_v1",
-    "mi355_w8a8_bf16_grouped_bwd_v1",
+    "mi355_w8a8_bf16_grouped_bwd_joint_tile", "mi355_w8a8_bf16_grouped_bwd_v1",
     "mi355_w8a8_embedding_v1", "mi355_w8a8_embedding_bwd_workspace_bytes", "mi355_w8a8_embedding_bwd_v1",
     "mi355_w8a8_grad_workspace_bytes", "mi355_w8a8_grad_norm_v1", "mi355_w8a8_grad_clip_v1",
 )
@@ -368,6 +368,8 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.mi355_w8a8_bf16_grouped_workspace_bytes.argtypes = (_u32,) * 5
     lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes.restype = _u64
     lib.mi355_w8a8_bf16_grouped_bwd_workspace_bytes.argtypes = (_u32,) * 7
+    lib.mi355_w8a8_bf16_grouped_bwd_joint_tile.restype = _u32
+    lib.mi355_w8a8_bf16_grouped_bwd_joint_tile.argtypes = (_u32,) * 5
     lib.mi355_w8a8_embedding_bwd_workspace_bytes.restype = _u64
     lib.mi355_w8a8_embedding_bwd_workspace_bytes.argtypes = (_u32,) * 5
     lib.mi355_w8a8_grad_workspace_bytes.restype = _u64

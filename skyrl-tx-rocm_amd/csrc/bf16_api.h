@@ -53,6 +53,8 @@ typedef struct mi355_w8a8_bf16_grouped_bwd_problem {
 uint64_t mi355_w8a8_bf16_grouped_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags);
 uint64_t mi355_w8a8_bf16_grouped_bwd_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags, uint32_t want_dx,
                                                      uint32_t want_dw);
+/* The tiles (a flag) of a backward call that computes both gradients in one launch, 0: each has its own. */
+uint32_t mi355_w8a8_bf16_grouped_bwd_joint_tile(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags);
 int mi355_w8a8_bf16_grouped_v1(const mi355_w8a8_bf16_grouped_problem* problem, void* stream);
 int mi355_w8a8_bf16_grouped_bwd_v1(const mi355_w8a8_bf16_grouped_bwd_problem* problem, void* stream);
 

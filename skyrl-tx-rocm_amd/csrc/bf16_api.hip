@@ -207,6 +207,16 @@ uint64_t grouped_bwd_workspace(uint32_t m, uint32_t k, uint32_t n, uint32_t grou
   return a > b ? a : b;
 }
 
+// What the two gradients' products are made of, but for the tensors.
+void bwd_sizes(uint32_t m, uint32_t k, uint32_t n, uint32_t groups, BgArgs& dx, BgArgs& dw) {
+  dx.m = dw.m = m;
+  dx.groups = dw.groups = groups;
+  dx.rows_ld = n; dx.cols_ld = n; dx.depth = n; dx.cols = k;
+  dx.b_group = (uint64_t)k * n;
+  dw.rows_ld = k; dw.cols_ld = n; dw.depth = 0; dw.cols = n; dw.rows = k;
+  dw.out_group = (uint64_t)k * n;
+}
+
 int run_grouped(const mi355_w8a8_bf16_grouped_problem* p, hipStream_t s) {
   if (!p) return MI355_W8A8_ERR_NULL;
   if (p->struct_size != sizeof(mi355_w8a8_bf16_grouped_problem)) return MI355_W8A8_ERR_STRUCT;
@@ -260,15 +270,10 @@ int run_grouped_bwd(const mi355_w8a8_bf16_grouped_bwd_problem* p, hipStream_t s)
   if (overlaps(p->dx, x_bytes, p->dw, dw_bytes) || overlaps(p->workspace, needed, p->dx, x_bytes) || overlaps(p->workspace, needed, p->dw, dw_bytes)) return MI355_W8A8_ERR_ALIAS;
   (void)hipGetLastError();
   BgArgs dx{}, dw{};
+  bwd_sizes(p->m, p->k, p->n, p->n_groups, dx, dw);
   dx.sizes = dw.sizes = p->group_sizes;
-  dx.m = dw.m = p->m;
-  dx.groups = dw.groups = p->n_groups;
   dx.a = static_cast<const uint16_t*>(p->dy); dx.b = static_cast<const uint16_t*>(p->weight); dx.out = p->dx;
-  dx.rows_ld = p->n; dx.cols_ld = p->n; dx.depth = p->n; dx.cols = p->k;
-  dx.b_group = (uint64_t)p->k * p->n;
   dw.a = static_cast<const uint16_t*>(p->x); dw.b = static_cast<const uint16_t*>(p->dy); dw.out = p->dw;
-  dw.rows_ld = p->k; dw.cols_ld = p->n; dw.depth = 0; dw.cols = p->n; dw.rows = p->k;
-  dw.out_group = (uint64_t)p->k * p->n;
   if (p->dx && p->dw) {
     const uint32_t tile = plan_grouped_both(dx, dw, f32 ? 4u : 2u, forced);
     if (tile) return f32 ? launch_both<true>(dx, dw, tile, s) : launch_both<false>(dx, dw, tile, s);
@@ -598,6 +603,12 @@ uint64_t mi355_w8a8_bf16_grouped_workspace_bytes(uint32_t m, uint32_t k, uint32_
 uint64_t mi355_w8a8_bf16_grouped_bwd_workspace_bytes(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags, uint32_t want_dx,
                                                      uint32_t want_dw) {
   return check_grouped_dims(m, k, n, n_groups) ? 0u : grouped_bwd_workspace(m, k, n, n_groups, flags & kGroupedTiles, want_dx, want_dw);
+}
+uint32_t mi355_w8a8_bf16_grouped_bwd_joint_tile(uint32_t m, uint32_t k, uint32_t n, uint32_t n_groups, uint32_t flags) {
+  if (check_grouped_dims(m, k, n, n_groups)) return 0;
+  BgArgs dx{}, dw{};
+  bwd_sizes(m, k, n, n_groups, dx, dw);
+  return plan_grouped_both(dx, dw, flags & MI355_W8A8_FLAG_BF16_GROUPED_DW_F32 ? 4u : 2u, flags & kGroupedTiles);
 }
 int mi355_w8a8_bf16_grouped_v1(const mi355_w8a8_bf16_grouped_problem* problem, void* stream) {
   return run_grouped(problem, static_cast<hipStream_t>(stream));

@@ -292,3 +292,17 @@ def test_captures_beside_forwards_of_other_threads(native, monkeypatch):
             w.join()
         sys.setswitchinterval(interval)
     assert not failed
+
+
+@pytest.mark.parametrize("rows,k,n,groups,tiles", [
+    (4051, 128, 120, 22, (16, 16)), (886, 168, 736, 13, (16, 16)), (1003, 712, 1096, 13, (8, 8)), (4096, 1024, 1024, 8, (8, 8)), (300, 64, 280, 28, (16, 16)),
+    (8000, 1576, 1744, 25, (8, 8)), (1, 8, 8, 1, (16, 16)), (70, 40, 136, 1024, (16, 16)),
+    (560, 1944, 2072, 115, (0, 0)), (32768, 768, 2048, 128, (0, 0)),  # bytes bound both
+    (9000, 8, 520, 1, (0, 0)), (1, 4096, 4096, 8, (0, 0)),            # parts of a contraction
+    (1, 12, 8, 1, (0, 0))])
+def test_sizes_whose_gradients_share_a_launch(native, rows, k, n, groups, tiles):
+    """The sizes that test_both_gradients_and_each of the GPU tests takes for this, and others; a bf16 dw and a float32 one."""
+    joint = native.load().mi355_w8a8_bf16_grouped_bwd_joint_tile
+    assert tuple(joint(rows, k, n, groups, f32) for f32 in (0, native.FLAG_BF16_GROUPED_DW_F32)) == tiles
+    if k % 8 == 0:
+        assert [joint(rows, k, n, groups, f) for f in (4, 8, 16)] == [4, 8, 16]
