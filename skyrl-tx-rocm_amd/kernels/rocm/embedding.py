@@ -63,9 +63,9 @@ def _problem(ids, shape, scale, adapter_indices, dtype, dev):
             raise TypeError("the scale of a plain table must be a number")
         scales = scale.detach().to(device=dev, dtype=torch.float32).reshape(-1).contiguous()
     elif scale is not None:
-        factor = float(scale)
+        factor = ctypes.c_float(scale).value
         if not math.isfinite(factor):
-            raise ValueError(f"scale must be finite, got {scale!r}")
+            raise ValueError(f"scale must be finite as float32, got {scale!r}")
     p = _native.EmbeddingProblem(ctypes.sizeof(_native.EmbeddingProblem),
                                  _TYPES[dtype] | (_native.FLAG_EMBEDDING_IDS64 if flat.dtype == torch.int64 else 0), n, vocab, width, adapters,
                                  factor, 0)

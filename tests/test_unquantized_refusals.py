@@ -306,3 +306,15 @@ def test_sizes_whose_gradients_share_a_launch(native, rows, k, n, groups, tiles)
     assert tuple(joint(rows, k, n, groups, f32) for f32 in (0, native.FLAG_BF16_GROUPED_DW_F32)) == tiles
     if k % 8 == 0:
         assert [joint(rows, k, n, groups, f) for f in (4, 8, 16)] == [4, 8, 16]
+
+
+def test_scales_that_float32_cannot_hold(native, monkeypatch):
+    """The product is float32: a larger scale would be an infinity there, also where the product itself could be held."""
+    from skyrl_tx_rocm_amd.kernels.rocm import embedding as em
+    monkeypatch.setattr(em, "_require_cuda", lambda t, name: None)
+    ids = torch.zeros(3, dtype=torch.int64)
+    of = lambda scale: em._problem(ids, (4, 8), scale, None, torch.bfloat16, ids.device)[0].scale
+    for bad in (float("inf"), float("nan"), 1e39, -3.5e38, 10 ** 40):
+        with pytest.raises(ValueError, match="finite"):
+            of(bad)
+    assert of(None) == 1.0 and of(-2) == -2.0 and of(torch.finfo(torch.float32).max) == torch.finfo(torch.float32).max and of(1e-50) == 0.0
