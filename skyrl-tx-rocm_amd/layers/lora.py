@@ -229,18 +229,27 @@ class LoRAEmbed(LoRAMixin):
             raise ValueError("adapter_indices must hold one entry per example (leading axis of ids)")
         n_ad = self.max_lora_adapters
         flat = ids.reshape(-1)
-        adapters = whole_numbers(adapter_indices, "adapter_indices", -1, n_ad).to(flat.device)
+        adapters = whole_numbers(adapter_indices, "adapter_indices", -1, n_ad).clamp(-1, n_ad).to(flat.device)
         adapters = adapters.repeat_interleave(flat.numel() // adapter_indices.shape[0])
-        # A token without an adapter or a row goes behind the last adapter's: there it has no part in the product and its gradients, which would
-        # carry infinities of B into its row and those of the row's gradient into B's.
-        held = (flat >= 0) & (flat < self.num_embeddings) & (adapters >= 0) & (adapters < n_ad)
-        adapters = torch.where(held, adapters, n_ad)
-        groups = min(n_ad + 1, MAX_GROUPS)
-        _, sizes, order, back, _ = w8.moe_dispatch(None, adapters, groups)
-        z = emb.embed(self.lora_A, flat.index_select(0, order), self.lora_scaling, adapter_indices=adapters.index_select(0, order))
-        delta = bf16_grouped_linear(_whole_units(z, 1), _whole_units(self.lora_B, 1), sizes[:n_ad])
-        delta = _Reorder.apply(delta, back, order)
-        if groups == n_ad:  # (no group is left for them: they are among the last adapter's)
+        # A token without an adapter or a row has no part in the product and its gradients: infinities of B would reach its row, those of its
+        # gradient B's.  It goes behind the last adapter's tokens, or its results are masked where nothing is sorted or no group is left for it.
+        # (16384 tokens x 2560, forward and backward, without this / with it: 8 adapters 313 / 335 us, one adapter 195 / 275.)
+        held = flat.clamp(0, self.num_embeddings - 1) == flat
+        behind = 1 < n_ad < MAX_GROUPS
+        if behind:
+            adapters = torch.where(held, adapters & 0x7fffffff, n_ad)  # (-1 becomes a group behind the last one, which the dispatch takes for that)
+        else:
+            held &= adapters.clamp(0, n_ad - 1) == adapters
+        order = back = None
+        sizes = torch.full((1,), flat.numel(), dtype=torch.int32, device=flat.device)
+        if n_ad > 1:
+            _, sizes, order, back, _ = w8.moe_dispatch(None, adapters, n_ad + behind)
+            flat, adapters, sizes = flat.index_select(0, order), adapters.index_select(0, order), sizes[:n_ad]
+        z = emb.embed(self.lora_A, flat, self.lora_scaling, adapter_indices=adapters)
+        delta = bf16_grouped_linear(_whole_units(z, 1), _whole_units(self.lora_B, 1), sizes)
+        if order is not None:
+            delta = _Reorder.apply(delta, back, order)
+        if not behind:
             delta = torch.where(held[:, None], delta, 0)
         return out + delta.reshape(out.shape)
 
