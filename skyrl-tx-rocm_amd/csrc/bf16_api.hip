@@ -467,8 +467,9 @@ int run_embedding_bwd(const mi355_w8a8_embedding_problem* p, hipStream_t s) {
 
 // ---- gradient norms and clipping -------------------------------------------------------------------------------------
 
-// values of a piece: as few as leave the chip 2048 workgroups, at most 64 KiB, so that the last of them end soon after the first; more where an
-// adapter's parts would be more than 4096 (every workgroup of the scaling reads them all)
+// values of a piece: as few as leave the chip 2048 workgroups, at most 64 KiB, so that the last of them end soon after the first; more where the
+// values of an adapter would make more than 4096 parts, since every workgroup of the scaling reads them all.  A tensor is one piece at least: thousands of
+// tensors are as many parts more, and what the workgroups read together grows with the square of that.
 uint32_t grad_piece_values(const mi355_w8a8_grad_tensor* t, uint32_t n, uint32_t adapters) {
   uint64_t values = 0;
   uint32_t most = 32768u, piece = 2048u;
