@@ -177,28 +177,37 @@ def note_leaves(*tensors: torch.Tensor) -> list:
     return uses
 
 
-def check_capture(uses: list) -> None:
+def _leaves_behind(node):
+    """The leaves whose gradients the backward of ``node`` leads to, through whatever operations."""
+    seen, todo = set(), [node]
+    while todo:
+        for behind, _ in todo.pop().next_functions:
+            if behind is None or behind in seen:
+                continue
+            seen.add(behind)
+            if behind.name() == "torch::autograd::AccumulateGrad":
+                yield behind.variable
+            else:
+                todo.append(behind)
+
+
+def check_capture(uses: list, node=None) -> None:
     """Refuse a backward pass under stream capture that would draw the default stream into the capture, which ends the process.  Autograd adds to
     a leaf's gradient on the stream on which the leaf was first used, by any operation, since a graph of it last lived throughout: the
-    host module knows that stream.  (Any other stream joins the capture and leaves it again: a warm-up on a side stream may live on.)
-    Without the module: refuse it beside a graph of the same leaves made here on another stream."""
-    if not uses or not torch.cuda.is_current_stream_capturing():
+    host module knows that stream, ``node`` (the backward's) the leaves.  (Any other stream joins the capture and leaves it again: a warm-up on a
+    side stream may live on.)  Without the module: refuse it beside a graph of the same leaves made here on another stream."""
+    if (not uses and node is None) or not torch.cuda.is_current_stream_capturing():
         return
-    unknown = []
-    for use in uses:
-        leaf = use.leaf()
-        host = _native.host() if leaf is not None and leaf.is_cuda else None
-        if host is None:
-            unknown.append(use)
-        elif host.accumulation_stream(leaf) == 0:
+    host = _native.host() if node is not None else None
+    if host is not None:
+        if any(host.accumulation_stream(leaf) == 0 for leaf in _leaves_behind(node) if leaf.is_cuda):
             raise RuntimeError(_LIVING)
-    if not unknown:
         return
     with _leaf_uses_lock:
         others = list(_leaf_uses)
     for other in others:
         leaf = other.leaf()
-        if leaf is not None and any(use.leaf() is leaf and use.stream != other.stream for use in unknown):
+        if leaf is not None and any(use.leaf() is leaf and use.stream != other.stream for use in uses):
             raise RuntimeError(_LIVING)
 
 
@@ -220,7 +229,7 @@ class _GroupedMatmulFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        check_capture(ctx.uses)
+        check_capture(ctx.uses, ctx)
         x, weight, group_sizes = ctx.saved_tensors
         dx, dw = grouped_matmul_backward(x, dy, weight, group_sizes, need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
         return dx, dw, None

@@ -141,7 +141,7 @@ class _LookupFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        check_capture(ctx.uses)
+        check_capture(ctx.uses, ctx)
         ids, adapter_indices, scales = ctx.saved_tensors
         grad = lookup_backward(d_out, ids, ctx.shape, ctx.scale if scales is None else scales, adapter_indices=adapter_indices)
         return grad, None, None, None

@@ -463,3 +463,31 @@ def test_a_capture_beside_the_last_warm_up(lora, kept):
         want = step(*twins)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, (want.detach(), *(p.grad for p in twins)))), turn
+
+
+def test_streams_of_living_graphs_behind_other_operations(lora, monkeypatch):
+    """The same rule for leaves that reach the products through other operations: a view, a sum, adapters whose rank is filled up, a graph in between."""
+    gl = load_package().bf16_grouped_linear
+    x, sizes = torch.ones(8, 8, dtype=BF16, device=DEV), torch.tensor([8], dtype=torch.int32, device=DEV)
+    w, v = (torch.ones(1, 8, 8, dtype=BF16, device=DEV).requires_grad_() for _ in range(2))
+    embed = lora.LoRAEmbed(20, 16, embedding=torch.ones(20, 16, device=DEV), max_lora_adapters=2, max_lora_rank=5)
+    embed.lora_B.requires_grad_()  # (B alone is trained)
+    ids, index = torch.arange(6, device=DEV), torch.zeros(6, dtype=torch.int32, device=DEV)
+    calls = [(w, lambda: gl.bf16_grouped_linear(x, w.transpose(1, 2), sizes)), (w, lambda: gl.bf16_grouped_linear(x, w + v, sizes)),
+             (v, lambda: gl.bf16_grouped_linear(x, w + v, sizes)), (w, lambda: gl.bf16_grouped_linear(gl.bf16_grouped_linear(x, w * 2, sizes), v, sizes)),
+             (embed.lora_B, lambda: embed(ids, index))]
+    for leaf, call in calls:
+
+        def captured():
+            with monkeypatch.context() as m:
+                m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+                with torch.cuda.stream(torch.cuda.Stream()):
+                    return torch.autograd.grad(call().sum(), leaf)
+
+        captured()
+        living = (leaf * 2).sum()
+        with pytest.raises(RuntimeError, match="lives"):
+            captured()
+        del living
+        captured()
+        torch.cuda.synchronize()
